@@ -457,6 +457,81 @@ int maple_quantize_rtn(const void* w, int w_dtype, int64_t rows, int64_t k, int6
 int maple_dequantize_rtn(const uint32_t* packed, const float* scales, const float* biases, int64_t rows, int64_t k,
                          int64_t group_size, float* out, void* stream);
 
+/* ---- speculative decoding: a tree of drafted tokens per step -------------
+ * No counterpart in the reference, which decodes one token per step.  A
+ * sequence's tree has `nodes` <= 64 nodes; parents[i] < i is node i's parent,
+ * -1 a root, anything below -1 padding.  Node 0 is the root: the last token
+ * that was drawn, not yet in the cache.  The nodes' K/V rows stand in the cache
+ * behind the sequence's seqlen positions, node j at slot seqlen + j.
+ *
+ * maple_tree_plan: mask[i] = bit i and the bits of node i's ancestors, depth[i]
+ * = their number (both [batch, nodes], contiguous; 0 for padding).  parents:
+ * element strides p_sb, p_sn.  A parent >= i sets bit 2 of *err; the node and
+ * what hangs on it become padding. */
+int maple_tree_plan(const int32_t* parents, int64_t batch, int64_t nodes, int64_t p_sb, int64_t p_sn, int64_t* mask,
+                    int32_t* depth, int* err, void* stream);
+
+/* GQA attention of every node over the cache and its branch:
+ *   out[b, i] = sum_t softmax_t(scale * q[b, i] . K[t]) V[t]
+ * over the cached positions t < seqlen[b] and the slots seqlen[b] + j with bit
+ * j of tree_mask[b, i] set (any mask will do, not ancestors only).  With
+ * window > 0 only keys whose position is above p_i - window count, a node's
+ * position being p_i = seqlen + popcount(mask_i) - 1.  A node with mask 0, and
+ * one that sees nothing, gets zeros.  What a node does not see never reaches
+ * its output, NaN and infinities included.
+ * q [batch, nodes, H, D] with D contiguous (element strides q_sb, q_sn, q_sh),
+ * out [batch, nodes, H, D] contiguous; caches [cache_batch, Hkv, max_len, D],
+ * (max_len, D) contiguous, cache row row_map[b] (b when NULL).  f32 or bf16,
+ * D in {64, 128, 256}; pointers and strides multiples of 16 bytes.  With nodes
+ * = 1 and mask 1 this is maple_decode_gqa_attn.  A length or cache row outside
+ * the cache sets bit 2 of *err (that sequence gets zeros); a bounded wait that
+ * gives up sets bit 1.  A row's result depends on no other sequence's length
+ * or contents.  The workspace needs no initial value and is free again when
+ * the call's work is done; concurrent calls need their own. */
+int64_t maple_tree_gqa_workspace_bytes(int64_t batch, int64_t nodes, int64_t num_heads, int64_t num_kv_heads,
+                                       int64_t head_dim, int64_t max_len, int x_dtype);
+int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, int64_t nodes, int64_t num_heads, int64_t q_sb,
+                        int64_t q_sn, int64_t q_sh, const void* k_cache, const void* v_cache, int64_t cache_batch,
+                        int64_t num_kv_heads, int64_t cache_sb, int64_t cache_sh, int64_t max_len, int64_t head_dim,
+                        const int64_t* seqlen, const int64_t* tree_mask, const int32_t* row_map, float scale,
+                        int64_t window, void* out, void* workspace, int64_t workspace_bytes, int* err, void* stream);
+
+/* Verification of the drafted tokens by rejection sampling from the caller's
+ * uniforms.  The target's distribution p at a node is maple_fused_sample's
+ * (top_k <= 64, temperature, top_p) over logits[b, node].  From node 0 the
+ * children of the current node are tried in index order: child c with token x
+ * is accepted where uniform[b, c] * q(x) < p(x), q = draft_probs[b, current]
+ * (all on x when NULL); else p = norm(max(p - q, 0)), unless nothing would be
+ * left, and unless `replacement` q loses x and is normalised again.  Where no
+ * child is left the next token is drawn from p by its inverse distribution at
+ * uniform[b, 0], ids in order of falling logits.  In 64 bits.
+ * logits [batch, nodes, vocab] (f32 or bf16, element strides l_sb, l_sn),
+ * draft_probs likewise; tokens, parents, uniform [batch, nodes] contiguous.
+ * path [batch, nodes]: the accepted nodes, node 0 first, then -1; n_path: their
+ * number (0 where node 0 is padding); out [batch, nodes]: the n_path tokens
+ * drawn, the last one from the target itself, then -1.  A drafted token outside
+ * the vocabulary is refused and sets bit 2 of *err, as a parent >= its node
+ * does.  NaN logits rank lowest.  Workspace as above, 16-byte aligned. */
+int64_t maple_verify_tree_workspace_bytes(int64_t batch, int64_t nodes, int64_t vocab, int64_t top_k);
+int maple_verify_tree(const void* logits, int x_dtype, int64_t batch, int64_t nodes, int64_t vocab, int64_t l_sb,
+                      int64_t l_sn, const int64_t* tokens, const int32_t* parents, const float* uniform,
+                      const void* draft_probs, int d_dtype, int64_t d_sb, int64_t d_sn, float temperature,
+                      float top_p, int64_t top_k, int replacement, int32_t* path, int32_t* n_path, int64_t* out,
+                      void* workspace, int64_t workspace_bytes, int* err, void* stream);
+
+/* Keeps the accepted rows: slot seqlen[b] + d takes slot seqlen[b] + path[b, d]
+ * for d < n_path[b], in K and V of every layer, in place; the other slots stay
+ * as they are.  path [batch, nodes] and n_path as maple_verify_tree writes
+ * them (rising along d).  k_caches / v_caches: host arrays of `layers` device
+ * pointers to [cache_batch, Hkv, max_len, D] caches of one geometry, 16-byte
+ * aligned.  A path that does not rise, or a slot or cache row outside the
+ * cache, moves nothing of that sequence and sets bit 2 of *err.  Two sequences
+ * on one cache row are not ordered. */
+int maple_commit_tree(void* const* k_caches, void* const* v_caches, int64_t layers, int x_dtype, int64_t batch,
+                      int64_t nodes, int64_t cache_batch, int64_t num_kv_heads, int64_t cache_sb, int64_t cache_sh,
+                      int64_t max_len, int64_t head_dim, const int64_t* seqlen, const int32_t* path,
+                      const int32_t* n_path, const int32_t* row_map, int* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,481 @@
+// Trees of drafted tokens (speculative decoding): the ancestors' masks, the
+// attention of every node over the cache and its branch, and the move of the
+// accepted rows.  No counterpart in the reference, which decodes one token per
+// step (generate.py:168-373).
+#include "bulk.cuh"
+#include "launch.cuh"
+#include "tree.cuh"
+
+namespace mb {
+
+// ------------------------------------------------------------------- plan --
+// mask_i = 2^i | mask_parent(i) by pointer doubling: after round r a node's
+// mask holds its ancestors within 2^r steps and `up` points 2^r steps up, so
+// six rounds cover 64 nodes.  One warp per sequence, nodes `lane` and
+// `lane + 32` in registers: no shared memory, no barrier; the 16 bytes per
+// node make the launch itself the bound (latency).
+__global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, int64_t sb, int64_t sn, int B, int N,
+                                                        unsigned long long* mask, int32_t* depth, int* err) {
+  const int lane = threadIdx.x & 31, b = blockIdx.x * 4 + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_trigger();
+  if (b >= B) return;
+  unsigned long long m[2];
+  int up[2];
+  bool off[2], wrong = false;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = lane + 32 * u;
+    const int par = i < N ? parents[(int64_t)b * sb + i * sn] : -2;
+    wrong |= i < N && par >= i;
+    off[u] = par < -1 || par >= i;
+    up[u] = (off[u] || par < 0) ? i : par;
+    m[u] = 1ull << i;
+  }
+#pragma unroll
+  for (int r = 0; r < 6; ++r) {
+    unsigned long long nm[2];
+    int nu[2];
+    bool no[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int a = up[u] & 31;
+      const bool high = up[u] >= 32;
+      const unsigned long long m0 = __shfl_sync(0xffffffffu, m[0], a), m1 = __shfl_sync(0xffffffffu, m[1], a);
+      const int u0 = __shfl_sync(0xffffffffu, up[0], a), u1 = __shfl_sync(0xffffffffu, up[1], a);
+      const int f0 = __shfl_sync(0xffffffffu, (int)off[0], a), f1 = __shfl_sync(0xffffffffu, (int)off[1], a);
+      nm[u] = m[u] | (high ? m1 : m0);
+      nu[u] = high ? u1 : u0;
+      no[u] = off[u] || (high ? f1 : f0);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) { m[u] = nm[u]; up[u] = nu[u]; off[u] = no[u]; }
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = lane + 32 * u;
+    if (i >= N) continue;
+    mask[(int64_t)b * N + i] = off[u] ? 0ull : m[u];
+    depth[(int64_t)b * N + i] = off[u] ? 0 : __popcll(m[u]) - 1;
+  }
+  if (wrong) atomicOr(err, kErrFlagBounds);
+}
+
+// -------------------------------------------------- attention, CUDA cores --
+// fp32 caches, and heads of 256: one CTA per (split of the keys, KV head and
+// tile of 32 query rows, sequence).  Row r of a KV head is node r / G, query
+// head h G + r % G, so the whole tree reads each K/V row once per 32 rows.
+// Tiles of 32 keys stand in shared memory as fp32; a warp owns four rows: its
+// lanes are the tile's keys for the scores (one K row per lane, row pitch D + 4
+// floats: 16-byte reads without bank conflicts) and the head's dimensions for
+// the products with V.  Softmax online: running maximum, sum and output in
+// fp32 registers.  A key that a row does not see never meets its sums (the
+// weight carries the sign as a mark), so NaN or infinities there stay out.
+constexpr int kSimtRows = 32;
+constexpr int kSimtKeys = 32;
+
+template <int XT, int D>
+__global__ void __launch_bounds__(256) tree_simt_kernel(TreeAttnParams p, int row_tiles) {
+  constexpr int U = D / 32, PITCH = D + 4;
+  constexpr int es = XT == kBF16 ? 2 : 4, EPC = 16 / es;
+  extern __shared__ __align__(16) float sm[];
+  float* sq = sm;                        // [32][D]
+  float* sk = sq + kSimtRows * D;        // [32][PITCH]
+  float* sv = sk + kSimtKeys * PITCH;    // [32][D]
+  __shared__ unsigned long long s_mask[kTreeMaxNodes];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int sp = blockIdx.x, h = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles, b = blockIdx.z;
+  const float ninf = __int_as_float(0xff800000);
+  pdl_wait();
+  pdl_trigger();
+  if (tid < kTreeMaxNodes) {
+    const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
+    s_mask[tid] = tid < p.N ? p.mask[(int64_t)b * p.N + tid] & keep : 0ull;
+  }
+  __syncthreads();
+  unsigned long long used = 0;
+  for (int i = 0; i < p.N; ++i) used |= s_mask[i] | (s_mask[i] ? 1ull << i : 0ull);
+  const TreeRange rg = tree_range(p, b, used);
+  if (rg.bad && tid == 0) atomicOr(p.err, kErrFlagBounds);
+  int k0, k1;
+  tree_split(rg.lo, rg.hi, kSimtKeys, p.NS, sp, k0, k1);
+  if (sp > 0 && k0 >= k1) return;  // nothing here; split 0 always answers
+
+  const int rows = p.N * p.G, r0 = rt * kSimtRows + warp * 4;
+  // q rows, zero past the last one
+  for (int c = tid; c < kSimtRows * D / EPC; c += 256) {
+    const int r = c / (D / EPC), cc = c % (D / EPC), gr = rt * kSimtRows + r;
+    float f[EPC];
+    if (gr < rows) {
+      const int i = gr / p.G, g = gr - i * p.G;
+      widen_u4<XT>(ld_u4(static_cast<const char*>(p.q) +
+                         (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + g) * p.q_sh + cc * EPC) * es), f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) f[e] = 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) sq[r * D + cc * EPC + e] = f[e];
+  }
+  const char* kb = static_cast<const char*>(p.kc) + (rg.cb * p.c_sb + h * p.c_sh) * es;
+  const char* vb = static_cast<const char*>(p.vc) + (rg.cb * p.c_sb + h * p.c_sh) * es;
+
+  unsigned long long mine[4];
+  int depth[4];
+  float m[4], l[4], acc[4][U];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    const int r = r0 + a;
+    mine[a] = r < rows ? s_mask[r / p.G] : 0ull;
+    depth[a] = __popcll(mine[a]) - 1;
+    m[a] = ninf;
+    l[a] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc[a][u] = 0.0f;
+  }
+  for (int t0 = k0; t0 < k1; t0 += kSimtKeys) {
+    const int n = min(kSimtKeys, k1 - t0);
+    __syncthreads();  // the last tile's readers are done
+    for (int c = tid; c < kSimtKeys * D / EPC; c += 256) {
+      const int r = c / (D / EPC), cc = c % (D / EPC);
+      float f[EPC], g[EPC];
+      if (r < n) {
+        widen_u4<XT>(ld_u4(kb + ((int64_t)(t0 + r) * D + cc * EPC) * es), f);
+        widen_u4<XT>(ld_u4(vb + ((int64_t)(t0 + r) * D + cc * EPC) * es), g);
+      } else {
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) f[e] = g[e] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) {
+        sk[r * PITCH + cc * EPC + e] = f[e];
+        sv[r * D + cc * EPC + e] = g[e];
+      }
+    }
+    __syncthreads();
+    // scores: this lane's key against the warp's four rows
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int d = 0; d < D; d += 4) {
+      const float4 kk = *reinterpret_cast<const float4*>(&sk[lane * PITCH + d]);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const float4 qq = *reinterpret_cast<const float4*>(&sq[(warp * 4 + a) * D + d]);
+        s[a] = fmaf(qq.x, kk.x, s[a]);
+        s[a] = fmaf(qq.y, kk.y, s[a]);
+        s[a] = fmaf(qq.z, kk.z, s[a]);
+        s[a] = fmaf(qq.w, kk.w, s[a]);
+      }
+    }
+    const int t = t0 + lane;
+    const int j = t - rg.s;  // node of this key, below 0: a cached position
+    const int kpos = j < 0 ? t : (j < kTreeMaxNodes ? rg.s + __popcll(s_mask[j]) - 1 : 0);
+    float w[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      bool vis = lane < n && mine[a] != 0 && (j < 0 || ((mine[a] >> (j & 63)) & 1));
+      if (p.window > 0) vis = vis && kpos > rg.s + depth[a] - p.window;
+      const float x = vis ? s[a] * p.scale : ninf;
+      const float mt = fmaxf(m[a], warp_max(x));
+      const float base = mt == ninf ? 0.0f : mt;
+      w[a] = vis ? mexp(x - base) : 0.0f;
+      const float fix = mexp(m[a] - base);
+      l[a] = fmaf(l[a], fix, warp_butterfly_sum(w[a]));
+      m[a] = mt;
+#pragma unroll
+      for (int u = 0; u < U; ++u) acc[a][u] *= fix;
+      if (!vis) w[a] = -1.0f;  // mark: not this row's
+    }
+    for (int kx = 0; kx < n; ++kx) {
+      float vv[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) vv[u] = sv[kx * D + lane + 32 * u];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const float wk = __shfl_sync(0xffffffffu, w[a], kx);
+        if (!(wk < 0.0f)) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) acc[a][u] = fmaf(wk, vv[u], acc[a][u]);
+        }
+      }
+    }
+  }
+  const bool alone = tree_splits_used(rg.lo, rg.hi, kSimtKeys, p.NS) <= 1;
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    const int r = r0 + a;
+    if (r >= rows) continue;
+    if (alone) {
+      const int i = r / p.G, g = r - i * p.G;
+      const int64_t o = (((int64_t)b * p.N + i) * p.H + h * p.G + g) * D;
+#pragma unroll
+      for (int u = 0; u < U; ++u) store_f<XT>(p.out, o + lane + 32 * u, l[a] == 0.0f ? 0.0f : acc[a][u] / l[a]);
+    } else {
+      const int64_t R = ((int64_t)b * p.Hkv + h) * rows + r;
+      float* ac = p.ws_acc + (R * p.NS + sp) * D;
+#pragma unroll
+      for (int u = 0; u < U; ++u) ac[lane + 32 * u] = acc[a][u];
+      if (lane == 0) {
+        p.ws_ml[(R * p.NS + sp) * 2] = m[a];
+        p.ws_ml[(R * p.NS + sp) * 2 + 1] = l[a];
+      }
+    }
+  }
+}
+
+// Joins the splits of each row: M = max m_j, out = sum e^(m_j - M) acc_j / sum
+// e^(m_j - M) l_j, in split order.  A warp per row, its lanes the dimensions;
+// the partials were just written and come from L2.
+template <int XT, int D>
+__global__ void __launch_bounds__(256) tree_merge_kernel(TreeAttnParams p, int tile) {
+  constexpr int U = D / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = p.N * p.G, hr = blockIdx.x * 8 + warp, b = blockIdx.y;
+  pdl_wait();
+  pdl_trigger();
+  const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
+  unsigned long long used = 0;
+  for (int i = lane; i < p.N; i += 32) {
+    const unsigned long long mi = p.mask[(int64_t)b * p.N + i] & keep;
+    used |= mi | (mi ? 1ull << i : 0ull);
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) used |= __shfl_xor_sync(0xffffffffu, used, o);
+  const TreeRange rg = tree_range(p, b, used);
+  const int ns = tree_splits_used(rg.lo, rg.hi, tile, p.NS);
+  if (hr >= p.Hkv * rows || ns <= 1) return;  // one split wrote its output itself
+  const int h = hr / rows, r = hr - h * rows;
+  const int64_t R = (int64_t)b * p.Hkv * rows + hr;
+  const float ninf = __int_as_float(0xff800000);
+  const float* ml = p.ws_ml + R * p.NS * 2;
+  const float* ac = p.ws_acc + R * p.NS * D;
+  float mj[2], lj[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int j = lane + 32 * u;
+    mj[u] = j < ns ? __ldcg(ml + 2 * j) : ninf;
+    lj[u] = j < ns ? __ldcg(ml + 2 * j + 1) : 0.0f;
+  }
+  const float M = warp_max(fmaxf(mj[0], mj[1]));
+  const float base = M == ninf ? 0.0f : M;
+  float wj[2] = {mexp(mj[0] - base), mexp(mj[1] - base)};
+  float den = 0.0f, num[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) num[u] = 0.0f;
+  constexpr int kB = 8;
+  for (int j0 = 0; j0 < ns; j0 += kB) {
+    float a[kB][U];
+#pragma unroll
+    for (int i = 0; i < kB; ++i)
+      if (j0 + i < ns) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) a[i][u] = __ldcg(ac + (int64_t)(j0 + i) * D + lane + 32 * u);
+      }
+#pragma unroll
+    for (int i = 0; i < kB; ++i)
+      if (j0 + i < ns) {
+        const int j = j0 + i;
+        const float w = __shfl_sync(0xffffffffu, j < 32 ? wj[0] : wj[1], j & 31);
+        const float lw = __shfl_sync(0xffffffffu, j < 32 ? lj[0] : lj[1], j & 31);
+        if (w == 0.0f && lw == 0.0f) continue;  // a split that this row sees nothing of
+        den = fmaf(w, lw, den);
+#pragma unroll
+        for (int u = 0; u < U; ++u) num[u] = fmaf(w, a[i][u], num[u]);
+      }
+  }
+  const int i = r / p.G, g = r - i * p.G;
+  const int64_t o = (((int64_t)b * p.N + i) * p.H + h * p.G + g) * D;
+#pragma unroll
+  for (int u = 0; u < U; ++u) store_f<XT>(p.out, o + lane + 32 * u, den == 0.0f ? 0.0f : num[u] / den);
+}
+
+// ----------------------------------------------------------------- commit --
+// cache[row, :, seqlen + d] <- cache[row, :, seqlen + path[d]] for d < n_path,
+// every layer's K and V in one launch.  path rises (path[d] >= d), so one
+// thread that walks d upwards with its own 16-byte column may move in place:
+// what it overwrites at d it has read already.  Batches of eight loads keep the
+// column's reads in flight; bound by latency at the sizes of a draft.
+constexpr int kCommitLayers = 128;
+
+struct CommitParams {
+  void* ptr[2 * kCommitLayers];  // K and V of each layer
+  const int64_t* seqlen;
+  const int32_t* path;
+  const int32_t* n_path;
+  const int32_t* row_map;
+  int* err;
+  int64_t sb, sh, sbh;  // cache strides in 16-byte units (batch, KV head); sbh: units per row
+  int B, N, Hkv, Bc, T, nptr;
+};
+
+__global__ void __launch_bounds__(256) commit_kernel(const __grid_constant__ CommitParams p) {
+  __shared__ int s_path[kTreeMaxNodes];
+  __shared__ int s_bad;
+  const int tid = threadIdx.x, b = blockIdx.y;
+  pdl_wait();
+  pdl_trigger();
+  const int n = p.n_path[b];
+  const int64_t s = p.seqlen[b];
+  const int cb = p.row_map != nullptr ? p.row_map[b] : b;
+  if (tid == 0) s_bad = 0;
+  __syncthreads();
+  if (n <= 0) return;
+  const bool ok = n <= p.N && s >= 0 && s <= p.T && cb >= 0 && cb < p.Bc;
+  if (ok && tid < n) {
+    const int d = tid, x = p.path[(int64_t)b * p.N + d];
+    const int before = d > 0 ? p.path[(int64_t)b * p.N + d - 1] : -1;
+    if (x <= before || x >= p.N || s + x >= p.T) s_bad = 1;
+    s_path[d] = x;
+  }
+  __syncthreads();
+  if (!ok || s_bad) {  // a path that does not rise or leaves the cache: nothing moves
+    if (tid == 0) atomicOr(p.err, kErrFlagBounds);
+    return;
+  }
+  const int64_t cols = (int64_t)p.nptr * p.Hkv * p.sbh;
+  for (int64_t c = (int64_t)blockIdx.x * 256 + tid; c < cols; c += (int64_t)gridDim.x * 256) {
+    const int64_t lane = c % p.sbh, hl = c / p.sbh;
+    uint4* base = static_cast<uint4*>(p.ptr[hl / p.Hkv]) + cb * p.sb + (hl % p.Hkv) * p.sh + s * p.sbh + lane;
+    for (int d0 = 0; d0 < n; d0 += 8) {
+      uint4 r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (d0 + e < n && s_path[d0 + e] != d0 + e) r[e] = base[s_path[d0 + e] * p.sbh];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (d0 + e < n && s_path[d0 + e] != d0 + e) base[(d0 + e) * p.sbh] = r[e];
+    }
+  }
+}
+
+// How many splits a row's keys are cut into: enough CTAs for two per SM at
+// full length, no more than the join can hold.
+inline int tree_simt_splits(int64_t ctas, int64_t max_len) {
+  const int64_t want = (2 * 148 + ctas - 1) / ctas, most = (max_len + kSimtKeys - 1) / kSimtKeys;
+  const int64_t ns = want < most ? want : most;
+  return (int)(ns < 1 ? 1 : ns > kTreeMaxSplits ? kTreeMaxSplits : ns);
+}
+
+inline int tree_splits(int64_t batch, int64_t nodes, int64_t num_heads, int64_t num_kv_heads, int64_t max_len) {
+  const int64_t tiles = (nodes * (num_heads / num_kv_heads) + kSimtRows - 1) / kSimtRows;
+  return tree_simt_splits(batch * num_kv_heads * tiles, max_len);
+}
+
+}  // namespace mb
+
+using namespace mb;
+
+extern "C" int maple_tree_plan(const int32_t* parents, int64_t batch, int64_t nodes, int64_t p_sb, int64_t p_sn,
+                               int64_t* mask, int32_t* depth, int* err, void* stream) {
+  if (batch < 0 || nodes <= 0 || nodes > kTreeMaxNodes || batch > (1LL << 30)) return kErrShape;
+  if (batch == 0) return kOk;
+  if (!parents || !mask || !depth || !err) return kErrShape;
+  const cudaError_t e = launch_k(tree_plan_kernel, dim3((unsigned)((batch + 3) / 4)), dim3(128), 0,
+                                 static_cast<cudaStream_t>(stream), parents, p_sb, p_sn, (int)batch, (int)nodes,
+                                 reinterpret_cast<unsigned long long*>(mask), depth, err);
+  return e == cudaSuccess ? kOk : kErrCuda;
+}
+
+extern "C" int64_t maple_tree_gqa_workspace_bytes(int64_t batch, int64_t nodes, int64_t num_heads,
+                                                  int64_t num_kv_heads, int64_t head_dim, int64_t max_len,
+                                                  int x_dtype) {
+  (void)x_dtype;
+  if (batch <= 0 || nodes <= 0 || nodes > kTreeMaxNodes || num_heads <= 0 || num_kv_heads <= 0 ||
+      num_heads % num_kv_heads || head_dim <= 0 || max_len <= 0)
+    return -1;
+  const int64_t ns = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len);
+  return ns <= 1 ? 0 : batch * num_heads * nodes * ns * (head_dim + 2) * 4;
+}
+
+extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, int64_t nodes, int64_t num_heads,
+                                   int64_t q_sb, int64_t q_sn, int64_t q_sh, const void* k_cache, const void* v_cache,
+                                   int64_t cache_batch, int64_t num_kv_heads, int64_t cache_sb, int64_t cache_sh,
+                                   int64_t max_len, int64_t head_dim, const int64_t* seqlen, const int64_t* tree_mask,
+                                   const int32_t* row_map, float scale, int64_t window, void* out, void* workspace,
+                                   int64_t workspace_bytes, int* err, void* stream) {
+  if (batch < 0 || nodes <= 0 || nodes > kTreeMaxNodes || num_heads <= 0 || num_kv_heads <= 0 || max_len <= 0 ||
+      cache_batch < 0 || window < 0)
+    return kErrShape;
+  if (batch == 0) return kOk;
+  if (x_dtype != kF32 && x_dtype != kBF16) return kErrDtype;
+  if (num_heads % num_kv_heads != 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return kErrShape;
+  if (!q || !k_cache || !v_cache || !seqlen || !tree_mask || !out || !err || batch > 65535 || cache_batch < 1 ||
+      num_heads > 65535 || max_len > (1LL << 30) || cache_batch > (1LL << 30))
+    return kErrShape;
+  const int es = x_dtype == kBF16 ? 2 : 4;
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
+        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
+      (((q_sb | q_sn | q_sh | cache_sb | cache_sh) * es) & 15))
+    return kErrAlign;
+  TreeAttnParams p{};
+  p.q = q; p.kc = k_cache; p.vc = v_cache; p.seqlen = seqlen; p.row_map = row_map; p.out = out; p.err = err;
+  p.mask = reinterpret_cast<const unsigned long long*>(tree_mask);
+  p.q_sb = q_sb; p.q_sn = q_sn; p.q_sh = q_sh; p.c_sb = cache_sb; p.c_sh = cache_sh;
+  p.B = (int)batch; p.N = (int)nodes; p.H = (int)num_heads; p.Hkv = (int)num_kv_heads;
+  p.G = (int)(num_heads / num_kv_heads); p.Bc = (int)cache_batch; p.T = (int)max_len;
+  p.window = (int)(window > max_len ? 0 : window);  // a window past the cache hides nothing
+  p.scale = scale;
+  const int64_t rows = (int64_t)p.N * p.G, tiles = (rows + kSimtRows - 1) / kSimtRows;
+  if (num_kv_heads * tiles > 65535) return kErrShape;
+  p.NS = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len);
+  const int64_t need = p.NS <= 1 ? 0 : batch * num_heads * nodes * p.NS * (head_dim + 2) * 4;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return kErrWorkspace;
+  p.ws_acc = static_cast<float*>(workspace);
+  p.ws_ml = p.ws_acc ? p.ws_acc + batch * num_heads * nodes * p.NS * head_dim : nullptr;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+#define MB_TREE(XT, DD)                                                                                              \
+  do {                                                                                                               \
+    const size_t smem = (size_t)(kSimtRows * DD + kSimtKeys * (DD + 4) + kSimtKeys * DD) * 4;                        \
+    e = cudaFuncSetAttribute(tree_simt_kernel<XT, DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);      \
+    if (e == cudaSuccess)                                                                                            \
+      e = launch_k(tree_simt_kernel<XT, DD>, dim3((unsigned)p.NS, (unsigned)(num_kv_heads * tiles), (unsigned)batch), \
+                   dim3(256), smem, st, p, (int)tiles);                                                              \
+    if (e == cudaSuccess && p.NS > 1)                                                                                \
+      e = launch_k(tree_merge_kernel<XT, DD>,                                                                        \
+                   dim3((unsigned)((num_kv_heads * rows + 7) / 8), (unsigned)batch), dim3(256), 0, st, p, kSimtKeys); \
+  } while (0)
+  if (x_dtype == kBF16) {
+    if (head_dim == 64) MB_TREE(kBF16, 64); else if (head_dim == 128) MB_TREE(kBF16, 128); else MB_TREE(kBF16, 256);
+  } else {
+    if (head_dim == 64) MB_TREE(kF32, 64); else if (head_dim == 128) MB_TREE(kF32, 128); else MB_TREE(kF32, 256);
+  }
+#undef MB_TREE
+  return e == cudaSuccess ? kOk : kErrCuda;
+}
+
+extern "C" int maple_commit_tree(void* const* k_caches, void* const* v_caches, int64_t layers, int x_dtype,
+                                 int64_t batch, int64_t nodes, int64_t cache_batch, int64_t num_kv_heads,
+                                 int64_t cache_sb, int64_t cache_sh, int64_t max_len, int64_t head_dim,
+                                 const int64_t* seqlen, const int32_t* path, const int32_t* n_path,
+                                 const int32_t* row_map, int* err, void* stream) {
+  if (layers < 0 || batch < 0 || nodes <= 0 || nodes > kTreeMaxNodes || num_kv_heads <= 0 || max_len <= 0 ||
+      head_dim <= 0 || batch > 65535 || cache_batch < 0 || cache_batch > (1LL << 30) || max_len > (1LL << 30))
+    return kErrShape;
+  if (layers == 0 || batch == 0) return kOk;
+  if (x_dtype != kF32 && x_dtype != kBF16) return kErrDtype;
+  if (!k_caches || !v_caches || !seqlen || !path || !n_path || !err || cache_batch < 1) return kErrShape;
+  const int64_t epu = x_dtype == kBF16 ? 8 : 4;  // elements per 16 bytes
+  if (head_dim % epu || cache_sb % epu || cache_sh % epu) return kErrAlign;
+  for (int64_t i = 0; i < layers; ++i) {
+    if (!k_caches[i] || !v_caches[i]) return kErrShape;
+    if ((reinterpret_cast<uintptr_t>(k_caches[i]) | reinterpret_cast<uintptr_t>(v_caches[i])) & 15) return kErrAlign;
+  }
+  for (int64_t l0 = 0; l0 < layers; l0 += kCommitLayers) {
+    const int64_t nl = layers - l0 < kCommitLayers ? layers - l0 : kCommitLayers;
+    CommitParams p{};
+    for (int64_t i = 0; i < nl; ++i) {
+      p.ptr[2 * i] = k_caches[l0 + i];
+      p.ptr[2 * i + 1] = v_caches[l0 + i];
+    }
+    p.seqlen = seqlen; p.path = path; p.n_path = n_path; p.row_map = row_map; p.err = err;
+    p.sb = cache_sb / epu; p.sh = cache_sh / epu; p.sbh = head_dim / epu;
+    p.B = (int)batch; p.N = (int)nodes; p.Hkv = (int)num_kv_heads; p.Bc = (int)cache_batch; p.T = (int)max_len;
+    p.nptr = (int)(2 * nl);
+    const int64_t cols = (int64_t)p.nptr * num_kv_heads * p.sbh, blocks = (cols + 255) / 256;
+    const cudaError_t e = launch_k(commit_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024), (unsigned)batch),
+                                   dim3(256), 0, static_cast<cudaStream_t>(stream), p);
+    if (e != cudaSuccess) return kErrCuda;
+  }
+  return kOk;
+}

@@ -1,0 +1,84 @@
+// Attention over a KV cache for trees of drafted tokens: what the CUDA-core
+// and the tcgen05 kernels share (arguments, visibility, the split of a row's
+// keys and the layout of the partial results).
+//
+// A sequence has s = seqlen[b] cached positions and N <= 64 drafted nodes
+// whose K/V rows stand behind them, node j at slot s + j.  mask_i has bit j
+// set where node i sees node j (its ancestors and itself); the node's position
+// is p_i = s + popcount(mask_i) - 1.  Node i sees key t < s, and key s + j
+// where bit j is set; with a window W > 0 only keys whose position is above
+// p_i - W.  mask_i = 0 marks padding: its output is zero.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace mb {
+
+constexpr int kTreeMaxNodes = 64;
+constexpr int kTreeMaxSplits = 64;
+
+struct TreeAttnParams {
+  const void* q;              // [B, N, H, D], D contiguous
+  const void* kc;             // [Bc, Hkv, T, D]
+  const void* vc;
+  const int64_t* seqlen;      // [B]
+  const unsigned long long* mask;  // [B, N]
+  const int32_t* row_map;     // [B] cache row, or null: b
+  void* out;                  // [B, N, H, D] contiguous
+  float* ws_acc;              // [B * Hkv * N * G, NS, D] unnormalised partial sums
+  float* ws_ml;               // [B * Hkv * N * G, NS, 2] maximum, sum of weights
+  int* err;
+  int64_t q_sb, q_sn, q_sh, c_sb, c_sh;
+  int B, N, H, Hkv, G, Bc, T, NS, window;
+  float scale;
+};
+
+// The keys of sequence b: [lo, hi) of slots, hi = s + (nodes in use); every
+// node's visible keys are inside.  Empty (lo = hi) where the sequence has no
+// node or its length or cache row is not in the cache.
+struct TreeRange {
+  int s, lo, hi, cb;
+  bool bad;
+};
+
+__device__ __forceinline__ TreeRange tree_range(const TreeAttnParams& p, int b, unsigned long long used) {
+  TreeRange r;
+  const int64_t s = p.seqlen[b];
+  int cb = b;
+  if (p.row_map != nullptr) cb = p.row_map[b];
+  r.cb = cb;
+  const int n = 64 - __clzll((long long)used);  // nodes up to the last one that is real or seen
+  r.bad = s < 0 || s > p.T || cb < 0 || cb >= p.Bc || s + n > p.T;
+  if (r.bad || n == 0) {
+    r.bad = r.bad && n > 0;
+    r.s = r.lo = r.hi = 0;
+    return r;
+  }
+  r.s = (int)s;
+  r.hi = r.s + n;
+  r.lo = p.window > 0 ? max(0, r.s + 1 - p.window) : 0;  // depth 0 reaches back the furthest
+  return r;
+}
+
+// Split sp of NS: tiles [t0, t1) of `tile` keys each, counted from lo.  The
+// number of splits is fixed by the shapes, the split's length by the row's own
+// length: a row's result depends on no other row.
+__device__ __forceinline__ void tree_split(int lo, int hi, int tile, int ns, int sp, int& k0, int& k1) {
+  const int tiles = (hi - lo + tile - 1) / tile;
+  const int per = (tiles + ns - 1) / ns;
+  k0 = min(hi, lo + sp * per * tile);
+  k1 = min(hi, k0 + per * tile);
+}
+
+// How many splits hold keys.
+__device__ __forceinline__ int tree_splits_used(int lo, int hi, int tile, int ns) {
+  const int tiles = (hi - lo + tile - 1) / tile;
+  if (tiles == 0) return 0;
+  const int per = (tiles + ns - 1) / ns;
+  return (tiles + per - 1) / per;
+}
+
+}  // namespace mb

@@ -8,6 +8,8 @@ runs unchanged.  All arithmetic happens in ``libmaple_b200.so``.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from maple_flash_dgx_spark_b200 import _lib
@@ -924,3 +926,235 @@ def batched_sampler_workspace(vocab: int, top_k: int, batch: int, device):
     """Sampler scratch for up to ``batch`` rows.  Reference kernels/sampler.py:219."""
     n = lib().maple_fused_sample_workspace_bytes(batch, vocab, top_k)
     return (torch.zeros(n, dtype=torch.uint8, device=device),)
+
+
+# ---------------------------------------------------- speculative decoding --
+MAX_TREE_NODES = 64
+
+
+def _one_device(op, first, *tensors):
+    """Every tensor on the first one's GPU; returns it."""
+    require_cuda(op, first, *tensors)
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{op}: tensors on {first.device} and {t.device}.")
+    return first.device
+
+
+def _launch(fn, op, device, *args):
+    """``check(fn(*args, stream))`` with ``device`` current."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, stream_ptr(device)), op)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream_ptr(device)), op)
+
+
+def _as(t, dtype):
+    return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
+def _tree_shape(op, t, what):
+    if t.ndim < 2 or not 1 <= t.shape[1] <= MAX_TREE_NODES:
+        raise ValueError(f"{op}: {what} must be [B, N, ...] with 1 to {MAX_TREE_NODES} nodes, got {tuple(t.shape)}.")
+    return int(t.shape[0]), int(t.shape[1])
+
+
+class TreePlan:
+    """The trees of one step, shared by every layer's attention: ``parents``
+    int32, ``mask`` int64 (bit j: the node sees node j) and ``depth`` int32
+    (the node's ancestors), all ``[B, N]``."""
+
+    def __init__(self, parents: torch.Tensor, mask: torch.Tensor, depth: torch.Tensor):
+        self.parents = parents
+        self.mask = mask
+        self.depth = depth
+
+
+def tree_plan(parents: torch.Tensor) -> TreePlan:
+    """Ancestor masks and depths of ``B`` trees of ``N <= 64`` drafted nodes.
+
+    ``parents`` ``[B, N]``: ``parents[b, i] < i`` is node i's parent, -1 a root
+    (node 0: the last drawn token), less than -1 padding.  A parent that is not
+    before its node sets the device error word; that branch becomes padding."""
+    op = "tree_plan"
+    dev = _one_device(op, parents)
+    B, N = _tree_shape(op, parents, "parents")
+    if parents.ndim != 2:
+        raise ValueError(f"{op}: parents must be [B, N], got {tuple(parents.shape)}.")
+    if parents.is_floating_point() or parents.dtype == torch.bool:
+        raise TypeError(f"{op}: parents must be whole numbers, got {parents.dtype}.")
+    par = _as(parents, torch.int32)
+    mask = torch.empty(B, N, dtype=torch.int64, device=dev)
+    depth = torch.empty(B, N, dtype=torch.int32, device=dev)
+    _launch(lib().maple_tree_plan, op, dev, ptr(par), B, N, N, 1, ptr(mask), ptr(depth), ptr(_err(dev)))
+    return TreePlan(par, mask, depth)
+
+
+def tree_gqa_attn(q, k_cache, v_cache, seqlen, tree_mask, *, row_map=None, scale: float, window: int | None = None):
+    """GQA attention of every node of a tree of drafted tokens over the cache
+    and its own branch.
+
+    ``q`` ``[B, N, H, D]``; caches ``[Bc, n_kv, T, D]``, node j's K/V rows at
+    slot ``seqlen[b] + j``; ``tree_mask`` int64 ``[B, N]``
+    (:attr:`TreePlan.mask`): node i sees the ``seqlen[b]`` cached positions and
+    the nodes of its bits; 0 is padding (zeros).  With ``window`` a node sees
+    keys of positions above its own (``seqlen + popcount(mask) - 1``) minus
+    ``window``.  Returns ``[B, N, H, D]`` in ``q.dtype`` (fp32 or bf16); with
+    ``N = 1`` it is :func:`decode_gqa_attn`."""
+    op = "tree_gqa_attn"
+    if q.ndim != 4:
+        raise ValueError(f"{op} expects q [B, N, H, D], got {tuple(q.shape)}.")
+    dev = _one_device(op, q, k_cache, v_cache, seqlen, tree_mask, row_map)
+    B, N = _tree_shape(op, q, "q")
+    H, D = int(q.shape[2]), int(q.shape[3])
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != D:
+        raise ValueError(f"{op}: caches must be [Bc, n_kv, T, {D}], got {tuple(k_cache.shape)} and "
+                         f"{tuple(v_cache.shape)}.")
+    Bc, n_kv, T = int(k_cache.shape[0]), int(k_cache.shape[1]), int(k_cache.shape[2])
+    if H % n_kv:
+        raise ValueError(f"n_q={H} not divisible by n_kv={n_kv}.")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError("KV cache dtype must match q dtype.")
+    if row_map is None and Bc != B:
+        raise ValueError(f"KV cache batch {Bc} != q batch {B}.")
+    if seqlen.numel() != B or (row_map is not None and row_map.numel() != B):
+        raise ValueError(f"{op}: seqlen and row_map need {B} entries.")
+    if tuple(tree_mask.shape) != (B, N) or tree_mask.dtype != torch.int64:
+        raise ValueError(f"{op}: tree_mask must be int64 {(B, N)}, got {tree_mask.dtype} {tuple(tree_mask.shape)}.")
+    ks = k_cache.stride()
+    if ks[3] != 1 or ks[2] != D or ks != v_cache.stride():
+        raise ValueError("KV caches must be [B, n_kv, T, D] with contiguous (T, D).")
+    if window is not None and window < 0:
+        raise ValueError(f"{op}: window must not be negative, got {window}.")
+    code, es = dtype_code(q, op), q.element_size()
+    if q.stride(3) != 1 or q.data_ptr() % 16 or any(s * es % 16 for s in q.stride()[:3]):
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+    qs = q.stride()
+    sl, tm = _as(seqlen, torch.int64), _as(tree_mask, torch.int64)
+    rm = _as(row_map, torch.int32) if row_map is not None else None
+    out = torch.empty(B, N, H, D, dtype=q.dtype, device=dev)
+    if B == 0:
+        return out
+    L = lib()
+    nbytes = L.maple_tree_gqa_workspace_bytes(B, N, H, n_kv, D, T, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
+    _launch(L.maple_tree_gqa_attn, op, dev, ptr(q), code, B, N, H, qs[0], qs[1], qs[2], ptr(k_cache), ptr(v_cache),
+            Bc, n_kv, ks[0], ks[1], T, D, ptr(sl), ptr(tm), ptr(rm), float(scale), int(window or 0), ptr(out), ptr(ws),
+            max(nbytes, 0), ptr(_err(dev)))
+    return out
+
+
+def verify_tree(logits, tokens, parents, uniform, *, temperature: float, top_p: float, top_k: int, draft_probs=None,
+                replacement: bool = False):
+    """Which drafted tokens stand, by rejection sampling against the target.
+
+    ``logits`` ``[B, N, V]`` are the target's at every node; its distribution is
+    the fused sampler's (``temperature``, ``top_p``, ``top_k`` 1..64; 1 is
+    greedy).  ``tokens`` ``[B, N]`` are the nodes' tokens, ``uniform`` ``[B, N]``
+    draws in [0, 1): node i's test, and at 0 the draw of the last token.
+    ``draft_probs`` ``[B, N, V]``: at each node, the distribution its children
+    were drawn from (without replacement unless ``replacement``); without it a
+    drafted token counts as certain, so it is accepted with the target's
+    probability of it.  The accepted tokens and the last one follow the
+    target's distribution.
+
+    Returns ``(path, n_path, ids)``: ``path`` int32 ``[B, N]`` the accepted
+    nodes from node 0 on, then -1; ``n_path`` int32 ``[B]``; ``ids`` int64
+    ``[B, N]`` the ``n_path`` tokens drawn, then -1.  A sequence whose node 0 is
+    padding has ``n_path`` 0."""
+    op = "verify_tree"
+    if logits.ndim != 3:
+        raise ValueError(f"{op} expects logits [B, N, V], got {tuple(logits.shape)}.")
+    dev = _one_device(op, logits, tokens, parents, uniform, draft_probs)
+    B, N = _tree_shape(op, logits, "logits")
+    V = int(logits.shape[2])
+    for t, what in ((tokens, "tokens"), (parents, "parents"), (uniform, "uniform")):
+        if tuple(t.shape) != (B, N):
+            raise ValueError(f"{op}: {what} must be {(B, N)}, got {tuple(t.shape)}.")
+    if tokens.is_floating_point() or parents.is_floating_point():
+        raise TypeError(f"{op}: tokens and parents must be whole numbers.")
+    if V < 1:
+        raise ValueError(f"{op}: empty vocabulary.")
+    if not 0 < top_k <= MAX_TOP_K:
+        raise ValueError(f"{op} needs 0 < top_k <= {MAX_TOP_K}, got {top_k}.")
+    if not temperature > 0:
+        raise ValueError(f"{op} needs temperature > 0 (greedy is top_k = 1).")
+    if not top_p > 0:
+        raise ValueError(f"{op} needs top_p > 0, got {top_p}.")
+    if draft_probs is not None and tuple(draft_probs.shape) != (B, N, V):
+        raise ValueError(f"{op}: draft_probs must be {(B, N, V)}, got {tuple(draft_probs.shape)}.")
+    code = dtype_code(logits, op)
+    dcode = dtype_code(draft_probs, op) if draft_probs is not None else 0
+    lg = logits if logits.stride(2) == 1 else logits.contiguous()
+    dp = draft_probs
+    if dp is not None and dp.stride(2) != 1:
+        dp = dp.contiguous()
+    tok, par, u = _as(tokens, torch.int64), _as(parents, torch.int32), _as(uniform, torch.float32)
+    path = torch.empty(B, N, dtype=torch.int32, device=dev)
+    n_path = torch.empty(B, dtype=torch.int32, device=dev)
+    ids = torch.empty(B, N, dtype=torch.int64, device=dev)
+    if B == 0:
+        return path, n_path, ids
+    L = lib()
+    nbytes = L.maple_verify_tree_workspace_bytes(B, N, V, top_k)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    _launch(L.maple_verify_tree, op, dev, ptr(lg), code, B, N, V, lg.stride(0), lg.stride(1), ptr(tok), ptr(par),
+            ptr(u), ptr(dp), dcode, dp.stride(0) if dp is not None else 0, dp.stride(1) if dp is not None else 0,
+            float(temperature), float(top_p), int(top_k), int(bool(replacement)), ptr(path), ptr(n_path), ptr(ids),
+            ptr(ws), ws.numel(), ptr(_err(dev)))
+    return path, n_path, ids
+
+
+class CacheRows:
+    """The K and V caches of all layers for :func:`commit_tree`: looked over
+    once and held as a table of device pointers (the caches stay where they
+    are, as a captured graph needs them to).  Holds the tensors."""
+
+    def __init__(self, k_caches, v_caches):
+        op = "commit_tree"
+        k, v = list(k_caches), list(v_caches)
+        if len(k) != len(v) or not k:
+            raise ValueError(f"{op}: {len(k)} K caches and {len(v)} V caches.")
+        first = k[0]
+        if first.ndim != 4 or first.stride(3) != 1 or first.stride(2) != first.shape[3]:
+            raise ValueError(f"{op}: KV caches must be [B, n_kv, T, D] with contiguous (T, D).")
+        self.device = _one_device(op, *k, *v)
+        self.code = dtype_code(first, op)
+        for t in k + v:
+            if t.shape != first.shape or t.stride() != first.stride():
+                raise ValueError(f"{op}: every layer's caches need one shape and stride, got {tuple(t.shape)} and "
+                                 f"{tuple(first.shape)}.")
+            if t.dtype != first.dtype:
+                raise TypeError(f"{op}: caches of {first.dtype} and {t.dtype}.")
+        self.k, self.v = k, v
+        self.shape = tuple(int(x) for x in first.shape)
+        self.strides = first.stride()
+        table = ctypes.c_void_p * len(k)
+        self.k_ptrs, self.v_ptrs = table(*[t.data_ptr() for t in k]), table(*[t.data_ptr() for t in v])
+
+
+def commit_tree(rows: CacheRows, seqlen, path, n_path, *, row_map=None) -> None:
+    """Keep the accepted nodes' K/V rows, in every layer and in place: slot
+    ``seqlen[b] + d`` takes slot ``seqlen[b] + path[b, d]`` for ``d <
+    n_path[b]`` (``path`` / ``n_path`` as :func:`verify_tree` returns them).
+    ``seqlen`` is not advanced."""
+    op = "commit_tree"
+    dev = rows.device
+    B, N = _tree_shape(op, path, "path")
+    Bc, n_kv, T, D = rows.shape
+    for t in (seqlen, path, n_path, row_map):
+        if t is not None and t.device != dev:
+            raise (ValueError if t.is_cuda else RuntimeError)(f"{op}: caches on {dev}, {t.device} given.")
+    if path.ndim != 2 or seqlen.numel() != B or n_path.numel() != B or (row_map is not None and row_map.numel() != B):
+        raise ValueError(f"{op}: path must be [B, N]; seqlen, n_path and row_map need {B} entries.")
+    if row_map is None and Bc < B:
+        raise ValueError(f"{op}: {B} sequences in a cache of {Bc} rows.")
+    if B == 0:
+        return
+    sl, pa, n = _as(seqlen, torch.int64), _as(path, torch.int32), _as(n_path, torch.int32)
+    rm = _as(row_map, torch.int32) if row_map is not None else None
+    _launch(lib().maple_commit_tree, op, dev, rows.k_ptrs, rows.v_ptrs, len(rows.k), rows.code, B, N, Bc, n_kv,
+            rows.strides[0], rows.strides[1], T, D, ptr(sl), ptr(pa), ptr(n), ptr(rm), ptr(_err(dev)))

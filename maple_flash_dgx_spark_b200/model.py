@@ -24,13 +24,18 @@ from maple_flash_dgx_spark_b200.kernels import (
     GROUPED_MIN_TOKENS,
     add_rms_norm,
     add_rms_norm_router_topk,
+    CacheRows,
+    TreePlan,
     apply_qkv_decode,
     attn_split_len,
+    commit_tree,
     decode_gqa_attn,
     decode_gqa_attn_qk,
     moe_plan,
     rms_norm,
     router_topk,
+    tree_gqa_attn,
+    tree_plan,
 )
 from maple_flash_dgx_spark_b200.linear import (
     DenseEmbedding,
@@ -128,6 +133,7 @@ class KVCache:
         self.row_of = list(range(batch))
         self.row_map = torch.arange(batch, dtype=torch.int32, device=device)
         self.remap = False
+        self._rows: CacheRows | None = None
         self.split_len = attn_split_len(max_len, batch, n_kv)
         # Decode attention on the tensor pipe (the reference's bf16 dots) where
         # the canonical CUDA-core kernel is instruction-bound: caches with more
@@ -205,6 +211,21 @@ class KVCache:
         for b in range(width):
             self.seen[b] += n
 
+    def commit_tree(self, path: torch.Tensor, n_path: torch.Tensor, kept: list[int] | None = None) -> None:
+        """Keep the accepted nodes of the last :meth:`MapleForCausalLM.forward_tree`
+        (``path`` / ``n_path`` as ``verify_tree`` returns them): their K/V rows
+        close up behind the sequences' positions and the lengths grow by
+        ``n_path``.  ``kept`` are the counts on the host, read (synchronising)
+        where the caller has not got them."""
+        first = 0 if self.slot is None else self.slot
+        slots = slice(first, first + path.shape[0])
+        if self._rows is None:
+            self._rows = CacheRows(self.k, self.v)
+        commit_tree(self._rows, self.seqlen[slots], path, n_path, row_map=self.row_map[slots])
+        self.seqlen[slots].add_(n_path)
+        for i, n in enumerate(n_path.tolist() if kept is None else kept):
+            self.seen[first + i] += int(n)
+
     def snapshot(self) -> dict:
         return {"seqlen": self.seqlen.clone(), "seen": list(self.seen), "k": [t.clone() for t in self.k],
                 "v": [t.clone() for t in self.v]}
@@ -216,6 +237,23 @@ class KVCache:
             dst.copy_(src)
         for dst, src in zip(self.v, snap["v"], strict=True):
             dst.copy_(src)
+
+
+class TreeStep:
+    """One step over trees of drafted tokens: the trees' plan, the sequences'
+    lengths and cache rows, and per node its cache slot, cache row and RoPE row
+    (at the position ``seqlen + depth``; siblings share one)."""
+
+    def __init__(self, plan: TreePlan, seqlen: torch.Tensor, rows: torch.Tensor, rotary: "MapleRotaryEmbedding"):
+        B, N = plan.mask.shape
+        self.plan = plan
+        self.seqlen = seqlen
+        self.rows = rows
+        node = torch.arange(N, device=seqlen.device)
+        self.slots = (seqlen[:, None] + node).reshape(-1)
+        self.slot_rows = rows.repeat_interleave(N)
+        at = (seqlen[:, None] + plan.depth).reshape(-1).clamp(0, rotary.max_cached - 1)
+        self.cos, self.sin = rotary.cos_table[at], rotary.sin_table[at]
 
 
 class MapleAttention:
@@ -246,11 +284,24 @@ class MapleAttention:
         self.use_rope = use_rope
         self.layer_idx = layer_idx
 
-    def __call__(self, hidden, seqlen, row_map, rotary, cache, *, rms_weight, rms_eps, kv_final=False):
+    def __call__(self, hidden, seqlen, row_map, rotary, cache, *, rms_weight, rms_eps, kv_final=False,
+                 tree: TreeStep | None = None):
         rows = hidden.shape[0]
         qkv = self.qkv_proj(hidden, rms_weight=rms_weight, rms_eps=rms_eps)
         self._mark("qkv")
         k_cache, v_cache = cache.k[self.layer_idx], cache.v[self.layer_idx]
+        if tree is not None:
+            # every node's K/V row behind its sequence, then attention over the cache and the node's branch
+            q = apply_qkv_decode(qkv, self.q_norm.weight, self.k_norm.weight, tree.cos, tree.sin, k_cache, v_cache,
+                                 tree.slots, row_map=tree.slot_rows, num_heads=self.num_heads,
+                                 num_kv_heads=self.num_kv_heads, head_dim=self.head_dim,
+                                 rotary_dim=rotary.rotary_dim, use_rope=self.use_rope, use_qk_norm=True,
+                                 eps=self.q_norm.eps)
+            B, N = tree.plan.mask.shape
+            attn = tree_gqa_attn(q.reshape(B, N, self.num_heads, self.head_dim), k_cache, v_cache, tree.seqlen,
+                                 tree.plan.mask, row_map=tree.rows, scale=self.scale, window=self.sliding_window)
+            self._mark("attention")
+            return self.o_proj(attn.reshape(rows, -1))
         if row_map is None:
             k_cache, v_cache = k_cache[:rows], v_cache[:rows]
         splits = -(-int(k_cache.shape[2]) // int(cache.split_len))
@@ -315,9 +366,9 @@ class MapleDecoderLayer:
         self.input_layernorm = input_layernorm
         self.post_attention_layernorm = post_attention_layernorm
 
-    def __call__(self, hidden, seqlen, row_map, rotary, cache, kv_final=False):
+    def __call__(self, hidden, seqlen, row_map, rotary, cache, kv_final=False, tree=None):
         attn_out = self.self_attn(hidden, seqlen, row_map, rotary, cache, rms_weight=self.input_layernorm.weight,
-                                  rms_eps=self.input_layernorm.eps, kv_final=kv_final)
+                                  rms_eps=self.input_layernorm.eps, kv_final=kv_final, tree=tree)
         if hasattr(self.mlp, "fused_add_norm"):
             return self.mlp.fused_add_norm(hidden, attn_out, self.post_attention_layernorm)
         hidden, mlp_in = add_rms_norm(hidden, attn_out, self.post_attention_layernorm.weight,
@@ -551,6 +602,31 @@ class MapleForCausalLM:
         return self.lm_head(normed).reshape(bsz, -1, self.vocab_size)
 
     __call__ = forward
+
+    def forward_tree(self, tokens: torch.Tensor, parents: torch.Tensor | TreePlan, cache: KVCache) -> torch.Tensor:
+        """Logits ``[B, N, V]`` of every node of ``B`` trees of drafted tokens
+        (``tokens`` and ``parents`` ``[B, N]``, node 0 the last drawn token; see
+        :func:`kernels.tree_plan`) over the first ``B`` slots of ``cache``, or
+        its prefill slot.  The nodes' K/V rows go to the slots behind each
+        sequence's positions; :meth:`KVCache.commit_tree` keeps those that
+        ``verify_tree`` accepts.  The lengths stay as they are."""
+        plan = parents if isinstance(parents, TreePlan) else tree_plan(parents)
+        bsz, n = plan.mask.shape
+        if tuple(tokens.shape) != (bsz, n):
+            raise ValueError(f"forward_tree: tokens {tuple(tokens.shape)} and trees {(bsz, n)}.")
+        first = 0 if cache.slot is None else cache.slot
+        if first + bsz > (cache.batch if cache.slot is None else first + 1):
+            raise ValueError(f"forward_tree: {bsz} trees for {cache.batch if cache.slot is None else 1} cache slots.")
+        need = max(cache.seen[first:first + bsz]) + n
+        if need > cache.max_len:
+            raise RuntimeError(f"KV cache overflow: need {need} slots, max_len={cache.max_len}.")
+        self.rotary.ensure_length(cache.max_len)
+        slots = slice(first, first + bsz)
+        step = TreeStep(plan, cache.seqlen[slots], cache.row_map[slots], self.rotary)
+        hidden = self.embed(tokens.reshape(-1))
+        for layer in self.layers:
+            hidden = layer(hidden, step.slots, step.slot_rows, self.rotary, cache, tree=step)
+        return self.lm_head(self.norm(hidden)).reshape(bsz, n, self.vocab_size)
 
     @torch.inference_mode()
     def generate(self, input_ids, max_tokens: int = 128):
