@@ -356,7 +356,14 @@ inline int tree_simt_splits(int64_t ctas, int64_t max_len) {
   return (int)(ns < 1 ? 1 : ns > kTreeMaxSplits ? kTreeMaxSplits : ns);
 }
 
-inline int tree_splits(int64_t batch, int64_t nodes, int64_t num_heads, int64_t num_kv_heads, int64_t max_len) {
+inline bool tree_use_tc(int x_dtype, int64_t head_dim) {
+  return x_dtype == kBF16 && (head_dim == 64 || head_dim == 128);
+}
+
+inline int tree_splits(int64_t batch, int64_t nodes, int64_t num_heads, int64_t num_kv_heads, int64_t max_len,
+                       int x_dtype, int64_t head_dim) {
+  if (tree_use_tc(x_dtype, head_dim))
+    return tree_tc_splits(batch * num_kv_heads * tree_tc_groups(nodes * (num_heads / num_kv_heads)), max_len);
   const int64_t tiles = (nodes * (num_heads / num_kv_heads) + kSimtRows - 1) / kSimtRows;
   return tree_simt_splits(batch * num_kv_heads * tiles, max_len);
 }
@@ -379,11 +386,10 @@ extern "C" int maple_tree_plan(const int32_t* parents, int64_t batch, int64_t no
 extern "C" int64_t maple_tree_gqa_workspace_bytes(int64_t batch, int64_t nodes, int64_t num_heads,
                                                   int64_t num_kv_heads, int64_t head_dim, int64_t max_len,
                                                   int x_dtype) {
-  (void)x_dtype;
   if (batch <= 0 || nodes <= 0 || nodes > kTreeMaxNodes || num_heads <= 0 || num_kv_heads <= 0 ||
       num_heads % num_kv_heads || head_dim <= 0 || max_len <= 0)
     return -1;
-  const int64_t ns = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len);
+  const int64_t ns = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim);
   return ns <= 1 ? 0 : batch * num_heads * nodes * ns * (head_dim + 2) * 4;
 }
 
@@ -417,7 +423,7 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   p.scale = scale;
   const int64_t rows = (int64_t)p.N * p.G, tiles = (rows + kSimtRows - 1) / kSimtRows;
   if (num_kv_heads * tiles > 65535) return kErrShape;
-  p.NS = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len);
+  p.NS = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim);
   const int64_t need = p.NS <= 1 ? 0 : batch * num_heads * nodes * p.NS * (head_dim + 2) * 4;
   if (need > 0 && (!workspace || workspace_bytes < need)) return kErrWorkspace;
   p.ws_acc = static_cast<float*>(workspace);
@@ -435,8 +441,15 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
       e = launch_k(tree_merge_kernel<XT, DD>,                                                                        \
                    dim3((unsigned)((num_kv_heads * rows + 7) / 8), (unsigned)batch), dim3(256), 0, st, p, kSimtKeys); \
   } while (0)
-  if (x_dtype == kBF16) {
-    if (head_dim == 64) MB_TREE(kBF16, 64); else if (head_dim == 128) MB_TREE(kBF16, 128); else MB_TREE(kBF16, 256);
+  if (tree_use_tc(x_dtype, head_dim)) {
+    if (batch * num_kv_heads * p.NS * tree_tc_groups(rows) > (1LL << 30)) return kErrShape;
+    e = tree_tc_launch(p, (int)head_dim, st);
+    const dim3 grid((unsigned)((num_kv_heads * rows + 7) / 8), (unsigned)batch);
+    if (e == cudaSuccess && p.NS > 1)
+      e = head_dim == 64 ? launch_k(tree_merge_kernel<kBF16, 64>, grid, dim3(256), 0, st, p, tree_tc_tile())
+                         : launch_k(tree_merge_kernel<kBF16, 128>, grid, dim3(256), 0, st, p, tree_tc_tile());
+  } else if (x_dtype == kBF16) {
+    MB_TREE(kBF16, 256);
   } else {
     if (head_dim == 64) MB_TREE(kF32, 64); else if (head_dim == 128) MB_TREE(kF32, 128); else MB_TREE(kF32, 256);
   }

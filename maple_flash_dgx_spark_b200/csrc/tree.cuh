@@ -81,4 +81,10 @@ __device__ __forceinline__ int tree_splits_used(int lo, int hi, int tile, int ns
   return (tiles + per - 1) / per;
 }
 
+// tree_tc.cu: the tcgen05 kernel (bf16, heads of 64 or 128).
+int tree_tc_splits(int64_t ctas, int64_t max_len);
+int tree_tc_groups(int64_t rows);
+int tree_tc_tile();
+cudaError_t tree_tc_launch(const TreeAttnParams& p, int D, cudaStream_t st);
+
 }  // namespace mb

@@ -1,0 +1,621 @@
+// Attention over a KV cache for trees of drafted tokens on the 5th-generation
+// tensor cores (bf16 caches, heads of 64 or 128).
+//
+// The rows of a KV head are (node, query head of the group) pairs, row r =
+// node r / G, head r % G, in tiles of 128 = the MMA's M; a tile of 128 keys is
+// its N.  Per key tile S = Q K^T (K-major operands from 128-byte-swizzled
+// shared memory), softmax in registers, then O += P V with P as bf16 in tensor
+// memory (over the scores it came from) and V read as stored, [keys][dims], an
+// MN-major operand.  Each K/V row crosses HBM once per 256 rows.
+//
+// Roles (320 threads, one CTA per SM, persistent over work items): warp 9
+// works the items out and streams K and V tiles by TMA into two rings; warp 8
+// issues the MMAs; two warpgroups of four warps do the softmax, a thread per
+// row.  Up to 128 rows (PAIR = false) both warpgroups share the row tile and
+// take alternate key tiles, each with its own scores, output, maximum and sum,
+// joined at the item's end; more rows (PAIR = true) give each its own row tile.
+// Either way one's softmax runs under the other's MMAs.  A unit = one key tile
+// of one warpgroup; the tensor pipe runs S(0) S(1) O(0) S(2) O(1) S(3) ..., so
+// a unit's scores overwrite its predecessor's weights right behind the product
+// that read them.  Because scores are committed behind that product, a
+// warpgroup that sees them knows its output is at rest, and may rescale it;
+// it does so only when a row's maximum has grown by more than 2^8 (the weights
+// then still fit fp32 and bf16 many times over).
+//
+// An item is one split of one sequence's keys for one KV head and row tile (or
+// pair).  A tile that some row sees only in part is masked in registers; its
+// V tile is cleared of NaN and infinities in shared memory first (0 x NaN is
+// NaN), and where a visible one was cleared the item's end adds it back to the
+// rows that see it.
+//
+// Waits are bounded: one that gives up sets the error word; every role then
+// leaves, waits (bounded) for its copies and MMAs in flight, frees the tensor
+// memory and returns.  Loads read this GPU's own memory, without multicast.
+#include "bulk.cuh"
+#include "launch.cuh"
+#include "tcgen05.cuh"
+#include "tmap.cuh"
+#include "tree.cuh"
+
+namespace mb {
+
+constexpr int kTtKeys = 128;   // keys per tile: MMA N of the scores, K of the output
+constexpr int kTtRows = 128;   // rows per tile: MMA M
+constexpr int kTtThreads = 320;
+constexpr int kTtInfo = 2;     // items known ahead
+constexpr float kTtGrow = 8.0f;  // log2 growth of a row's maximum that rescales
+
+struct TtItem {
+  int b, h, rt, sp;     // sequence, KV head, row tile (pair), split
+  int s, lo, k0, k1;    // cached positions, the row's first key, this split's keys
+  int tiles, alone, fix, dmax;  // key tiles; the only split; V was cleared; largest depth
+  unsigned long long mask[kTreeMaxNodes];
+};
+
+template <int D, bool PAIR>
+struct TtShape {
+  static constexpr int kTile = kTtKeys * D * 2;              // one K, V or Q tile
+  static constexpr int kQ = PAIR ? 2 : 1;
+  static constexpr int NK = D == 128 ? 3 : 4;                // ring depths
+  static constexpr int NV = D == 128 ? (PAIR ? 2 : 3) : 4;
+  static constexpr int kTiles = (kQ + NK + NV) * kTile;
+  static constexpr int kSmem = kTiles + kTtInfo * (int)sizeof(TtItem) + 288;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ bool odd_bf16x2(uint32_t w) {  // a NaN or infinity in either half
+  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+// A barrier among warps on an mbarrier (one arrival per warp), so that a warp
+// that gave up cannot leave the others waiting for good.
+__device__ __forceinline__ bool tt_sync(uint64_t* bar, int& count, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+  const bool ok = mbar_wait_bounded(bar, (unsigned)(count & 1));
+  ++count;
+  return __all_sync(0xffffffffu, ok);
+}
+
+// Whether some row of the item misses a key of the tile at t0: it reaches into
+// the tree, past the split's end, or before a window.
+__device__ __forceinline__ bool tt_mixed(const TtItem& it, int t0, int window) {
+  return t0 + kTtKeys > min(it.s, it.k1) || (window > 0 && t0 <= it.s + it.dmax - window);
+}
+
+// This row's view of a tile as 128 bits: cached positions past the window's
+// start, and its nodes' bits.
+struct TtView {
+  unsigned long long nodes;  // nodes seen, the window applied
+  int first;                 // first cached position seen
+  bool real;
+};
+__device__ __forceinline__ void tt_bits(const TtView& v, int s, int k1, int t0, uint32_t (&w)[4]) {
+  const int a = max(0, v.first - t0), e = min(s, k1) - t0;  // cached: columns [a, e)
+  const int off = s - t0;                                   // column of node 0
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int lo = min(max(a - 32 * q, 0), 32), hi = min(max(e - 32 * q, 0), 32);
+    const uint32_t upto = hi >= 32 ? 0xffffffffu : (1u << hi) - 1u, from = lo >= 32 ? 0xffffffffu : (1u << lo) - 1u;
+    const int sh = 32 * q - off;  // node of this word's bit 0
+    uint32_t nb = 0;
+    if (sh >= 0 && sh < 64) nb = (uint32_t)(v.nodes >> sh);
+    else if (sh < 0 && sh > -32) nb = (uint32_t)(v.nodes << -sh);
+    w[q] = v.real ? (upto & ~from) | nb : 0u;
+  }
+  // nodes past the split's end belong to the next split
+  const int end = k1 - t0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int hi = min(max(end - 32 * q, 0), 32);
+    w[q] &= hi >= 32 ? 0xffffffffu : (1u << hi) - 1u;
+  }
+}
+
+template <int D, bool PAIR>
+__global__ void __launch_bounds__(kTtThreads, 1)
+    tree_tc_kernel(TreeAttnParams p, int row_groups, int items, const __grid_constant__ CUtensorMap tmk,
+                   const __grid_constant__ CUtensorMap tmv) {
+  using Sh = TtShape<D, PAIR>;
+  constexpr int TILE = Sh::kTile, NK = Sh::NK, NV = Sh::NV, HALVES = D / 64, BOX = kTtKeys * 128;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char* sq = smem;
+  unsigned char* sk = sq + Sh::kQ * TILE;
+  unsigned char* sv = sk + NK * TILE;
+  TtItem* info = reinterpret_cast<TtItem*>(sv + NV * TILE);
+  float2* s_ml = reinterpret_cast<float2*>(sq);  // [2][128] maximum and sum, once the queries are done with
+  uint64_t* bars = reinterpret_cast<uint64_t*>(info + kTtInfo);
+  uint64_t *kfull = bars, *kempty = kfull + NK, *vfull = kempty + NK, *vempty = vfull + NV, *sfull = vempty + NV,
+           *pready = sfull + 2, *ofull = pready + 2, *oempty = ofull + 2, *qfull = oempty + 1, *ifull = qfull + 1,
+           *iempty = ifull + kTtInfo, *both = iempty + kTtInfo, *each = both + 1, *drain = each + 2;
+  unsigned* s_tmem = reinterpret_cast<unsigned*>(drain + 1);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  if (warp == 8) tmem_alloc(s_tmem, 512);
+  if (tid == 0) {
+    for (int i = 0; i < NK; ++i) { mbar_init(&kfull[i], 1); mbar_init(&kempty[i], 1); }
+    for (int i = 0; i < NV; ++i) { mbar_init(&vfull[i], 1); mbar_init(&vempty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&sfull[i], 1); mbar_init(&pready[i], 4); mbar_init(&ofull[i], 1); }
+    mbar_init(oempty, 8);
+    mbar_init(qfull, 8);
+    for (int i = 0; i < kTtInfo; ++i) { mbar_init(&ifull[i], 1); mbar_init(&iempty[i], 9); }
+    mbar_init(both, 8);
+    for (int i = 0; i < 2; ++i) mbar_init(&each[i], 4);
+    mbar_init(drain, 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = *s_tmem;
+  pdl_wait();
+  pdl_trigger();
+  bool ok = (smem_u32(smem) & 1023u) == 0;  // the swizzled tiles need it; the launch gives it
+
+  if (warp == 9) {
+    // -------------------------------------------------- items, K and V tiles --
+    const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
+    int n_items = 0, kt_all = 0;
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const int rt = item % row_groups, sp = item / row_groups % p.NS, bh = item / row_groups / p.NS;
+      const int h = bh % p.Hkv, b = bh / p.Hkv;
+      unsigned long long m[2], used = 0;
+      int dm = 0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i = lane + 32 * u;
+        m[u] = i < p.N ? p.mask[(int64_t)b * p.N + i] & keep : 0ull;
+        used |= m[u] | (m[u] ? 1ull << i : 0ull);
+        dm = max(dm, __popcll(m[u]) - 1);
+      }
+      const unsigned ul = __reduce_or_sync(0xffffffffu, (unsigned)used);
+      const unsigned uh = __reduce_or_sync(0xffffffffu, (unsigned)(used >> 32));
+      dm = __reduce_max_sync(0xffffffffu, dm);
+      const TreeRange rg = tree_range(p, b, ((unsigned long long)uh << 32) | ul);
+      if (rg.bad && lane == 0) atomicOr(p.err, kErrFlagBounds);
+      int k0, k1;
+      tree_split(rg.lo, rg.hi, kTtKeys, p.NS, sp, k0, k1);
+      if (sp > 0 && k0 >= k1) continue;  // nothing here; split 0 always answers
+      const int tiles = (k1 - k0 + kTtKeys - 1) / kTtKeys, slot = n_items % kTtInfo, use = n_items / kTtInfo;
+      if (use > 0) ok = mbar_wait_bounded(&iempty[slot], (unsigned)((use - 1) & 1));
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      TtItem& it = info[slot];
+      it.mask[lane] = m[0];
+      it.mask[lane + 32] = m[1];
+      if (lane == 0) {
+        it.b = b; it.h = h; it.rt = rt; it.sp = sp;
+        it.s = rg.s; it.lo = rg.lo; it.k0 = k0; it.k1 = k1; it.tiles = tiles; it.fix = 0; it.dmax = dm;
+        it.alone = tree_splits_used(rg.lo, rg.hi, kTtKeys, p.NS) <= 1;
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&ifull[slot]);
+        // K runs ahead of V by one tile (two where the warpgroups take turns), as the MMAs use them
+        constexpr int AHEAD = PAIR ? 1 : 2;
+        for (int c = 0; c < tiles + AHEAD && ok; ++c) {
+          if (c < tiles) {
+            const int g = kt_all + c, st = g % NK;
+            if (g >= NK) ok = mbar_wait_bounded(&kempty[st], (unsigned)((g / NK - 1) & 1));
+            if (!ok) break;
+            mbar_expect_tx(&kfull[st], (unsigned)TILE);
+#pragma unroll
+            for (int hf = 0; hf < HALVES; ++hf)
+              tma_load_4d(sk + st * TILE + hf * BOX, &tmk, 64 * hf, k0 + c * kTtKeys, h, rg.cb, &kfull[st]);
+          }
+          if (c >= AHEAD) {
+            const int g = kt_all + c - AHEAD, st = g % NV;
+            if (g >= NV) ok = mbar_wait_bounded(&vempty[st], (unsigned)((g / NV - 1) & 1));
+            if (!ok) break;
+            mbar_expect_tx(&vfull[st], (unsigned)TILE);
+#pragma unroll
+            for (int hf = 0; hf < HALVES; ++hf)
+              tma_load_4d(sv + st * TILE + hf * BOX, &tmv, 64 * hf, k0 + (c - AHEAD) * kTtKeys, h, rg.cb, &vfull[st]);
+          }
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      kt_all += tiles;
+      ++n_items;
+    }
+    if (ok) {  // the end
+      const int slot = n_items % kTtInfo, use = n_items / kTtInfo;
+      if (use > 0) ok = mbar_wait_bounded(&iempty[slot], (unsigned)((use - 1) & 1));
+      if (ok && lane == 0) {
+        info[slot].tiles = -1;
+        mbar_arrive(&ifull[slot]);
+      }
+    }
+    if (lane == 0) {
+      if (!ok) atomicOr(p.err, kErrFlagTimeout);
+      // copies in flight land before the CTA's memory is given up: no use for the ones that were consumed
+      for (int i = 0; i < NK; ++i)
+        if (kt_all > i) mbar_wait_bounded(&kfull[i], (unsigned)(((kt_all - 1 - i) / NK) & 1));
+      for (int i = 0; i < NV; ++i)
+        if (kt_all > i) mbar_wait_bounded(&vfull[i], (unsigned)(((kt_all - 1 - i) / NV) & 1));
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // --------------------------------------------------------------- MMAs --
+    if (lane == 0) {
+      constexpr unsigned id_s = umma_idesc_bf16(kTtRows, kTtKeys, false), id_o = umma_idesc_bf16(kTtRows, D, true);
+      int kbase = 0, work = 0, pcount[2] = {0, 0};
+      for (int n = 0; ok; ++n) {
+        const int slot = n % kTtInfo;
+        ok = mbar_wait_bounded(&ifull[slot], (unsigned)((n / kTtInfo) & 1));
+        if (!ok) break;
+        const int tiles = info[slot].tiles;
+        mbar_arrive(&iempty[slot]);
+        if (tiles < 0) break;
+        if (tiles == 0) continue;
+        const int units = PAIR ? 2 * tiles : tiles;
+        auto scores = [&](int u) {
+          const int w = u & 1, g = kbase + (PAIR ? u >> 1 : u), st = g % NK;
+          if (!PAIR || w == 0) ok = mbar_wait_bounded(&kfull[st], (unsigned)((g / NK) & 1));
+          if (!ok) return;
+          tc_fence_after();
+          const unsigned qa = smem_u32(sq + (PAIR ? w : 0) * TILE), ka = smem_u32(sk + st * TILE);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const unsigned o = (kk >> 2) * BOX + (kk & 3) * 32;
+            umma_bf16(tmem + w * kTtKeys, umma_desc_sw128(qa + o), umma_desc_sw128(ka + o), id_s, kk > 0);
+          }
+          umma_commit(&sfull[w]);
+          if (!PAIR || w == 1) umma_commit(&kempty[st]);
+        };
+        ok = mbar_wait_bounded(qfull, (unsigned)(work & 1));
+        if (ok) scores(0);
+        if (ok && units > 1) scores(1);
+        // the item before has read its output
+        if (ok && work > 0) ok = mbar_wait_bounded(oempty, (unsigned)((work - 1) & 1));
+        for (int u = 0; u < units && ok; ++u) {
+          const int w = u & 1, kt = PAIR ? u >> 1 : u, g = kbase + kt, st = g % NV;
+          ok = mbar_wait_bounded(&pready[w], (unsigned)(pcount[w] & 1));
+          ++pcount[w];
+          if (ok && (!PAIR || w == 0)) ok = mbar_wait_bounded(&vfull[st], (unsigned)((g / NV) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          const unsigned va = smem_u32(sv + st * TILE);
+#pragma unroll
+          for (int kk = 0; kk < kTtKeys / 16; ++kk)
+            umma_bf16_ta(tmem + 2 * kTtKeys + w * D, tmem + w * kTtKeys + 8 * kk,
+                         umma_desc_sw128_mn(va + 2048 * kk, BOX), id_o, u >= 2 || kk > 0);
+          if (!PAIR || w == 1) umma_commit(&vempty[st]);
+          if (u + 2 < units) scores(u + 2);
+        }
+        if (ok) {
+          umma_commit(&ofull[0]);
+          umma_commit(&ofull[1]);
+        }
+        kbase += tiles;
+        ++work;
+      }
+      if (!ok) atomicOr(p.err, kErrFlagTimeout);
+      umma_commit(drain);  // nothing of the tensor pipe is left behind
+      mbar_wait_bounded(drain, 0);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax --
+    const int w = warp >> 2, r = tid & 127;
+    const unsigned lanes = (unsigned)(warp & 3) << 21;  // TMEM lane base of this warp, in bits 31:16
+    const unsigned t_s = tmem + lanes + w * kTtKeys, t_o = tmem + lanes + 2 * kTtKeys;
+    const float ninf = __int_as_float(0xff800000);
+    const float c = fabsf(p.scale) * 1.44269504088896341f;
+    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;  // the queries carry the scale's sign
+    const int rows = p.N * p.G;
+    int kbase = 0, work = 0, scount = 0, n_both = 0, n_each = 0;
+    for (int n = 0; ok; ++n) {
+      const int slot = n % kTtInfo;
+      ok = mbar_wait_bounded(&ifull[slot], (unsigned)((n / kTtInfo) & 1));
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      TtItem& it = info[slot];
+      const int tiles = it.tiles;
+      if (tiles < 0) break;
+      const int b = it.b, h = it.h, s = it.s, k0 = it.k0, k1 = it.k1;
+      const int row = (PAIR ? 2 * it.rt + w : it.rt) * kTtRows + r;
+      const int node = row / p.G, head = h * p.G + row - node * p.G;
+      TtView view{};
+      const unsigned long long mine = row < rows ? it.mask[node] : 0ull;
+      view.real = mine != 0;
+      view.nodes = mine;
+      if (p.window > 0) {
+        const int first = s + __popcll(mine) - p.window;  // lowest position seen
+        view.first = max(0, first);
+        for (unsigned long long left = mine; left; left &= left - 1) {
+          const int j = __ffsll((long long)left) - 1;
+          if (s + __popcll(it.mask[j]) - 1 < first) view.nodes &= ~(1ull << j);
+        }
+      }
+      const int64_t out = (((int64_t)b * p.N + node) * p.H + head) * D;
+      float mc = ninf, l = 0.0f;  // maximum times c, sum of weights
+      int mine_units = 0;
+      if (tiles > 0) {
+        // Q, 128-byte swizzled: the WG's own tile, or both WGs half of the shared one
+        {
+          constexpr int CH = D / 8;  // 16-byte chunks per row
+          unsigned char* tile = sq + (PAIR ? w : 0) * TILE;
+          const int t = PAIR ? r : tid, nt = PAIR ? 128 : 256, base = (PAIR ? 2 * it.rt + w : it.rt) * kTtRows;
+          for (int x = t; x < kTtRows * CH; x += nt) {
+            const int qr = x / CH, cc = x % CH, gr = base + qr;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (gr < rows) {
+              const int i = gr / p.G, g = gr - i * p.G;
+              v = ld_u4(static_cast<const char*>(p.q) +
+                        (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + g) * p.q_sh + cc * 8) * 2);
+              v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+            }
+            *reinterpret_cast<uint4*>(tile + (cc >> 3) * BOX + qr * 128 + (((cc & 7) ^ (qr & 7)) << 4)) = v;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(qfull);
+        }
+        const bool idle = __all_sync(0xffffffffu, row >= rows);  // this warp has no row: it only keeps step
+        for (int kt = PAIR ? 0 : w; kt < tiles && ok; kt += PAIR ? 1 : 2, ++mine_units) {
+          ok = mbar_wait_bounded(&sfull[w], (unsigned)(scount & 1));
+          ++scount;
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          tc_fence_after();
+          const int t0 = k0 + kt * kTtKeys;
+          const bool mixed = tt_mixed(it, t0, p.window);
+          if (mixed) {
+            // clear the V tile of NaN and infinities before its product
+            const int g = kbase + kt, st = g % NV;
+            ok = mbar_wait_bounded(&vfull[st], (unsigned)((g / NV) & 1));
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+              unsigned char* tile = sv + st * TILE;
+              constexpr int UNITS = TILE / 16;
+              bool found = false;
+              for (int x = PAIR ? tid : r; x < UNITS; x += PAIR ? 256 : 128) {
+                uint4* q = reinterpret_cast<uint4*>(tile) + x;
+                uint4 v = *q;
+                uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (odd_bf16x2(e[i])) {
+                    odd = true;
+                    if ((e[i] & 0x7f80u) == 0x7f80u) e[i] &= 0xffff0000u;
+                    if ((e[i] & 0x7f800000u) == 0x7f800000u) e[i] &= 0x0000ffffu;
+                  }
+                if (odd) {
+                  *q = v;
+                  found |= t0 + (x % (BOX / 16)) / 8 < k1;
+                }
+              }
+              if (found) it.fix = 1;
+              fence_proxy_async_smem();
+            }
+            const bool met = PAIR ? tt_sync(both, n_both, lane) : tt_sync(&each[w], n_each, lane);
+            ok = ok && met;
+            if (!ok) break;
+          }
+          if (!idle) {
+            uint32_t bits[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            if (mixed) tt_bits(view, s, k1, t0, bits);
+            // the scores are read twice from tensor memory, 64 columns at a time: 128 registers of them would spill
+            float top[4] = {ninf, ninf, ninf, ninf};
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t x[64];
+              tmem_ld32(t_s + 64 * q, x);
+              tmem_ld32(t_s + 64 * q + 32, x + 32);
+              tmem_wait32(x);
+              tmem_wait32(x + 32);
+              if (mixed) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                  if (!((bits[2 * q + (i >> 5)] >> (i & 31)) & 1u)) x[i] = 0xff800000u;
+              }
+#pragma unroll
+              for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
+            }
+            const float tc = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+            const bool grow = tc > mc + kTtGrow || (mc == ninf && tc > ninf);
+            if (__any_sync(0xffffffffu, grow)) {
+              const float f = grow ? (mc == ninf ? 0.0f : ex2(mc - tc)) : 1.0f;
+              if (grow) mc = tc;
+              l *= f;
+              if (mine_units > 0) {
+#pragma unroll
+                for (int q = 0; q < D / 32; ++q) {
+                  uint32_t o[32];
+                  tmem_ld32(t_o + w * D + 32 * q, o);
+                  tmem_wait32(o);
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                  tmem_st32(t_o + w * D + 32 * q, o);
+                }
+              }
+            }
+            const float sub = mc == ninf ? 0.0f : -mc;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t x[64];
+              tmem_ld32(t_s + 64 * q, x);
+              tmem_ld32(t_s + 64 * q + 32, x + 32);
+              tmem_wait32(x);
+              tmem_wait32(x + 32);
+#pragma unroll
+              for (int i = 0; i < 64; i += 2) {
+                float a = ex2(fmaf(__uint_as_float(x[i]), c, sub)), e = ex2(fmaf(__uint_as_float(x[i + 1]), c, sub));
+                if (mixed) {
+                  if (!((bits[2 * q + (i >> 5)] >> (i & 31)) & 1u)) a = 0.0f;
+                  if (!((bits[2 * q + (i >> 5)] >> ((i + 1) & 31)) & 1u)) e = 0.0f;
+                }
+                sum[i & 2] += a;
+                sum[(i & 2) + 1] += e;
+                x[i >> 1] = bf16x2(a, e);
+              }
+              tmem_st32(t_s + 32 * q, x);  // over scores that are read already
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_wait_st();
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pready[w]);
+        }
+        if (!ok) break;
+        // the end: the output of every unit is in
+        ok = mbar_wait_bounded(&ofull[w], (unsigned)(work & 1));
+        if (!PAIR) ok = mbar_wait_bounded(&ofull[w ^ 1], (unsigned)(work & 1)) && ok;
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+      }
+      float f0 = 1.0f, f1 = 0.0f;  // weights of this warpgroup's output and the other's
+      int other_units = 0;
+      if (!PAIR && tiles > 0) {
+        s_ml[w * kTtRows + r] = make_float2(mc, l);
+        ok = tt_sync(both, n_both, lane);
+        if (!ok) break;
+        const float2 o = s_ml[(w ^ 1) * kTtRows + r];
+        other_units = w == 0 ? tiles / 2 : (tiles + 1) / 2;
+        const float M = fmaxf(mc, o.x);
+        f0 = mc == ninf ? 0.0f : ex2(mc - M);
+        f1 = o.x == ninf ? 0.0f : ex2(o.x - M);
+        // the same order in both warpgroups
+        const float la = w == 0 ? f0 * l : f1 * o.y, lb = w == 0 ? f1 * o.y : f0 * l;
+        l = la + lb;
+        mc = M;
+      }
+      const bool zero = !(row < rows && mine != 0) || l == 0.0f;
+      const float inv = zero ? 0.0f : 1.0f / l;
+      const int64_t R = ((int64_t)b * p.Hkv + h) * rows + row;
+      constexpr int COLS = PAIR ? D : D / 2;  // sharing the rows, each warpgroup writes half of the dimensions
+#pragma unroll
+      for (int q = 0; q < COLS / 32; ++q) {
+        const int col = (PAIR ? 0 : w * COLS) + 32 * q;
+        uint32_t o[32];
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+        if (mine_units > 0) {
+          tmem_ld32(t_o + w * D + col, o);
+          tmem_wait32(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = f0 * __uint_as_float(o[i]);
+        }
+        if (other_units > 0) {
+          tmem_ld32(t_o + (w ^ 1) * D + col, o);
+          tmem_wait32(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += f1 * __uint_as_float(o[i]);
+        }
+        if (it.fix && row < rows) {
+          // NaN and infinities that were cleared, to the rows that see them
+          const uint16_t* vb = static_cast<const uint16_t*>(p.vc) +
+                               (p.row_map != nullptr ? p.row_map[b] : b) * p.c_sb + h * p.c_sh + col;
+          for (int t0 = k0; t0 < k1; t0 += kTtKeys) {
+            if (!tt_mixed(it, t0, p.window)) continue;
+            uint32_t bits[4];
+            tt_bits(view, s, k1, t0, bits);
+            for (int x = 0; x < kTtKeys && t0 + x < k1; ++x) {
+              const uint32_t word = x < 64 ? (x < 32 ? bits[0] : bits[1]) : (x < 96 ? bits[2] : bits[3]);
+              if (!((word >> (x & 31)) & 1u)) continue;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const uint16_t y = vb[(int64_t)(t0 + x) * D + i];
+                if ((y & 0x7f80u) == 0x7f80u) v[i] += bf16_to_f32(y);
+              }
+            }
+          }
+        }
+        if (row < rows) {
+          if (it.alone) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + out + col);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t y[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                y[j] = zero ? 0u : bf16x2(v[8 * i + 2 * j] * inv, v[8 * i + 2 * j + 1] * inv);
+              dst[i] = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.ws_acc + (R * p.NS + it.sp) * D + col);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dst[i] = zero ? make_float4(0.f, 0.f, 0.f, 0.f)
+                            : make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        }
+      }
+      if (!it.alone && row < rows && (PAIR || w == 0)) {
+        p.ws_ml[(R * p.NS + it.sp) * 2] = zero ? ninf : mc * 0.693147180559945309f;
+        p.ws_ml[(R * p.NS + it.sp) * 2 + 1] = zero ? 0.0f : l;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (tiles > 0) {
+        // both have read the exchange: the queries may be overwritten
+        if (!PAIR) ok = tt_sync(both, n_both, lane);
+        if (lane == 0) mbar_arrive(oempty);
+        ++work;
+        kbase += tiles;
+      }
+      if (lane == 0) mbar_arrive(&iempty[slot]);
+    }
+    if (!ok && lane == 0) atomicOr(p.err, kErrFlagTimeout);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+// Splits of a sequence's keys.  Few items leave SMs idle, more splits cost a
+// join: time in key tiles (1.4 us each at 44 GB/s per SM) ~ waves x (tiles per
+// split + 4 of start and end), + 6 for the join's launch, + the partials'
+// traffic (a split writes and reads 128 KB per 128 rows: 2 tiles' worth).
+int tree_tc_splits(int64_t ctas, int64_t max_len) {
+  const int64_t tiles = (max_len + kTtKeys - 1) / kTtKeys;
+  int64_t best = 1;
+  double cost = 1e30;
+  for (int64_t ns = 1; ns <= kTreeMaxSplits && ns <= tiles; ++ns) {
+    const int64_t waves = (ctas * ns + 147) / 148, per = (tiles + ns - 1) / ns;
+    const double t = (double)waves * ((double)per + 4.0 + (ns > 1 ? 2.0 : 0.0)) + (ns > 1 ? 6.0 : 0.0);
+    if (t < cost) {
+      cost = t;
+      best = ns;
+    }
+  }
+  return (int)best;
+}
+
+int tree_tc_groups(int64_t rows) { return rows <= kTtRows ? 1 : (int)((rows + 2 * kTtRows - 1) / (2 * kTtRows)); }
+
+int tree_tc_tile() { return kTtKeys; }
+
+template <int D, bool PAIR>
+cudaError_t tree_tc_launch1(const TreeAttnParams& p, int groups, const CUtensorMap& tmk, const CUtensorMap& tmv,
+                            cudaStream_t st) {
+  constexpr int smem = TtShape<D, PAIR>::kSmem;
+  static_assert(smem <= 232448, "shared memory of one SM");
+  const int items = p.B * p.Hkv * p.NS * groups;
+  const cudaError_t e = cudaFuncSetAttribute(tree_tc_kernel<D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  return launch_k(tree_tc_kernel<D, PAIR>, dim3((unsigned)(items < 148 ? items : 148)), dim3(kTtThreads), smem, st, p,
+                  groups, items, tmk, tmv);
+}
+
+cudaError_t tree_tc_launch(const TreeAttnParams& p, int D, cudaStream_t st) {
+  CUtensorMap tmk, tmv;
+  if (!tmap_bf16_4d(p.kc, D, p.T, p.Hkv, p.Bc, D, p.c_sh, p.c_sb, 64, kTtKeys, &tmk) ||
+      !tmap_bf16_4d(p.vc, D, p.T, p.Hkv, p.Bc, D, p.c_sh, p.c_sb, 64, kTtKeys, &tmv))
+    return cudaErrorInvalidValue;
+  const int rows = p.N * p.G, groups = tree_tc_groups(rows);
+  const bool pair = rows > kTtRows;
+  if (D == 64) return pair ? tree_tc_launch1<64, true>(p, groups, tmk, tmv, st) : tree_tc_launch1<64, false>(p, groups, tmk, tmv, st);
+  return pair ? tree_tc_launch1<128, true>(p, groups, tmk, tmv, st) : tree_tc_launch1<128, false>(p, groups, tmk, tmv, st);
+}
+
+}  // namespace mb
