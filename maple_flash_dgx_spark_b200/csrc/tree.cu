@@ -88,6 +88,8 @@ __global__ void __launch_bounds__(256) tree_simt_kernel(TreeAttnParams p, int ro
   const float ninf = __int_as_float(0xff800000);
   pdl_wait();
   pdl_trigger();
+  const int64_t len = p.seqlen[b];
+  const int cb = p.row_map != nullptr ? p.row_map[b] : b;
   if (tid < kTreeMaxNodes) {
     const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
     s_mask[tid] = tid < p.N ? p.mask[(int64_t)b * p.N + tid] & keep : 0ull;
@@ -95,7 +97,7 @@ __global__ void __launch_bounds__(256) tree_simt_kernel(TreeAttnParams p, int ro
   __syncthreads();
   unsigned long long used = 0;
   for (int i = 0; i < p.N; ++i) used |= s_mask[i] | (s_mask[i] ? 1ull << i : 0ull);
-  const TreeRange rg = tree_range(p, b, used);
+  const TreeRange rg = tree_range(p, len, cb, used);
   if (rg.bad && tid == 0) atomicOr(p.err, kErrFlagBounds);
   int k0, k1;
   tree_split(rg.lo, rg.hi, kSimtKeys, p.NS, sp, k0, k1);
@@ -233,6 +235,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeAttnParams p, int t
   const int rows = p.N * p.G, hr = blockIdx.x * 8 + warp, b = blockIdx.y;
   pdl_wait();
   pdl_trigger();
+  const int64_t len = p.seqlen[b];
+  const int cb = p.row_map != nullptr ? p.row_map[b] : b;
   const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
   unsigned long long used = 0;
   for (int i = lane; i < p.N; i += 32) {
@@ -241,7 +245,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeAttnParams p, int t
   }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) used |= __shfl_xor_sync(0xffffffffu, used, o);
-  const TreeRange rg = tree_range(p, b, used);
+  const TreeRange rg = tree_range(p, len, cb, used);
   const int ns = tree_splits_used(rg.lo, rg.hi, tile, p.NS);
   if (hr >= p.Hkv * rows || ns <= 1) return;  // one split wrote its output itself
   const int h = hr / rows, r = hr - h * rows;

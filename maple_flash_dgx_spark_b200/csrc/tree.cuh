@@ -36,7 +36,7 @@ struct TreeAttnParams {
   float scale;
 };
 
-// The keys of sequence b: [lo, hi) of slots, hi = s + (nodes in use); every
+// The keys of a sequence of length s in cache row cb: [lo, hi) of slots, hi = s + (nodes in use); every
 // node's visible keys are inside.  Empty (lo = hi) where the sequence has no
 // node or its length or cache row is not in the cache.
 struct TreeRange {
@@ -44,11 +44,8 @@ struct TreeRange {
   bool bad;
 };
 
-__device__ __forceinline__ TreeRange tree_range(const TreeAttnParams& p, int b, unsigned long long used) {
+__device__ __forceinline__ TreeRange tree_range(const TreeAttnParams& p, int64_t s, int cb, unsigned long long used) {
   TreeRange r;
-  const int64_t s = p.seqlen[b];
-  int cb = b;
-  if (p.row_map != nullptr) cb = p.row_map[b];
   r.cb = cb;
   const int n = 64 - __clzll((long long)used);  // nodes up to the last one that is real or seen
   r.bad = s < 0 || s > p.T || cb < 0 || cb >= p.Bc || s + n > p.T;

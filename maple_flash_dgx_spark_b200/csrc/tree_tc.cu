@@ -8,7 +8,7 @@
 // memory (over the scores it came from) and V read as stored, [keys][dims], an
 // MN-major operand.  Each K/V row crosses HBM once per 256 rows.
 //
-// Roles (320 threads, one CTA per SM, persistent over work items): warp 9
+// Roles (384 threads, one CTA per SM, persistent over work items): warp 9
 // works the items out and streams K and V tiles by TMA into two rings; warp 8
 // issues the MMAs; two warpgroups of four warps do the softmax, a thread per
 // row.  Up to 128 rows (PAIR = false) both warpgroups share the row tile and
@@ -41,7 +41,7 @@ namespace mb {
 
 constexpr int kTtKeys = 128;   // keys per tile: MMA N of the scores, K of the output
 constexpr int kTtRows = 128;   // rows per tile: MMA M
-constexpr int kTtThreads = 320;
+constexpr int kTtThreads = 384;
 constexpr int kTtInfo = 2;     // items known ahead
 constexpr float kTtGrow = 8.0f;  // log2 growth of a row's maximum that rescales
 
@@ -72,8 +72,27 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ bool odd_bf16x2(uint32_t w) {  // a NaN or infinity in either half
-  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+// Not zero where either half is a NaN or an infinity (exponent bits all set).
+__device__ __forceinline__ uint32_t odd_bf16x2(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+
+// Two fp32 in one 64-bit register: a * b + c and a + b, each rounded once.
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void f2_get(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 // A barrier among warps on an mbarrier (one arrival per warp), so that a warp
 // that gave up cannot leave the others waiting for good.
@@ -98,26 +117,16 @@ struct TtView {
   int first;                 // first cached position seen
   bool real;
 };
-__device__ __forceinline__ void tt_bits(const TtView& v, int s, int k1, int t0, uint32_t (&w)[4]) {
-  const int a = max(0, v.first - t0), e = min(s, k1) - t0;  // cached: columns [a, e)
-  const int off = s - t0;                                   // column of node 0
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int lo = min(max(a - 32 * q, 0), 32), hi = min(max(e - 32 * q, 0), 32);
-    const uint32_t upto = hi >= 32 ? 0xffffffffu : (1u << hi) - 1u, from = lo >= 32 ? 0xffffffffu : (1u << lo) - 1u;
-    const int sh = 32 * q - off;  // node of this word's bit 0
-    uint32_t nb = 0;
-    if (sh >= 0 && sh < 64) nb = (uint32_t)(v.nodes >> sh);
-    else if (sh < 0 && sh > -32) nb = (uint32_t)(v.nodes << -sh);
-    w[q] = v.real ? (upto & ~from) | nb : 0u;
-  }
-  // nodes past the split's end belong to the next split
-  const int end = k1 - t0;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int hi = min(max(end - 32 * q, 0), 32);
-    w[q] &= hi >= 32 ? 0xffffffffu : (1u << hi) - 1u;
-  }
+// Columns 32 q .. 32 q + 31 of the tile at t0, one bit each.
+__device__ __forceinline__ uint32_t tt_low(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t tt_bits(const TtView& v, int s, int k1, int t0, int q) {
+  const int t = t0 + 32 * q;
+  const int sh = t - s;  // node of bit 0
+  uint32_t nb = 0;
+  if (sh >= 0 && sh < 64) nb = (uint32_t)(v.nodes >> sh);
+  else if (sh < 0 && sh > -32) nb = (uint32_t)(v.nodes << -sh);
+  const uint32_t cached = tt_low(s - t) & ~tt_low(v.first - t);
+  return v.real ? (cached | nb) & tt_low(k1 - t) : 0u;  // past the split's end: the next split's
 }
 
 template <int D, bool PAIR>
@@ -159,6 +168,9 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   pdl_trigger();
   bool ok = (smem_u32(smem) & 1023u) == 0;  // the swizzled tiles need it; the launch gives it
 
+  // 384 threads launch with 168 registers each (64512): 2 x 128 x 208 + 128 x 80 = 63488 of them
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
   if (warp == 9) {
     // -------------------------------------------------- items, K and V tiles --
     const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
@@ -166,6 +178,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
       const int rt = item % row_groups, sp = item / row_groups % p.NS, bh = item / row_groups / p.NS;
       const int h = bh % p.Hkv, b = bh / p.Hkv;
+      const int64_t len = p.seqlen[b];
+      const int cb = p.row_map != nullptr ? p.row_map[b] : b;
       unsigned long long m[2], used = 0;
       int dm = 0;
 #pragma unroll
@@ -178,7 +192,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       const unsigned ul = __reduce_or_sync(0xffffffffu, (unsigned)used);
       const unsigned uh = __reduce_or_sync(0xffffffffu, (unsigned)(used >> 32));
       dm = __reduce_max_sync(0xffffffffu, dm);
-      const TreeRange rg = tree_range(p, b, ((unsigned long long)uh << 32) | ul);
+      const TreeRange rg = tree_range(p, len, cb, ((unsigned long long)uh << 32) | ul);
       if (rg.bad && lane == 0) atomicOr(p.err, kErrFlagBounds);
       int k0, k1;
       tree_split(rg.lo, rg.hi, kTtKeys, p.NS, sp, k0, k1);
@@ -243,65 +257,87 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     __syncwarp();
   } else if (warp == 8) {
     // --------------------------------------------------------------- MMAs --
-    if (lane == 0) {
-      constexpr unsigned id_s = umma_idesc_bf16(kTtRows, kTtKeys, false), id_o = umma_idesc_bf16(kTtRows, D, true);
-      int kbase = 0, work = 0, pcount[2] = {0, 0};
-      for (int n = 0; ok; ++n) {
-        const int slot = n % kTtInfo;
-        ok = mbar_wait_bounded(&ifull[slot], (unsigned)((n / kTtInfo) & 1));
-        if (!ok) break;
-        const int tiles = info[slot].tiles;
-        mbar_arrive(&iempty[slot]);
-        if (tiles < 0) break;
-        if (tiles == 0) continue;
-        const int units = PAIR ? 2 * tiles : tiles;
-        auto scores = [&](int u) {
-          const int w = u & 1, g = kbase + (PAIR ? u >> 1 : u), st = g % NK;
-          if (!PAIR || w == 0) ok = mbar_wait_bounded(&kfull[st], (unsigned)((g / NK) & 1));
-          if (!ok) return;
-          tc_fence_after();
-          const unsigned qa = smem_u32(sq + (PAIR ? w : 0) * TILE), ka = smem_u32(sk + st * TILE);
+    // The whole warp walks the units and one elected lane issues: with values
+    // that are the same in all lanes the descriptors stay in uniform registers
+    // (built per lane, each MMA waited some 50 cycles for its operands' move).
+    constexpr unsigned id_s = umma_idesc_bf16(kTtRows, kTtKeys, false), id_o = umma_idesc_bf16(kTtRows, D, true);
+    const uint64_t dq = umma_desc_sw128(smem_u32(sq)), dk = umma_desc_sw128(smem_u32(sk)),
+                   dv = umma_desc_sw128_mn(smem_u32(sv), BOX);
+    int work = 0, ks = 0, kp = 0, vs = 0, vp = 0, pp[2] = {0, 0};  // ring stages and phases
+    for (int n = 0; ok; ++n) {
+      const int slot = n % kTtInfo;
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ifull[slot], (unsigned)((n / kTtInfo) & 1)));
+      if (!ok) break;
+      const int tiles = __shfl_sync(0xffffffffu, info[slot].tiles, 0);
+      __syncwarp();
+      if (elect_one()) mbar_arrive(&iempty[slot]);
+      if (tiles < 0) break;
+      if (tiles == 0) continue;
+      const int units = PAIR ? 2 * tiles : tiles;
+      auto scores = [&](int w) {
+        if (!PAIR || w == 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&kfull[ks], (unsigned)kp));
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t a = dq + (unsigned)((PAIR ? w : 0) * (TILE >> 4)), k = dk + (unsigned)(ks * (TILE >> 4));
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const unsigned o = (kk >> 2) * BOX + (kk & 3) * 32;
-            umma_bf16(tmem + w * kTtKeys, umma_desc_sw128(qa + o), umma_desc_sw128(ka + o), id_s, kk > 0);
+            const unsigned o = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
+            umma_bf16(tmem + w * kTtKeys, a + o, k + o, id_s, kk > 0);
           }
           umma_commit(&sfull[w]);
-          if (!PAIR || w == 1) umma_commit(&kempty[st]);
-        };
-        ok = mbar_wait_bounded(qfull, (unsigned)(work & 1));
-        if (ok) scores(0);
-        if (ok && units > 1) scores(1);
-        // the item before has read its output
-        if (ok && work > 0) ok = mbar_wait_bounded(oempty, (unsigned)((work - 1) & 1));
-        for (int u = 0; u < units && ok; ++u) {
-          const int w = u & 1, kt = PAIR ? u >> 1 : u, g = kbase + kt, st = g % NV;
-          ok = mbar_wait_bounded(&pready[w], (unsigned)(pcount[w] & 1));
-          ++pcount[w];
-          if (ok && (!PAIR || w == 0)) ok = mbar_wait_bounded(&vfull[st], (unsigned)((g / NV) & 1));
-          if (!ok) break;
-          tc_fence_after();
-          const unsigned va = smem_u32(sv + st * TILE);
+          if (!PAIR || w == 1) umma_commit(&kempty[ks]);
+        }
+        __syncwarp();
+        if (!PAIR || w == 1) {
+          if (++ks == NK) { ks = 0; kp ^= 1; }
+        }
+      };
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(qfull, (unsigned)(work & 1)));
+      if (ok) scores(0);
+      if (ok && units > 1) scores(1);
+      // the item before has read its output
+      if (ok && work > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(oempty, (unsigned)((work - 1) & 1)));
+      auto step = [&](int u, int w) {
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pready[w], (unsigned)pp[w]));
+        pp[w] ^= 1;
+        if (ok && (!PAIR || w == 0)) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&vfull[vs], (unsigned)vp));
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t v = dv + (unsigned)(vs * (TILE >> 4));
 #pragma unroll
           for (int kk = 0; kk < kTtKeys / 16; ++kk)
-            umma_bf16_ta(tmem + 2 * kTtKeys + w * D, tmem + w * kTtKeys + 8 * kk,
-                         umma_desc_sw128_mn(va + 2048 * kk, BOX), id_o, u >= 2 || kk > 0);
-          if (!PAIR || w == 1) umma_commit(&vempty[st]);
-          if (u + 2 < units) scores(u + 2);
+            umma_bf16_ta(tmem + 2 * kTtKeys + w * D, tmem + w * kTtKeys + 8 * kk, v + (unsigned)(128 * kk), id_o,
+                         u >= 2 || kk > 0);
+          if (!PAIR || w == 1) umma_commit(&vempty[vs]);
         }
-        if (ok) {
-          umma_commit(&ofull[0]);
-          umma_commit(&ofull[1]);
+        __syncwarp();
+        if (!PAIR || w == 1) {
+          if (++vs == NV) { vs = 0; vp ^= 1; }
         }
-        kbase += tiles;
-        ++work;
+        if (u + 2 < units) scores(w);
+      };
+      for (int u = 0; u < units && ok; u += 2) {
+        step(u, 0);
+        if (ok && u + 1 < units) step(u + 1, 1);
       }
+      if (ok && elect_one()) {
+        umma_commit(&ofull[0]);
+        umma_commit(&ofull[1]);
+      }
+      __syncwarp();
+      ++work;
+    }
+    if (elect_one()) {
       if (!ok) atomicOr(p.err, kErrFlagTimeout);
       umma_commit(drain);  // nothing of the tensor pipe is left behind
       mbar_wait_bounded(drain, 0);
     }
     __syncwarp();
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
     // ------------------------------------------------------------ softmax --
     const int w = warp >> 2, r = tid & 127;
     const unsigned lanes = (unsigned)(warp & 3) << 21;  // TMEM lane base of this warp, in bits 31:16
@@ -342,16 +378,26 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           constexpr int CH = D / 8;  // 16-byte chunks per row
           unsigned char* tile = sq + (PAIR ? w : 0) * TILE;
           const int t = PAIR ? r : tid, nt = PAIR ? 128 : 256, base = (PAIR ? 2 * it.rt + w : it.rt) * kTtRows;
-          for (int x = t; x < kTtRows * CH; x += nt) {
-            const int qr = x / CH, cc = x % CH, gr = base + qr;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (gr < rows) {
-              const int i = gr / p.G, g = gr - i * p.G;
-              v = ld_u4(static_cast<const char*>(p.q) +
-                        (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + g) * p.q_sh + cc * 8) * 2);
-              v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+          uint4 v[8];
+#pragma unroll 1
+          for (int x0 = t; x0 < kTtRows * CH; x0 += 8 * nt) {  // eight rows' chunks in flight per thread
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int x = x0 + e * nt, qr = x / CH, cc = x % CH, gr = base + qr;
+              v[e] = make_uint4(0u, 0u, 0u, 0u);
+              if (x < kTtRows * CH && gr < rows) {
+                const int i = gr / p.G, g = gr - i * p.G;
+                v[e] = ld_u4(static_cast<const char*>(p.q) +
+                             (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + g) * p.q_sh + cc * 8) * 2);
+              }
             }
-            *reinterpret_cast<uint4*>(tile + (cc >> 3) * BOX + qr * 128 + (((cc & 7) ^ (qr & 7)) << 4)) = v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int x = x0 + e * nt, qr = x / CH, cc = x % CH;
+              if (x < kTtRows * CH)
+                *reinterpret_cast<uint4*>(tile + (cc >> 3) * BOX + qr * 128 + (((cc & 7) ^ (qr & 7)) << 4)) =
+                    make_uint4(v[e].x ^ flip, v[e].y ^ flip, v[e].z ^ flip, v[e].w ^ flip);
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -371,27 +417,29 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             ok = mbar_wait_bounded(&vfull[st], (unsigned)((g / NV) & 1));
             ok = __all_sync(0xffffffffu, ok);
             if (ok) {
-              unsigned char* tile = sv + st * TILE;
-              constexpr int UNITS = TILE / 16;
-              bool found = false;
-              for (int x = PAIR ? tid : r; x < UNITS; x += PAIR ? 256 : 128) {
-                uint4* q = reinterpret_cast<uint4*>(tile) + x;
-                uint4 v = *q;
-                uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-                bool odd = false;
+              uint4* tile = reinterpret_cast<uint4*>(sv + st * TILE) + (PAIR ? tid : r);
+              constexpr int STEP = PAIR ? 256 : 128, UNITS = TILE / 16 / STEP;
+              uint32_t odd = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (odd_bf16x2(e[i])) {
-                    odd = true;
-                    if ((e[i] & 0x7f80u) == 0x7f80u) e[i] &= 0xffff0000u;
-                    if ((e[i] & 0x7f800000u) == 0x7f800000u) e[i] &= 0x0000ffffu;
+              for (int x = 0; x < UNITS; ++x) {
+                const uint4 v = tile[x * STEP];
+                odd |= odd_bf16x2(v.x) | odd_bf16x2(v.y) | odd_bf16x2(v.z) | odd_bf16x2(v.w);
+              }
+              if (odd) {  // rare
+#pragma unroll 1
+                for (int x = 0; x < UNITS; ++x) {
+                  uint4 v = tile[x * STEP];
+                  if (!(odd_bf16x2(v.x) | odd_bf16x2(v.y) | odd_bf16x2(v.z) | odd_bf16x2(v.w))) continue;
+                  uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const uint32_t y = odd_bf16x2(e[i]);
+                    e[i] &= ~((y >> 15 & 1u) * 0xffffu | (y >> 31) * 0xffff0000u);
                   }
-                if (odd) {
-                  *q = v;
-                  found |= t0 + (x % (BOX / 16)) / 8 < k1;
+                  tile[x * STEP] = make_uint4(e[0], e[1], e[2], e[3]);
+                  if (t0 + ((PAIR ? tid : r) + x * STEP) % (BOX / 16) / 8 < k1) it.fix = 1;
                 }
               }
-              if (found) it.fix = 1;
               fence_proxy_async_smem();
             }
             const bool met = PAIR ? tt_sync(both, n_both, lane) : tt_sync(&each[w], n_each, lane);
@@ -399,66 +447,85 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             if (!ok) break;
           }
           if (!idle) {
-            uint32_t bits[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-            if (mixed) tt_bits(view, s, k1, t0, bits);
-            // the scores are read twice from tensor memory, 64 columns at a time: 128 registers of them would spill
-            float top[4] = {ninf, ninf, ninf, ninf};
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t x[64];
-              tmem_ld32(t_s + 64 * q, x);
-              tmem_ld32(t_s + 64 * q + 32, x + 32);
-              tmem_wait32(x);
-              tmem_wait32(x + 32);
-              if (mixed) {
-#pragma unroll
-                for (int i = 0; i < 64; ++i)
-                  if (!((bits[2 * q + (i >> 5)] >> (i & 31)) & 1u)) x[i] = 0xff800000u;
-              }
-#pragma unroll
-              for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
-            }
-            const float tc = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-            const bool grow = tc > mc + kTtGrow || (mc == ninf && tc > ninf);
-            if (__any_sync(0xffffffffu, grow)) {
+            // a row's new maximum, and its output and sum brought to it where it has grown enough
+            auto settle = [&](float top) {
+              const float tc = top * c;
+              const bool grow = tc > mc + kTtGrow || (mc == ninf && tc > ninf);
+              if (!__any_sync(0xffffffffu, grow)) return;
               const float f = grow ? (mc == ninf ? 0.0f : ex2(mc - tc)) : 1.0f;
               if (grow) mc = tc;
               l *= f;
-              if (mine_units > 0) {
+              if (mine_units == 0) return;
+#pragma unroll 1
+              for (int q = 0; q < D / 32; ++q) {
+                uint32_t o[32];
+                tmem_ld32(t_o + w * D + 32 * q, o);
+                tmem_wait32(o);
 #pragma unroll
-                for (int q = 0; q < D / 32; ++q) {
-                  uint32_t o[32];
-                  tmem_ld32(t_o + w * D + 32 * q, o);
-                  tmem_wait32(o);
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                  tmem_st32(t_o + w * D + 32 * q, o);
-                }
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st32(t_o + w * D + 32 * q, o);
               }
-            }
-            const float sub = mc == ninf ? 0.0f : -mc;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            };
+            if (!mixed) {
+              uint32_t x[kTtKeys];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t x[64];
-              tmem_ld32(t_s + 64 * q, x);
-              tmem_ld32(t_s + 64 * q + 32, x + 32);
-              tmem_wait32(x);
-              tmem_wait32(x + 32);
+              for (int q = 0; q < 4; ++q) tmem_ld32(t_s + 32 * q, x + 32 * q);
+              float top[4] = {ninf, ninf, ninf, ninf};
 #pragma unroll
-              for (int i = 0; i < 64; i += 2) {
-                float a = ex2(fmaf(__uint_as_float(x[i]), c, sub)), e = ex2(fmaf(__uint_as_float(x[i + 1]), c, sub));
-                if (mixed) {
-                  if (!((bits[2 * q + (i >> 5)] >> (i & 31)) & 1u)) a = 0.0f;
-                  if (!((bits[2 * q + (i >> 5)] >> ((i + 1) & 31)) & 1u)) e = 0.0f;
-                }
-                sum[i & 2] += a;
-                sum[(i & 2) + 1] += e;
+              for (int q = 0; q < 4; ++q) {
+                tmem_wait32(x + 32 * q);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[32 * q + i]));
+              }
+              settle(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+              const float sub = mc == ninf ? 0.0f : -mc;
+              const uint64_t c2 = f2(c, c), sub2 = f2(sub, sub);
+              uint64_t sum[2] = {0, 0};
+#pragma unroll
+              for (int i = 0; i < kTtKeys; i += 2) {
+                float a, e;
+                f2_get(f2_fma(f2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), c2, sub2), a, e);
+                a = ex2(a);
+                e = ex2(e);
+                sum[(i >> 1) & 1] = f2_add(sum[(i >> 1) & 1], f2(a, e));
                 x[i >> 1] = bf16x2(a, e);
               }
-              tmem_st32(t_s + 32 * q, x);  // over scores that are read already
+              tmem_st32(t_s, x);
+              tmem_st32(t_s + 32, x + 32);
+              float a, e;
+              f2_get(f2_add(sum[0], sum[1]), a, e);
+              l += a + e;
+            } else {
+              float top = ninf;
+#pragma unroll 1
+              for (int q = 0; q < 4; ++q) {
+                uint32_t x[32];
+                tmem_ld32(t_s + 32 * q, x);
+                const uint32_t bits = tt_bits(view, s, k1, t0, q);
+                tmem_wait32(x);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) top = fmaxf(top, (bits >> i) & 1u ? __uint_as_float(x[i]) : ninf);
+              }
+              settle(top);
+              const float sub = mc == ninf ? 0.0f : -mc;
+              float sum = 0.0f;
+#pragma unroll 1
+              for (int q = 0; q < 4; ++q) {
+                uint32_t x[32];
+                tmem_ld32(t_s + 32 * q, x);
+                const uint32_t bits = tt_bits(view, s, k1, t0, q);
+                tmem_wait32(x);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                  const float a = (bits >> i) & 1u ? ex2(fmaf(__uint_as_float(x[i]), c, sub)) : 0.0f;
+                  const float e = (bits >> i) & 2u ? ex2(fmaf(__uint_as_float(x[i + 1]), c, sub)) : 0.0f;
+                  sum += a + e;
+                  x[i >> 1] = bf16x2(a, e);
+                }
+                tmem_st16(t_s + 16 * q, x);  // over scores that are read already
+              }
+              l += sum;
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_wait_st();
           }
           tc_fence_before();
@@ -492,7 +559,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       const float inv = zero ? 0.0f : 1.0f / l;
       const int64_t R = ((int64_t)b * p.Hkv + h) * rows + row;
       constexpr int COLS = PAIR ? D : D / 2;  // sharing the rows, each warpgroup writes half of the dimensions
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < COLS / 32; ++q) {
         const int col = (PAIR ? 0 : w * COLS) + 32 * q;
         uint32_t o[32];
@@ -515,13 +582,12 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           // NaN and infinities that were cleared, to the rows that see them
           const uint16_t* vb = static_cast<const uint16_t*>(p.vc) +
                                (p.row_map != nullptr ? p.row_map[b] : b) * p.c_sb + h * p.c_sh + col;
+#pragma unroll 1
           for (int t0 = k0; t0 < k1; t0 += kTtKeys) {
             if (!tt_mixed(it, t0, p.window)) continue;
-            uint32_t bits[4];
-            tt_bits(view, s, k1, t0, bits);
+#pragma unroll 1
             for (int x = 0; x < kTtKeys && t0 + x < k1; ++x) {
-              const uint32_t word = x < 64 ? (x < 32 ? bits[0] : bits[1]) : (x < 96 ? bits[2] : bits[3]);
-              if (!((word >> (x & 31)) & 1u)) continue;
+              if (!((tt_bits(view, s, k1, t0, x >> 5) >> (x & 31)) & 1u)) continue;
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 const uint16_t y = vb[(int64_t)(t0 + x) * D + i];
