@@ -489,7 +489,7 @@ int maple_tree_plan(const int32_t* parents, int64_t batch, int64_t nodes, int64_
  * or contents.  The workspace needs no initial value and is free again when
  * the call's work is done; concurrent calls need their own. */
 int64_t maple_tree_gqa_workspace_bytes(int64_t batch, int64_t nodes, int64_t num_heads, int64_t num_kv_heads,
-                                       int64_t head_dim, int64_t max_len, int x_dtype);
+                                       int64_t head_dim, int64_t max_len, int64_t window, int x_dtype);
 int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, int64_t nodes, int64_t num_heads, int64_t q_sb,
                         int64_t q_sn, int64_t q_sh, const void* k_cache, const void* v_cache, int64_t cache_batch,
                         int64_t num_kv_heads, int64_t cache_sb, int64_t cache_sh, int64_t max_len, int64_t head_dim,

@@ -365,11 +365,20 @@ inline bool tree_use_tc(int x_dtype, int64_t head_dim) {
 }
 
 inline int tree_splits(int64_t batch, int64_t nodes, int64_t num_heads, int64_t num_kv_heads, int64_t max_len,
-                       int x_dtype, int64_t head_dim) {
+                       int x_dtype, int64_t head_dim, int64_t window) {
+  if (window > 0 && window + nodes < max_len) max_len = window + nodes;  // no row's keys span more
   if (tree_use_tc(x_dtype, head_dim))
     return tree_tc_splits(batch * num_kv_heads * tree_tc_groups(nodes * (num_heads / num_kv_heads)), max_len);
   const int64_t tiles = (nodes * (num_heads / num_kv_heads) + kSimtRows - 1) / kSimtRows;
   return tree_simt_splits(batch * num_kv_heads * tiles, max_len);
+}
+
+// Rows of partials per split and KV head, and the bytes of all of them.
+inline int64_t tree_partial_rows(int64_t rows, int x_dtype, int64_t head_dim) {
+  return tree_use_tc(x_dtype, head_dim) ? tree_tc_partial_rows(rows) : rows;
+}
+inline int64_t tree_partial_bytes(int64_t batch, int64_t num_kv_heads, int64_t rows, int64_t ns, int64_t head_dim) {
+  return ns <= 1 ? 0 : batch * num_kv_heads * rows * ns * (head_dim + 2) * 4;
 }
 
 }  // namespace mb
@@ -389,12 +398,13 @@ extern "C" int maple_tree_plan(const int32_t* parents, int64_t batch, int64_t no
 
 extern "C" int64_t maple_tree_gqa_workspace_bytes(int64_t batch, int64_t nodes, int64_t num_heads,
                                                   int64_t num_kv_heads, int64_t head_dim, int64_t max_len,
-                                                  int x_dtype) {
+                                                  int64_t window, int x_dtype) {
   if (batch <= 0 || nodes <= 0 || nodes > kTreeMaxNodes || num_heads <= 0 || num_kv_heads <= 0 ||
-      num_heads % num_kv_heads || head_dim <= 0 || max_len <= 0)
+      num_heads % num_kv_heads || head_dim <= 0 || max_len <= 0 || window < 0)
     return -1;
-  const int64_t ns = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim);
-  return ns <= 1 ? 0 : batch * num_heads * nodes * ns * (head_dim + 2) * 4;
+  const int64_t ns = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim, window);
+  const int64_t rows = tree_partial_rows(nodes * (num_heads / num_kv_heads), x_dtype, head_dim);
+  return tree_partial_bytes(batch, num_kv_heads, rows, ns, head_dim);
 }
 
 extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, int64_t nodes, int64_t num_heads,
@@ -427,11 +437,12 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   p.scale = scale;
   const int64_t rows = (int64_t)p.N * p.G, tiles = (rows + kSimtRows - 1) / kSimtRows;
   if (num_kv_heads * tiles > 65535) return kErrShape;
-  p.NS = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim);
-  const int64_t need = p.NS <= 1 ? 0 : batch * num_heads * nodes * p.NS * (head_dim + 2) * 4;
+  p.NS = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim, window);
+  const int64_t prows = tree_partial_rows(rows, x_dtype, head_dim);
+  const int64_t need = tree_partial_bytes(batch, num_kv_heads, prows, p.NS, head_dim);
   if (need > 0 && (!workspace || workspace_bytes < need)) return kErrWorkspace;
   p.ws_acc = static_cast<float*>(workspace);
-  p.ws_ml = p.ws_acc ? p.ws_acc + batch * num_heads * nodes * p.NS * head_dim : nullptr;
+  p.ws_ml = p.ws_acc ? p.ws_acc + batch * num_kv_heads * prows * p.NS * head_dim : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
 #define MB_TREE(XT, DD)                                                                                              \
@@ -448,10 +459,6 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   if (tree_use_tc(x_dtype, head_dim)) {
     if (batch * num_kv_heads * p.NS * tree_tc_groups(rows) > (1LL << 30)) return kErrShape;
     e = tree_tc_launch(p, (int)head_dim, st);
-    const dim3 grid((unsigned)((num_kv_heads * rows + 7) / 8), (unsigned)batch);
-    if (e == cudaSuccess && p.NS > 1)
-      e = head_dim == 64 ? launch_k(tree_merge_kernel<kBF16, 64>, grid, dim3(256), 0, st, p, tree_tc_tile())
-                         : launch_k(tree_merge_kernel<kBF16, 128>, grid, dim3(256), 0, st, p, tree_tc_tile());
   } else if (x_dtype == kBF16) {
     MB_TREE(kBF16, 256);
   } else {

@@ -28,8 +28,8 @@ struct TreeAttnParams {
   const unsigned long long* mask;  // [B, N]
   const int32_t* row_map;     // [B] cache row, or null: b
   void* out;                  // [B, N, H, D] contiguous
-  float* ws_acc;              // [B * Hkv * N * G, NS, D] unnormalised partial sums
-  float* ws_ml;               // [B * Hkv * N * G, NS, 2] maximum, sum of weights
+  float* ws_acc;              // unnormalised partial sums of each row, split and dim
+  float* ws_ml;               // maximum and sum of weights of each row and split
   int* err;
   int64_t q_sb, q_sn, q_sh, c_sb, c_sh;
   int B, N, H, Hkv, G, Bc, T, NS, window;
@@ -81,7 +81,7 @@ __device__ __forceinline__ int tree_splits_used(int lo, int hi, int tile, int ns
 // tree_tc.cu: the tcgen05 kernel (bf16, heads of 64 or 128).
 int tree_tc_splits(int64_t ctas, int64_t max_len);
 int tree_tc_groups(int64_t rows);
-int tree_tc_tile();
+int64_t tree_tc_partial_rows(int64_t rows);  // rows that a split's partials take
 cudaError_t tree_tc_launch(const TreeAttnParams& p, int D, cudaStream_t st);
 
 }  // namespace mb

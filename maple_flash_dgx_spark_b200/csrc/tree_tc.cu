@@ -48,7 +48,7 @@ constexpr float kTtGrow = 8.0f;  // log2 growth of a row's maximum that rescales
 struct TtItem {
   int b, h, rt, sp;     // sequence, KV head, row tile (pair), split
   int s, lo, k0, k1;    // cached positions, the row's first key, this split's keys
-  int tiles, alone, fix, dmax;  // key tiles; the only split; V was cleared; largest depth
+  int item, tiles, alone, fix, dmax;  // key tiles; the only split; V was cleared; largest depth
   unsigned long long mask[kTreeMaxNodes];
 };
 
@@ -94,6 +94,12 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // A barrier among warps on an mbarrier (one arrival per warp), so that a warp
 // that gave up cannot leave the others waiting for good.
 __device__ __forceinline__ bool tt_sync(uint64_t* bar, int& count, int lane) {
@@ -143,7 +149,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   float2* s_ml = reinterpret_cast<float2*>(sq);  // [2][128] maximum and sum, once the queries are done with
   uint64_t* bars = reinterpret_cast<uint64_t*>(info + kTtInfo);
   uint64_t *kfull = bars, *kempty = kfull + NK, *vfull = kempty + NK, *vempty = vfull + NV, *sfull = vempty + NV,
-           *pready = sfull + 2, *ofull = pready + 2, *oempty = ofull + 2, *qfull = oempty + 1, *ifull = qfull + 1,
+           *phalf = sfull + 2, *pready = phalf + 2, *ofull = pready + 2, *oempty = ofull + 2, *qfull = oempty + 1, *ifull = qfull + 1,
            *iempty = ifull + kTtInfo, *both = iempty + kTtInfo, *each = both + 1, *drain = each + 2;
   unsigned* s_tmem = reinterpret_cast<unsigned*>(drain + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -152,7 +158,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < NK; ++i) { mbar_init(&kfull[i], 1); mbar_init(&kempty[i], 1); }
     for (int i = 0; i < NV; ++i) { mbar_init(&vfull[i], 1); mbar_init(&vempty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&sfull[i], 1); mbar_init(&pready[i], 4); mbar_init(&ofull[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&sfull[i], 1); mbar_init(&phalf[i], 4); mbar_init(&pready[i], 4); mbar_init(&ofull[i], 1); }
     mbar_init(oempty, 8);
     mbar_init(qfull, 8);
     for (int i = 0; i < kTtInfo; ++i) { mbar_init(&ifull[i], 1); mbar_init(&iempty[i], 9); }
@@ -204,7 +210,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       it.mask[lane] = m[0];
       it.mask[lane + 32] = m[1];
       if (lane == 0) {
-        it.b = b; it.h = h; it.rt = rt; it.sp = sp;
+        it.item = item; it.b = b; it.h = h; it.rt = rt; it.sp = sp;
         it.s = rg.s; it.lo = rg.lo; it.k0 = k0; it.k1 = k1; it.tiles = tiles; it.fix = 0; it.dmax = dm;
         it.alone = tree_splits_used(rg.lo, rg.hi, kTtKeys, p.NS) <= 1;
       }
@@ -299,19 +305,28 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       // the item before has read its output
       if (ok && work > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(oempty, (unsigned)((work - 1) & 1)));
       auto step = [&](int u, int w) {
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pready[w], (unsigned)pp[w]));
-        pp[w] ^= 1;
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&phalf[w], (unsigned)pp[w]));
         if (ok && (!PAIR || w == 0)) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&vfull[vs], (unsigned)vp));
         if (!ok) return;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t v = dv + (unsigned)(vs * (TILE >> 4));
+        const uint64_t v = dv + (unsigned)(vs * (TILE >> 4));
+        auto half = [&](int k0) {
+          tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kTtKeys / 16; ++kk)
-            umma_bf16_ta(tmem + 2 * kTtKeys + w * D, tmem + w * kTtKeys + 8 * kk, v + (unsigned)(128 * kk), id_o,
-                         u >= 2 || kk > 0);
-          if (!PAIR || w == 1) umma_commit(&vempty[vs]);
-        }
+            for (int k = 0; k < kTtKeys / 32; ++k) {
+              const int kk = k0 + k;
+              umma_bf16_ta(tmem + 2 * kTtKeys + w * D, tmem + w * kTtKeys + 8 * kk, v + (unsigned)(128 * kk), id_o,
+                           u >= 2 || kk > 0);
+            }
+          }
+          __syncwarp();
+        };
+        half(0);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pready[w], (unsigned)pp[w]));
+        pp[w] ^= 1;
+        if (!ok) return;
+        half(kTtKeys / 32);
+        if ((!PAIR || w == 1) && elect_one()) umma_commit(&vempty[vs]);
         __syncwarp();
         if (!PAIR || w == 1) {
           if (++vs == NV) { vs = 0; vp ^= 1; }
@@ -343,11 +358,31 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     const unsigned lanes = (unsigned)(warp & 3) << 21;  // TMEM lane base of this warp, in bits 31:16
     const unsigned t_s = tmem + lanes + w * kTtKeys, t_o = tmem + lanes + 2 * kTtKeys;
     const float ninf = __int_as_float(0xff800000);
-    const float c = fabsf(p.scale) * 1.44269504088896341f;
+    // above 0, so that a masked score of -inf stays one under scale 0
+    const float c = fmaxf(fabsf(p.scale) * 1.44269504088896341f, 1e-30f);
     const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;  // the queries carry the scale's sign
     const int rows = p.N * p.G;
+    // row / G by a multiplication: exact while row x G < 2^32
+    const uint64_t per_g = (1ull << 32) / (unsigned)p.G + 1;
+    auto tt_node = [&](int x) { return (int)((uint64_t)(unsigned)x * per_g >> 32); };
     int kbase = 0, work = 0, scount = 0, n_both = 0, n_each = 0;
+    constexpr int CH = D / 8, QT = PAIR ? 128 : 256, QN = kTtRows * CH / QT;  // Q's 16-byte chunks per row, per thread
+    int guess = (int)blockIdx.x;  // the next item, if it has keys
     for (int n = 0; ok; ++n) {
+      // the guessed item's Q rows come near under the wait: they depend on its number alone
+      if (guess < items) {
+        const int bh = guess / row_groups / p.NS;
+        constexpr int LINES = D / 64;  // 128 bytes each
+        for (int x = PAIR ? r : tid; x < kTtRows * LINES; x += QT) {
+          const int gr = (PAIR ? 2 * (guess % row_groups) + w : guess % row_groups) * kTtRows + x / LINES;
+          if (gr < rows) {
+            const int i = tt_node(gr), g = gr - i * p.G;
+            asm volatile("prefetch.global.L1 [%0];\n" ::"l"(
+                static_cast<const char*>(p.q) + (bh / p.Hkv * p.q_sb + i * p.q_sn +
+                                                 (int64_t)(bh % p.Hkv * p.G + g) * p.q_sh + x % LINES * 64) * 2));
+          }
+        }
+      }
       const int slot = n % kTtInfo;
       ok = mbar_wait_bounded(&ifull[slot], (unsigned)((n / kTtInfo) & 1));
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
@@ -356,7 +391,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       if (tiles < 0) break;
       const int b = it.b, h = it.h, s = it.s, k0 = it.k0, k1 = it.k1;
       const int row = (PAIR ? 2 * it.rt + w : it.rt) * kTtRows + r;
-      const int node = row / p.G, head = h * p.G + row - node * p.G;
+      const int node = tt_node(row), head = h * p.G + row - node * p.G;
       TtView view{};
       const unsigned long long mine = row < rows ? it.mask[node] : 0ull;
       view.real = mine != 0;
@@ -373,36 +408,29 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       float mc = ninf, l = 0.0f;  // maximum times c, sum of weights
       int mine_units = 0;
       if (tiles > 0) {
-        // Q, 128-byte swizzled: the WG's own tile, or both WGs half of the shared one
-        {
-          constexpr int CH = D / 8;  // 16-byte chunks per row
-          unsigned char* tile = sq + (PAIR ? w : 0) * TILE;
-          const int t = PAIR ? r : tid, nt = PAIR ? 128 : 256, base = (PAIR ? 2 * it.rt + w : it.rt) * kTtRows;
-          uint4 v[8];
-#pragma unroll 1
-          for (int x0 = t; x0 < kTtRows * CH; x0 += 8 * nt) {  // eight rows' chunks in flight per thread
+        // Q, 128-byte swizzled: the warpgroup's own tile, or half of the shared one each
+        guess = it.item + (int)gridDim.x;
+        uint4 qv[QN];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int x = x0 + e * nt, qr = x / CH, cc = x % CH, gr = base + qr;
-              v[e] = make_uint4(0u, 0u, 0u, 0u);
-              if (x < kTtRows * CH && gr < rows) {
-                const int i = gr / p.G, g = gr - i * p.G;
-                v[e] = ld_u4(static_cast<const char*>(p.q) +
-                             (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + g) * p.q_sh + cc * 8) * 2);
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int x = x0 + e * nt, qr = x / CH, cc = x % CH;
-              if (x < kTtRows * CH)
-                *reinterpret_cast<uint4*>(tile + (cc >> 3) * BOX + qr * 128 + (((cc & 7) ^ (qr & 7)) << 4)) =
-                    make_uint4(v[e].x ^ flip, v[e].y ^ flip, v[e].z ^ flip, v[e].w ^ flip);
-            }
+        for (int e = 0; e < QN; ++e) {
+          const int x = (PAIR ? r : tid) + e * QT, gr = (PAIR ? 2 * it.rt + w : it.rt) * kTtRows + x / CH;
+          qv[e] = make_uint4(0u, 0u, 0u, 0u);
+          if (gr < rows) {
+            const int i = tt_node(gr), g = gr - i * p.G;
+            qv[e] = ld_u4(static_cast<const char*>(p.q) +
+                          (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + g) * p.q_sh + x % CH * 8) * 2);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(qfull);
         }
+        unsigned char* tile = sq + (PAIR ? w : 0) * TILE;
+#pragma unroll
+        for (int e = 0; e < QN; ++e) {
+          const int x = (PAIR ? r : tid) + e * QT, qr = x / CH, cc = x % CH;
+          *reinterpret_cast<uint4*>(tile + (cc >> 3) * BOX + qr * 128 + (((cc & 7) ^ (qr & 7)) << 4)) =
+              make_uint4(qv[e].x ^ flip, qv[e].y ^ flip, qv[e].z ^ flip, qv[e].w ^ flip);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qfull);
         const bool idle = __all_sync(0xffffffffu, row >= rows);  // this warp has no row: it only keeps step
         for (int kt = PAIR ? 0 : w; kt < tiles && ok; kt += PAIR ? 1 : 2, ++mine_units) {
           ok = mbar_wait_bounded(&sfull[w], (unsigned)(scount & 1));
@@ -466,67 +494,57 @@ __global__ void __launch_bounds__(kTtThreads, 1)
                 tmem_st32(t_o + w * D + 32 * q, o);
               }
             };
-            if (!mixed) {
-              uint32_t x[kTtKeys];
+            uint32_t x[kTtKeys];
 #pragma unroll
-              for (int q = 0; q < 4; ++q) tmem_ld32(t_s + 32 * q, x + 32 * q);
-              float top[4] = {ninf, ninf, ninf, ninf};
+            for (int q = 0; q < 4; ++q) tmem_ld32(t_s + 32 * q, x + 32 * q);
+            uint32_t bits[4];
+            if (mixed) {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                tmem_wait32(x + 32 * q);
+              for (int q = 0; q < 4; ++q) bits[q] = tt_bits(view, s, k1, t0, q);
+            }
+            float top[4] = {ninf, ninf, ninf, ninf};
 #pragma unroll
-                for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[32 * q + i]));
+            for (int q = 0; q < 4; ++q) {
+              tmem_wait32(x + 32 * q);
+              if (mixed) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[32 * q + i] = (bits[q] >> i) & 1u ? x[32 * q + i] : 0xff800000u;
               }
-              settle(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-              const float sub = mc == ninf ? 0.0f : -mc;
-              const uint64_t c2 = f2(c, c), sub2 = f2(sub, sub);
-              uint64_t sum[2] = {0, 0};
 #pragma unroll
-              for (int i = 0; i < kTtKeys; i += 2) {
+              for (int i = 0; i < 32; i += 2)
+                top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], __uint_as_float(x[32 * q + i]), __uint_as_float(x[32 * q + i + 1]));
+            }
+            settle(max3(fmaxf(top[0], top[1]), top[2], top[3]));
+            const float sub = mc == ninf ? 0.0f : -mc;
+            const uint64_t c2 = f2(c, c), sub2 = f2(sub, sub);
+            uint64_t sum[2] = {0, 0};
+            // the product starts on the first half of the weights while the second is formed
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+              for (int i = 64 * hf; i < 64 * hf + 64; i += 2) {
+                const uint64_t y = f2_fma(f2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), c2, sub2);
                 float a, e;
-                f2_get(f2_fma(f2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), c2, sub2), a, e);
+                f2_get(y, a, e);
                 a = ex2(a);
                 e = ex2(e);
                 sum[(i >> 1) & 1] = f2_add(sum[(i >> 1) & 1], f2(a, e));
                 x[i >> 1] = bf16x2(a, e);
               }
-              tmem_st32(t_s, x);
-              tmem_st32(t_s + 32, x + 32);
-              float a, e;
-              f2_get(f2_add(sum[0], sum[1]), a, e);
-              l += a + e;
-            } else {
-              float top = ninf;
-#pragma unroll 1
-              for (int q = 0; q < 4; ++q) {
-                uint32_t x[32];
-                tmem_ld32(t_s + 32 * q, x);
-                const uint32_t bits = tt_bits(view, s, k1, t0, q);
-                tmem_wait32(x);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) top = fmaxf(top, (bits >> i) & 1u ? __uint_as_float(x[i]) : ninf);
+              tmem_st32(t_s + 32 * hf, x + 32 * hf);
+              if (hf == 0) {
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&phalf[w]);
               }
-              settle(top);
-              const float sub = mc == ninf ? 0.0f : -mc;
-              float sum = 0.0f;
-#pragma unroll 1
-              for (int q = 0; q < 4; ++q) {
-                uint32_t x[32];
-                tmem_ld32(t_s + 32 * q, x);
-                const uint32_t bits = tt_bits(view, s, k1, t0, q);
-                tmem_wait32(x);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                  const float a = (bits >> i) & 1u ? ex2(fmaf(__uint_as_float(x[i]), c, sub)) : 0.0f;
-                  const float e = (bits >> i) & 2u ? ex2(fmaf(__uint_as_float(x[i + 1]), c, sub)) : 0.0f;
-                  sum += a + e;
-                  x[i >> 1] = bf16x2(a, e);
-                }
-                tmem_st16(t_s + 16 * q, x);  // over scores that are read already
-              }
-              l += sum;
             }
+            float a, e;
+            f2_get(f2_add(sum[0], sum[1]), a, e);
+            l += a + e;
             tmem_wait_st();
+          } else if (lane == 0) {
+            mbar_arrive(&phalf[w]);
           }
           tc_fence_before();
           __syncwarp();
@@ -555,9 +573,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         l = la + lb;
         mc = M;
       }
-      const bool zero = !(row < rows && mine != 0) || l == 0.0f;
+      const bool zero = !(row < rows && mine != 0) || mc == ninf;
       const float inv = zero ? 0.0f : 1.0f / l;
-      const int64_t R = ((int64_t)b * p.Hkv + h) * rows + row;
+      // partials [item][dim][row of the tile]: a warp's 32 rows store side by side
+      const int64_t part = (((int64_t)b * p.Hkv + h) * p.NS + it.sp) * ((rows + kTtRows - 1) / kTtRows) + row / kTtRows;
       constexpr int COLS = PAIR ? D : D / 2;  // sharing the rows, each warpgroup writes half of the dimensions
 #pragma unroll 1
       for (int q = 0; q < COLS / 32; ++q) {
@@ -608,18 +627,15 @@ __global__ void __launch_bounds__(kTtThreads, 1)
               dst[i] = make_uint4(y[0], y[1], y[2], y[3]);
             }
           } else {
-            float4* dst = reinterpret_cast<float4*>(p.ws_acc + (R * p.NS + it.sp) * D + col);
+            float* dst = p.ws_acc + (part * D + col) * kTtRows + r;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dst[i] = zero ? make_float4(0.f, 0.f, 0.f, 0.f)
-                            : make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            for (int i = 0; i < 32; ++i) dst[i * kTtRows] = zero ? 0.0f : v[i];
           }
         }
       }
-      if (!it.alone && row < rows && (PAIR || w == 0)) {
-        p.ws_ml[(R * p.NS + it.sp) * 2] = zero ? ninf : mc * 0.693147180559945309f;
-        p.ws_ml[(R * p.NS + it.sp) * 2 + 1] = zero ? 0.0f : l;
-      }
+      if (!it.alone && row < rows && (PAIR || w == 0))
+        reinterpret_cast<float2*>(p.ws_ml)[part * kTtRows + r] =
+            zero ? make_float2(ninf, 0.0f) : make_float2(mc * 0.693147180559945309f, l);
       tc_fence_before();
       __syncwarp();
       if (tiles > 0) {
@@ -636,6 +652,74 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+// Joins the splits: M = max m_j, out = sum e^(m_j - M) acc_j / sum e^(m_j - M)
+// l_j, in split order.  A CTA takes 32 rows (the lanes, as the partials lie) x
+// 32 dims (four per warp); eight splits' loads are in flight at a time.
+template <int D>
+__global__ void __launch_bounds__(256) tree_tc_merge_kernel(TreeAttnParams p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = p.N * p.G, rtiles = (rows + kTtRows - 1) / kTtRows;
+  const int h = blockIdx.y, b = blockIdx.z, rb = blockIdx.x / (D / 32), col = (blockIdx.x % (D / 32)) * 32 + warp * 4;
+  const int row = rb * 32 + lane;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t len = p.seqlen[b];
+  const int cb = p.row_map != nullptr ? p.row_map[b] : b;
+  const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
+  unsigned long long used = 0;
+  for (int i = lane; i < p.N; i += 32) {
+    const unsigned long long mi = p.mask[(int64_t)b * p.N + i] & keep;
+    used |= mi | (mi ? 1ull << i : 0ull);
+  }
+  const unsigned ul = __reduce_or_sync(0xffffffffu, (unsigned)used);
+  const unsigned uh = __reduce_or_sync(0xffffffffu, (unsigned)(used >> 32));
+  const TreeRange rg = tree_range(p, len, cb, ((unsigned long long)uh << 32) | ul);
+  const int ns = tree_splits_used(rg.lo, rg.hi, kTtKeys, p.NS);
+  if (row >= rows || ns <= 1) return;  // one split wrote its output itself
+  const int64_t first = ((int64_t)b * p.Hkv + h) * p.NS * rtiles + row / kTtRows;  // this row's tile in split 0
+  const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + first * kTtRows + row % kTtRows;
+  const float* ac = p.ws_acc + (first * D + col) * kTtRows + row % kTtRows;
+  const int64_t step_ml = (int64_t)rtiles * kTtRows, step_ac = (int64_t)rtiles * D * kTtRows;
+  const float ninf = __int_as_float(0xff800000);
+  constexpr int kB = 8;
+  float M = ninf;
+  for (int j0 = 0; j0 < ns; j0 += kB) {
+    float m[kB];
+#pragma unroll
+    for (int i = 0; i < kB; ++i) m[i] = j0 + i < ns ? __ldcg(ml + (j0 + i) * step_ml).x : ninf;
+#pragma unroll
+    for (int i = 0; i < kB; ++i) M = fmaxf(M, m[i]);
+  }
+  const float base = M == ninf ? 0.0f : M;
+  float den = 0.0f, num[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int j0 = 0; j0 < ns; j0 += kB) {
+    float2 y[kB];
+    float a[kB][4];
+#pragma unroll
+    for (int i = 0; i < kB; ++i) {
+      if (j0 + i < ns) {
+        y[i] = __ldcg(ml + (j0 + i) * step_ml);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) a[i][u] = __ldcg(ac + (j0 + i) * step_ac + u * kTtRows);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kB; ++i) {
+      if (j0 + i < ns && !(y[i].x == ninf && y[i].y == 0.0f)) {  // not a split that this row sees nothing of
+        const float w = mexp(y[i].x - base);
+        den = fmaf(w, y[i].y, den);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) num[u] = fmaf(w, a[i][u], num[u]);
+      }
+    }
+  }
+  const int node = row / p.G, g = row - node * p.G;
+  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+  uint2 out = make_uint2(0u, 0u);
+  if (den != 0.0f) out = make_uint2(bf16x2(num[0] * inv, num[1] * inv), bf16x2(num[2] * inv, num[3] * inv));
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (((int64_t)b * p.N + node) * p.H + h * p.G + g) * D + col) = out;
 }
 
 // Splits of a sequence's keys.  Few items leave SMs idle, more splits cost a
@@ -659,7 +743,7 @@ int tree_tc_splits(int64_t ctas, int64_t max_len) {
 
 int tree_tc_groups(int64_t rows) { return rows <= kTtRows ? 1 : (int)((rows + 2 * kTtRows - 1) / (2 * kTtRows)); }
 
-int tree_tc_tile() { return kTtKeys; }
+int64_t tree_tc_partial_rows(int64_t rows) { return (rows + kTtRows - 1) / kTtRows * kTtRows; }
 
 template <int D, bool PAIR>
 cudaError_t tree_tc_launch1(const TreeAttnParams& p, int groups, const CUtensorMap& tmk, const CUtensorMap& tmv,
@@ -667,10 +751,14 @@ cudaError_t tree_tc_launch1(const TreeAttnParams& p, int groups, const CUtensorM
   constexpr int smem = TtShape<D, PAIR>::kSmem;
   static_assert(smem <= 232448, "shared memory of one SM");
   const int items = p.B * p.Hkv * p.NS * groups;
-  const cudaError_t e = cudaFuncSetAttribute(tree_tc_kernel<D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  return launch_k(tree_tc_kernel<D, PAIR>, dim3((unsigned)(items < 148 ? items : 148)), dim3(kTtThreads), smem, st, p,
-                  groups, items, tmk, tmv);
+  cudaError_t e = cudaFuncSetAttribute(tree_tc_kernel<D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess)
+    e = launch_k(tree_tc_kernel<D, PAIR>, dim3((unsigned)(items < 148 ? items : 148)), dim3(kTtThreads), smem, st, p,
+                 groups, items, tmk, tmv);
+  if (e == cudaSuccess && p.NS > 1)
+    e = launch_k(tree_tc_merge_kernel<D>,
+                 dim3((unsigned)((p.N * p.G + 31) / 32 * (D / 32)), (unsigned)p.Hkv, (unsigned)p.B), dim3(256), 0, st, p);
+  return e;
 }
 
 cudaError_t tree_tc_launch(const TreeAttnParams& p, int D, cudaStream_t st) {

@@ -24,7 +24,10 @@ namespace mb {
 
 constexpr int kVerMaxK = 64;
 constexpr int kVerMaxNodes = 64;
-constexpr int kVerThreads = 512;
+constexpr int kVerThreads = 256;
+constexpr int kVerVecs = 8;      // 16-byte vectors per thread and tile
+constexpr int kVerCap = 128;     // candidates that a tile may hand on
+constexpr int kVerBatch = 4096;  // candidates that a row's selection holds at a time
 
 struct VerifyParams {
   const void* logits;     // [B, N, V], V contiguous
@@ -32,15 +35,19 @@ struct VerifyParams {
   const int32_t* parents; // [B, N]
   const float* uniform;   // [B, N]
   const void* draft;      // [B, N, V] or null, V contiguous
+  uint2* cand;            // [B * N, tiles, kVerCap] candidates: key, id
+  int32_t* n_cand;        // [B * N, tiles]
   double* w;              // [B * N, 64] kept weights, falling
   int32_t* id;            // [B * N, 64] their token ids
+  float* q;               // [B * N, 64] the draft's probabilities of them
+  float* raw;             // [B * N] the draft's probability of the node's token at its parent
   int32_t* path;          // [B, N]
   int32_t* n_path;        // [B]
   int64_t* out;           // [B, N]
   int* err;
   int64_t l_sb, l_sn, d_sb, d_sn;
   double inv_t, top_p;
-  int B, N, V, K, replacement;
+  int B, N, V, K, tiles, replacement;
 };
 
 // Order-preserving word of a logit: larger logit, larger word; NaN as -inf,
@@ -103,94 +110,367 @@ __device__ __forceinline__ void node_weights(const VerifyParams& p, const uint32
   }
 }
 
-// One CTA per node: its K largest logits by radix selection.  Four passes of
-// 8 bits over the row (from L2 after the first) find the K-th largest word;
-// a last pass collects what is above it and the lowest ids of its ties.
+// ------------------------------------------------------------- tile kernel --
+// The logits are read once.  A CTA holds a tile of a row in registers (eight
+// 16-byte vectors per thread, all in flight together) and hands on what may be
+// among the row's K largest: T = the K-th largest of the 256 threads' maxima is
+// at most the tile's K-th largest logit, and few logits reach it (about K of
+// 16384: threads seldom hold two), so one comparison per thread and a scan in
+// those that pass find them.  T is found bit by bit, one warp counting the
+// maxima with votes.  Where more than kVerCap reach T (ties, large logits side
+// by side) the tile's K largest are selected exactly, ties to the lowest ids.
+__device__ __forceinline__ uint4 ld_once_u4(const void* p) {  // written by the launch before: not the read-only path
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+
 template <int XT>
-__global__ void __launch_bounds__(kVerThreads) verify_topk_kernel(VerifyParams p) {
-  __shared__ unsigned hist[256];
-  __shared__ unsigned s_prefix, s_need, s_count, s_ties;
-  __shared__ uint32_t ck[kVerMaxK], sk[kVerMaxK];
-  __shared__ int ci[kVerMaxK], si[kVerMaxK];
-  __shared__ unsigned wcount[kVerThreads / 32];
+__device__ __forceinline__ float tile_value(const uint4& r, int e) {
+  if constexpr (XT == kBF16) {
+    const uint32_t w = e < 4 ? (e < 2 ? r.x : r.y) : (e < 6 ? r.z : r.w);
+    return __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
+  } else {
+    return __uint_as_float(e < 2 ? (e == 0 ? r.x : r.y) : (e == 2 ? r.z : r.w));
+  }
+}
+template <int XT>
+__device__ __forceinline__ uint32_t clean_word(uint32_t w) {  // NaN to -inf: the other operand of a maximum
+  if constexpr (XT == kBF16) {
+    asm("max.bf16x2 %0, %0, %1;\n" : "+r"(w) : "r"(0xff80ff80u));
+    return w;
+  } else {
+    return __float_as_uint(fmaxf(__uint_as_float(w), __int_as_float(0xff800000)));
+  }
+}
+template <int XT>
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
+  if constexpr (XT == kBF16) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  } else {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+}
+
+template <int XT>
+__global__ void __launch_bounds__(kVerThreads, 4) verify_tile_kernel(VerifyParams p) {
+  constexpr int ES = XT == kBF16 ? 2 : 4, EPC = 16 / ES, SH = XT == kBF16 ? 16 : 0;  // SH: low key bits that say nothing
+  __shared__ float s_max[kVerThreads];
+  __shared__ uint32_t s_t;
+  __shared__ int s_n, s_cnt[2];
+  __shared__ int s_warp[kVerThreads / 32];
+  __shared__ uint2 s_list[kVerCap];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tile = blockIdx.x, n = blockIdx.y, b = blockIdx.z;
+  const float ninf = __int_as_float(0xff800000);
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = (int64_t)b * p.N + n;
+  if (p.parents[row] < -1) return;  // padding
+  const char* x = static_cast<const char*>(p.logits) + (b * p.l_sb + n * p.l_sn) * ES;
+  const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15) / ES;  // elements between a 16-byte boundary and the row
+  auto first = [&](int i) { return (tile * (kVerVecs * kVerThreads) + i * kVerThreads + tid) * EPC - off; };  // < 2^30 + a tile
+  uint4 r[kVerVecs];
+#pragma unroll
+  for (int i = 0; i < kVerVecs; ++i) {
+    const int k = first(i);
+    if (k >= 0 && k + EPC <= p.V) {
+      r[i] = ld_once_u4(x + (int64_t)k * ES);
+    } else {  // the row's ends, element by element; -inf outside
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) {
+        const bool in = k + e >= 0 && k + e < p.V;
+        if constexpr (XT == kBF16) {
+          const uint32_t h = in ? reinterpret_cast<const uint16_t*>(x)[k + e] : 0xff80u;
+          w[e >> 1] |= h << (16 * (e & 1));
+        } else {
+          w[e] = in ? reinterpret_cast<const uint32_t*>(x)[k + e] : 0xff800000u;
+        }
+      }
+      r[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  if (tid == 0) s_n = 0;
+  uint32_t mw = XT == kBF16 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+  for (int i = 0; i < kVerVecs; ++i) {
+    r[i].x = clean_word<XT>(r[i].x); r[i].y = clean_word<XT>(r[i].y);
+    r[i].z = clean_word<XT>(r[i].z); r[i].w = clean_word<XT>(r[i].w);
+    mw = max_word<XT>(mw, max_word<XT>(max_word<XT>(r[i].x, r[i].y), max_word<XT>(r[i].z, r[i].w)));
+  }
+  float mx = __uint_as_float(mw);
+  if constexpr (XT == kBF16) mx = fmaxf(__uint_as_float(mw << 16), __uint_as_float(mw & 0xffff0000u));
+  s_max[tid] = mx;
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t key[kVerThreads / 32];
+#pragma unroll
+    for (int i = 0; i < kVerThreads / 32; ++i) key[i] = logit_key(s_max[lane + 32 * i]);
+    uint32_t t = 0;
+    for (int bit = 31; bit >= SH; --bit) {
+      const uint32_t c = t | (1u << bit);
+      int cnt = 0;
+#pragma unroll
+      for (int i = 0; i < kVerThreads / 32; ++i) cnt += __popc(__ballot_sync(0xffffffffu, key[i] >= c));
+      if (cnt >= p.K) t = c;
+      if (cnt == p.K) break;
+    }
+    if (lane == 0) s_t = t;
+  }
+  __syncthreads();
+  const float tf = s_t <= 0x007fffffu ? ninf : key_logit(s_t);  // at or below -inf's word
+  if (mx >= tf) {
+#pragma unroll
+    for (int i = 0; i < kVerVecs; ++i) {
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) {
+        const float v = tile_value<XT>(r[i], e);
+        const int k = first(i) + e;
+        if (v >= tf && k >= 0 && k < p.V) {
+          const int at = atomicAdd(&s_n, 1);
+          if (at < kVerCap) s_list[at] = make_uint2(logit_key(v), (uint32_t)k);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  int found = s_n;
+  if (found > kVerCap) {
+    // exactly the K largest of the tile: their smallest word by halving, all
+    // above it, and its first ties in order of ids
+    uint32_t t = 0;
+    int flip = 0;
+    for (int bit = 31; bit >= SH; --bit) {
+      const uint32_t c = t | (1u << bit);
+      if (tid == 0) s_cnt[flip] = 0;
+      __syncthreads();
+      int cnt = 0;
+#pragma unroll
+      for (int i = 0; i < kVerVecs; ++i) {
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) {
+          const int k = first(i) + e;
+          cnt += logit_key(tile_value<XT>(r[i], e)) >= c && k >= 0 && k < p.V;
+        }
+      }
+      cnt = __reduce_add_sync(0xffffffffu, cnt);
+      if (lane == 0) atomicAdd(&s_cnt[flip], cnt);
+      __syncthreads();
+      if (s_cnt[flip] >= p.K) t = c;
+      flip ^= 1;
+    }
+    const uint32_t tk = t >> SH, tie_key = (XT == kBF16 && !(t >> 31)) ? t | 0xffffu : t;
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kVerVecs; ++i) {
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) {
+        const uint32_t key = logit_key(tile_value<XT>(r[i], e));
+        const int k = first(i) + e;
+        if ((key >> SH) > tk && k >= 0 && k < p.V) s_list[atomicAdd(&s_n, 1)] = make_uint2(key, (uint32_t)k);
+      }
+    }
+    __syncthreads();
+    int base = s_n;  // fewer than K
+    for (int i = 0; i < kVerVecs; ++i) {
+      // this thread's ties in vector row i; ids rise with (i, thread, element)
+      uint32_t tie = 0;
+#pragma unroll
+      for (int j = 0; j < kVerVecs; ++j) {
+        if (j != i) continue;
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) {
+          const int k = first(j) + e;
+          if ((logit_key(tile_value<XT>(r[j], e)) >> SH) == tk && k >= 0 && k < p.V) tie |= 1u << e;
+        }
+      }
+      const int mine = __popc(tie);
+      int pre = mine;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, pre, m);
+        if (lane >= m) pre += o;
+      }
+      if (lane == 31) s_warp[warp] = pre;
+      __syncthreads();
+      int at = base + pre - mine, all = 0;
+      for (int w = 0; w < kVerThreads / 32; ++w) {
+        if (w < warp) at += s_warp[w];
+        all += s_warp[w];
+      }
+      for (; tie; tie &= tie - 1, ++at)
+        if (at < p.K) s_list[at] = make_uint2(tie_key, (uint32_t)(first(i) + __ffs((int)tie) - 1));
+      base += all;
+      __syncthreads();
+    }
+    found = p.K;
+  }
+  const int64_t slot = row * p.tiles + tile;
+  if (tid < found) p.cand[slot * kVerCap + tid] = s_list[tid];
+  if (tid == 0) p.n_cand[slot] = found;
+}
+
+// -------------------------------------------------------------- row kernel --
+// One CTA per node: the K largest of the tiles' candidates in order, their
+// weights, and the draft's probabilities at them (so that the walk has nothing
+// left to fetch token by token).  The K-th largest word is found bit by bit
+// over the candidates in shared memory, what reaches it is put in order by
+// counting what stands before each.
+__device__ __forceinline__ bool cand_before(const uint2& a, const uint2& b) {  // larger logit, then lower id
+  return a.x > b.x || (a.x == b.x && a.y < b.y);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kVerThreads) verify_row_kernel(VerifyParams p) {
+  __shared__ uint2 s_c[kVerBatch];
+  __shared__ uint2 s_best[kVerThreads];
+  __shared__ uint2 s_sorted[kVerMaxK];
+  __shared__ uint32_t s_key[kVerMaxK];
+  __shared__ int s_id[kVerMaxK];
+  __shared__ int s_red[2][kVerThreads / 32];
+  __shared__ int s_off[33];
+  __shared__ int s_m;
+  constexpr int PER = (kVerBatch - kVerMaxK) / kVerCap;  // tiles per batch
+  static_assert(PER <= 32, "a warp scans a batch's counts");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = blockIdx.x, b = blockIdx.y;
   pdl_wait();
   pdl_trigger();
   const int64_t row = (int64_t)b * p.N + n;
-  if (p.parents[row] < -1) return;  // padding
-  const void* x = static_cast<const char*>(p.logits) + (b * p.l_sb + n * p.l_sn) * (XT == kBF16 ? 2 : 4);
-  const unsigned K = p.K;
-  if (tid == 0) { s_prefix = 0; s_need = K; s_count = 0; s_ties = 0; }
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  const int parent = p.parents[row];
+  if (parent < -1) return;
+  int flip = 0;
+  auto count = [&](auto pred, int m) {  // candidates of the batch for which pred holds
+    int c = 0;
+    for (int e = tid; e < m; e += kVerThreads) c += pred(s_c[e]);
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) s_red[flip][warp] = c;
     __syncthreads();
-    const uint32_t prefix = s_prefix;
-    for (int k = tid; k < p.V; k += kVerThreads) {
-      const uint32_t key = logit_key(load_f<XT>(x, k));
-      if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
+    c = 0;
+#pragma unroll
+    for (int w = 0; w < kVerThreads / 32; ++w) c += s_red[flip][w];
+    flip ^= 1;
+    return c;
+  };
+  int have = 0;  // candidates carried from the batches before
+  for (int t0 = 0; t0 < p.tiles; t0 += PER) {
+    const int nt = min(PER, p.tiles - t0);
+    if (warp == 0) {
+      int c = lane < nt ? __ldcg(&p.n_cand[row * p.tiles + t0 + lane]) : 0, pre = c;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, pre, m);
+        if (lane >= m) pre += o;
+      }
+      s_off[lane] = have + pre - c;
+      if (lane == 31) s_off[32] = have + pre;
     }
     __syncthreads();
-    if (tid == 0) {
-      unsigned need = s_need;
-      int d = 255;
-      while (d > 0 && hist[d] < need) need -= hist[d--];
-      s_need = need;
-      s_prefix = (prefix << 8) | (unsigned)d;
+    for (int t = warp; t < nt; t += kVerThreads / 32) {
+      const int at = s_off[t], c = s_off[t + 1] - at;
+      for (int e = lane; e < c; e += 32) s_c[at + e] = __ldcg(&p.cand[(row * p.tiles + t0 + t) * kVerCap + e]);
+    }
+    if (tid < have) s_c[tid] = s_sorted[tid];
+    __syncthreads();
+    const int total = s_off[32], want = min(p.K, total);
+    int m = total;
+    if (total > kVerThreads) {
+      uint32_t t = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = t | (1u << bit);
+        const int k = count([&](const uint2& v) { return v.x >= c; }, total);
+        if (k >= want) t = c;
+        if (k == want) break;
+      }
+      int k = count([&](const uint2& v) { return v.x >= t; }, total);
+      uint32_t last = 0xffffffffu;  // highest id taken among the words equal to t
+      if (k > kVerThreads) {
+        const int ties = want - count([&](const uint2& v) { return v.x > t; }, total);
+        last = 0;
+        for (int bit = 30; bit >= 0; --bit) {  // ids are below 2^30; last + 1 such that `ties` are below it
+          const uint32_t c = last | (1u << bit);
+          if (count([&](const uint2& v) { return v.x == t && v.y < c; }, total) < ties) last = c;
+        }
+      }
+      if (tid == 0) s_m = 0;
+      __syncthreads();
+      for (int e = tid; e < total; e += kVerThreads) {
+        const uint2 v = s_c[e];
+        if (v.x > t || (v.x == t && v.y <= last)) s_best[atomicAdd(&s_m, 1)] = v;
+      }
+      __syncthreads();
+      m = s_m;
+    } else {
+      if (tid < total) s_best[tid] = s_c[tid];
+      __syncthreads();
+    }
+    if (tid < m) {
+      const uint2 v = s_best[tid];
+      int r = 0;
+      for (int j = 0; j < m; ++j) r += cand_before(s_best[j], v);
+      if (r < want) s_sorted[r] = v;
     }
     __syncthreads();
+    have = want;
   }
-  const uint32_t kth = s_prefix;
-  const unsigned above = K - s_need;  // words above the K-th; the rest are its first ties
-  for (int k0 = 0; k0 < p.V; k0 += kVerThreads) {
-    const int k = k0 + tid;
-    const uint32_t key = k < p.V ? logit_key(load_f<XT>(x, k)) : 0u;
-    if (k < p.V && key > kth) {
-      const unsigned at = atomicAdd(&s_count, 1u);
-      ck[at] = key;
-      ci[at] = k;
-    }
-    const unsigned vote = __ballot_sync(0xffffffffu, k < p.V && key == kth);
-    if (lane == 0) wcount[warp] = __popc(vote);
-    __syncthreads();
-    unsigned at = s_ties;
-    for (int w = 0; w < warp; ++w) at += wcount[w];
-    at += __popc(vote & ((1u << lane) - 1u));
-    if (((vote >> lane) & 1u) && above + at < K) {
-      ck[above + at] = key;
-      ci[above + at] = k;
-    }
-    __syncthreads();
-    if (tid == 0)
-      for (int w = 0; w < kVerThreads / 32; ++w) s_ties += wcount[w];
+  if (tid < kVerMaxK) {
+    const uint2 v = tid < have ? s_sorted[tid] : make_uint2(0u, 0u);
+    s_key[tid] = v.x;
+    s_id[tid] = (int)v.y;
+    if (p.draft != nullptr)
+      p.q[row * kVerMaxK + tid] =
+          tid < have ? load_f<DT>(static_cast<const char*>(p.draft) + (b * p.d_sb + n * p.d_sn) * (DT == kBF16 ? 2 : 4),
+                                  (int)v.y)
+                     : 0.0f;
+  }
+  if (tid == kVerMaxK && p.draft != nullptr) {
+    const int64_t x = p.tokens[row];
+    p.raw[row] = parent >= 0 && parent < n && x >= 0 && x < p.V
+                     ? load_f<DT>(static_cast<const char*>(p.draft) +
+                                  (b * p.d_sb + parent * p.d_sn) * (DT == kBF16 ? 2 : 4), x)
+                     : 0.0f;
   }
   __syncthreads();
-  if (tid < (int)K) {  // in order: larger logit first, then the lower id
-    int r = 0;
-    for (int j = 0; j < (int)K; ++j) r += ck[j] > ck[tid] || (ck[j] == ck[tid] && ci[j] < ci[tid]);
-    sk[r] = ck[tid];
-    si[r] = ci[tid];
-  }
-  __syncthreads();
-  if (warp == 0) node_weights(p, sk, si, row, lane);
+  if (warp == 0) node_weights(p, s_key, s_id, row, lane);
 }
 
-// The walk: one warp per sequence, nodes and candidates two per lane.
-template <int DT>
-__global__ void __launch_bounds__(32) verify_walk_kernel(VerifyParams p) {
-  const int lane = threadIdx.x, b = blockIdx.x;
+// ------------------------------------------------------------------- walk --
+// One CTA per sequence: all of its nodes' distributions into shared memory at
+// once, then one warp walks, nodes and candidates two per lane.
+__global__ void __launch_bounds__(kVerThreads) verify_walk_kernel(VerifyParams p) {
+  extern __shared__ __align__(16) unsigned char dyn[];
+  double* s_w = reinterpret_cast<double*>(dyn);                 // [N][64]
+  int* s_id = reinterpret_cast<int*>(s_w + p.N * kVerMaxK);     // [N][64]
+  float* s_q = reinterpret_cast<float*>(s_id + p.N * kVerMaxK); // [N][64]
+  const int tid = threadIdx.x, lane = tid & 31, b = blockIdx.x;
   pdl_wait();
   pdl_trigger();
   const int64_t base = (int64_t)b * p.N;
+  for (int e = tid; e < p.N * kVerMaxK; e += kVerThreads) {
+    s_w[e] = __ldcg(p.w + base * kVerMaxK + e);  // a padding node's is never looked at
+    s_id[e] = __ldcg(p.id + base * kVerMaxK + e);
+    s_q[e] = p.draft != nullptr ? __ldcg(p.q + base * kVerMaxK + e) : 0.0f;
+  }
   int par[2];
   int64_t tok[2];
-  float un[2];
+  float un[2], rw[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int i = lane + 32 * u;
     par[u] = i < p.N ? p.parents[base + i] : -2;
     tok[u] = i < p.N ? p.tokens[base + i] : -1;
     un[u] = i < p.N ? p.uniform[base + i] : 0.0f;
+    rw[u] = i < p.N && p.draft != nullptr ? __ldcg(p.raw + base + i) : 0.0f;
+  }
+  __syncthreads();
+  if (tid >= 32) return;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = lane + 32 * u;
     if (i < p.N) {
       p.path[base + i] = -1;
       p.out[base + i] = -1;
@@ -208,13 +488,10 @@ __global__ void __launch_bounds__(32) verify_walk_kernel(VerifyParams p) {
     auto enter = [&]() {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int j = lane + 32 * u;
-        pr[u] = __ldcg(p.w + (base + cur) * kVerMaxK + j);
-        id[u] = __ldcg(p.id + (base + cur) * kVerMaxK + j);
-        q[u] = 0.0;
-        if (p.draft != nullptr && id[u] >= 0)
-          q[u] = (double)load_f<DT>(static_cast<const char*>(p.draft) +
-                                    (b * p.d_sb + cur * p.d_sn) * (DT == kBF16 ? 2 : 4), id[u]);
+        const int j = cur * kVerMaxK + lane + 32 * u;
+        pr[u] = s_w[j];
+        id[u] = s_id[j];
+        q[u] = (double)s_q[j];
       }
       left = 1.0;
       if (lane == 0) p.path[base + kept] = cur;
@@ -243,9 +520,8 @@ __global__ void __launch_bounds__(32) verify_walk_kernel(VerifyParams p) {
         const unsigned long long twin =
             (((unsigned long long)__ballot_sync(0xffffffffu, tok[1] == x) << 32) |
              __ballot_sync(0xffffffffu, tok[0] == x)) & kids & ((1ull << c) - 1ull);
-        if (in && (p.replacement || twin == 0))
-          raw = (double)load_f<DT>(static_cast<const char*>(p.draft) +
-                                   (b * p.d_sb + cur * p.d_sn) * (DT == kBF16 ? 2 : 4), x);
+        raw = (double)__shfl_sync(0xffffffffu, c < 32 ? rw[0] : rw[1], c & 31);
+        if (!p.replacement && twin != 0) raw = 0.0;
         qx = fmin(raw / left, 1.0);
       }
       if (uc * qx < px) {
@@ -287,13 +563,20 @@ __global__ void __launch_bounds__(32) verify_walk_kernel(VerifyParams p) {
   if (lane == 0) p.n_path[b] = kept;
 }
 
+// Tiles of a row of `vocab` logits, `per` of them in 16 bytes, wherever the row starts.
+inline int64_t verify_tiles(int64_t vocab, int64_t per) {
+  const int64_t tile = (int64_t)kVerThreads * kVerVecs * per;
+  return (vocab + per - 1 + tile - 1) / tile;
+}
+
 }  // namespace mb
 
 using namespace mb;
 
 extern "C" int64_t maple_verify_tree_workspace_bytes(int64_t batch, int64_t nodes, int64_t vocab, int64_t top_k) {
-  if (batch < 0 || nodes <= 0 || nodes > kVerMaxNodes || vocab <= 0 || top_k <= 0) return -1;
-  return batch * nodes * kVerMaxK * 12;
+  if (batch < 0 || nodes <= 0 || nodes > kVerMaxNodes || vocab <= 0 || vocab > (1LL << 30) || top_k <= 0) return -1;
+  const int64_t tiles = verify_tiles(vocab, 4);  // fp32 rows have the more tiles
+  return batch * nodes * (tiles * (kVerCap * 8 + 4) + kVerMaxK * 16 + 8) + 64;
 }
 
 extern "C" int maple_verify_tree(const void* logits, int x_dtype, int64_t batch, int64_t nodes, int64_t vocab,
@@ -312,19 +595,30 @@ extern "C" int maple_verify_tree(const void* logits, int x_dtype, int64_t batch,
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return kErrAlign;
   VerifyParams p{};
   p.logits = logits; p.tokens = tokens; p.parents = parents; p.uniform = uniform; p.draft = draft_probs;
+  const int64_t rows = batch * nodes;
+  p.tiles = (int)verify_tiles(vocab, x_dtype == kBF16 ? 8 : 4);
   p.w = static_cast<double*>(workspace);
-  p.id = reinterpret_cast<int32_t*>(p.w + batch * nodes * kVerMaxK);
+  p.cand = reinterpret_cast<uint2*>(p.w + rows * kVerMaxK);
+  p.id = reinterpret_cast<int32_t*>(p.cand + rows * p.tiles * kVerCap);
+  p.q = reinterpret_cast<float*>(p.id + rows * kVerMaxK);
+  p.raw = p.q + rows * kVerMaxK;
+  p.n_cand = reinterpret_cast<int32_t*>(p.raw + rows);
   p.path = path; p.n_path = n_path; p.out = out; p.err = err;
   p.l_sb = l_sb; p.l_sn = l_sn; p.d_sb = d_sb; p.d_sn = d_sn;
   p.inv_t = 1.0 / (double)temperature; p.top_p = (double)top_p;
   p.B = (int)batch; p.N = (int)nodes; p.V = (int)vocab; p.K = (int)(top_k < vocab ? top_k : vocab);
   p.replacement = replacement != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)nodes, (unsigned)batch);
-  cudaError_t e = x_dtype == kBF16 ? launch_k(verify_topk_kernel<kBF16>, grid, dim3(kVerThreads), 0, st, p)
-                                   : launch_k(verify_topk_kernel<kF32>, grid, dim3(kVerThreads), 0, st, p);
+  const dim3 grid((unsigned)p.tiles, (unsigned)nodes, (unsigned)batch), rgrid((unsigned)nodes, (unsigned)batch);
+  cudaError_t e = x_dtype == kBF16 ? launch_k(verify_tile_kernel<kBF16>, grid, dim3(kVerThreads), 0, st, p)
+                                   : launch_k(verify_tile_kernel<kF32>, grid, dim3(kVerThreads), 0, st, p);
   if (e == cudaSuccess)
-    e = (draft_probs && d_dtype == kBF16) ? launch_k(verify_walk_kernel<kBF16>, dim3((unsigned)batch), dim3(32), 0, st, p)
-                                          : launch_k(verify_walk_kernel<kF32>, dim3((unsigned)batch), dim3(32), 0, st, p);
+    e = (draft_probs && d_dtype == kBF16) ? launch_k(verify_row_kernel<kBF16>, rgrid, dim3(kVerThreads), 0, st, p)
+                                          : launch_k(verify_row_kernel<kF32>, rgrid, dim3(kVerThreads), 0, st, p);
+  if (e == cudaSuccess) {
+    const int smem = (int)nodes * kVerMaxK * 16;
+    e = cudaFuncSetAttribute(verify_walk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = launch_k(verify_walk_kernel, dim3((unsigned)batch), dim3(kVerThreads), smem, st, p);
+  }
   return e == cudaSuccess ? kOk : kErrCuda;
 }

@@ -1039,7 +1039,7 @@ def tree_gqa_attn(q, k_cache, v_cache, seqlen, tree_mask, *, row_map=None, scale
     if B == 0:
         return out
     L = lib()
-    nbytes = L.maple_tree_gqa_workspace_bytes(B, N, H, n_kv, D, T, code)
+    nbytes = L.maple_tree_gqa_workspace_bytes(B, N, H, n_kv, D, T, int(window or 0), code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
     _launch(L.maple_tree_gqa_attn, op, dev, ptr(q), code, B, N, H, qs[0], qs[1], qs[2], ptr(k_cache), ptr(v_cache),
             Bc, n_kv, ks[0], ks[1], T, D, ptr(sl), ptr(tm), ptr(rm), float(scale), int(window or 0), ptr(out), ptr(ws),
