@@ -80,17 +80,18 @@ __device__ __forceinline__ void warp_prefix_d(const double (&a)[2], double (&c)[
   c[1] += __shfl_sync(0xffffffffu, c[0], 31);
 }
 
-// A node's distribution from its K largest logits (sorted in v / id).
-__device__ __forceinline__ void node_weights(const VerifyParams& p, const uint32_t* key, const int* ids, int64_t row,
-                                             int lane) {
-  const float v0 = key_logit(key[0]);
+// A node's distribution from its `have` <= K largest logits above -inf, in order
+// (none: all alike).
+__device__ __forceinline__ void node_weights(const VerifyParams& p, const uint32_t* key, const int* ids, int have,
+                                             int64_t row, int lane) {
+  const float v0 = have > 0 ? key_logit(key[0]) : 0.0f;
   double w[2], c[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int j = lane + 32 * u;
     w[u] = 0.0;
-    if (j < p.K) {
-      const float v = key_logit(key[j]);
+    if (j < have || (have == 0 && j < p.K)) {
+      const float v = have > 0 ? key_logit(key[j]) : 0.0f;
       w[u] = v == v0 ? 1.0 : exp(((double)v - (double)v0) * p.inv_t);
     }
   }
@@ -106,43 +107,28 @@ __device__ __forceinline__ void node_weights(const VerifyParams& p, const uint32
   for (int u = 0; u < 2; ++u) {
     const int j = lane + 32 * u;
     p.w[row * kVerMaxK + j] = w[u] / t;
-    p.id[row * kVerMaxK + j] = j < p.K ? ids[j] : -1;
+    p.id[row * kVerMaxK + j] = j < have || (have == 0 && j < p.K) ? ids[j] : -1;
   }
 }
 
 // ------------------------------------------------------------- tile kernel --
-// The logits are read once.  A CTA holds a tile of a row in registers (eight
-// 16-byte vectors per thread, all in flight together) and hands on what may be
-// among the row's K largest: T = the K-th largest of the 256 threads' maxima is
-// at most the tile's K-th largest logit, and few logits reach it (about K of
-// 16384: threads seldom hold two), so one comparison per thread and a scan in
-// those that pass find them.  T is found bit by bit, one warp counting the
-// maxima with votes.  Where more than kVerCap reach T (ties, large logits side
-// by side) the tile's K largest are selected exactly, ties to the lowest ids.
+// The logits are read once.  A CTA takes a tile of a row, eight 16-byte vectors
+// per thread in flight together, and keeps each vector's maximum.  T, just
+// below the K-th largest of the 256 threads' maxima, is at most the tile's
+// K-th largest logit, and few logits reach it (about K of 16384: threads seldom
+// hold two); the vectors that do are looked at again, one element per thread.
+// T is found bit by bit, one warp counting the maxima with votes, from the
+// first bit in which they differ until close to K of them reach it: a T a
+// little too low only lets a few more through.  Where more than kVerCap come
+// through (ties, large logits side by side) the tile's K largest are selected
+// exactly, ties to the lowest ids.  -inf and NaN are not handed on: they have no weight, and a row
+// of nothing else is known by having no candidates.
 __device__ __forceinline__ uint4 ld_once_u4(const void* p) {  // written by the launch before: not the read-only path
   uint4 r;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   return r;
 }
-
-template <int XT>
-__device__ __forceinline__ float tile_value(const uint4& r, int e) {
-  if constexpr (XT == kBF16) {
-    const uint32_t w = e < 4 ? (e < 2 ? r.x : r.y) : (e < 6 ? r.z : r.w);
-    return __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
-  } else {
-    return __uint_as_float(e < 2 ? (e == 0 ? r.x : r.y) : (e == 2 ? r.z : r.w));
-  }
-}
-template <int XT>
-__device__ __forceinline__ uint32_t clean_word(uint32_t w) {  // NaN to -inf: the other operand of a maximum
-  if constexpr (XT == kBF16) {
-    asm("max.bf16x2 %0, %0, %1;\n" : "+r"(w) : "r"(0xff80ff80u));
-    return w;
-  } else {
-    return __float_as_uint(fmaxf(__uint_as_float(w), __int_as_float(0xff800000)));
-  }
-}
+// Larger of two words of logits (two bf16, or one fp32), NaN giving way.
 template <int XT>
 __device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
   if constexpr (XT == kBF16) {
@@ -153,14 +139,26 @@ __device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
     return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
   }
 }
+template <int XT>
+__device__ __forceinline__ float word_max(uint32_t w) {
+  if constexpr (XT == kBF16) return fmaxf(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __uint_as_float(w);
+}
 
 template <int XT>
-__global__ void __launch_bounds__(kVerThreads, 4) verify_tile_kernel(VerifyParams p) {
+struct VerWord { using type = uint32_t; };
+template <>
+struct VerWord<kBF16> { using type = uint16_t; };
+
+template <int XT>
+__global__ void __launch_bounds__(kVerThreads, 5) verify_tile_kernel(VerifyParams p) {
   constexpr int ES = XT == kBF16 ? 2 : 4, EPC = 16 / ES, SH = XT == kBF16 ? 16 : 0;  // SH: low key bits that say nothing
   __shared__ float s_max[kVerThreads];
   __shared__ uint32_t s_t;
-  __shared__ int s_n, s_cnt[2];
+  __shared__ int s_n, s_vecs, s_cnt[2];
   __shared__ int s_warp[kVerThreads / 32];
+  __shared__ uint4 s_tile[kVerThreads * kVerVecs];  // vectors of interest (their numbers), or the tile's words
+  int* s_vec = reinterpret_cast<int*>(s_tile);
   __shared__ uint2 s_list[kVerCap];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tile = blockIdx.x, n = blockIdx.y, b = blockIdx.z;
@@ -171,11 +169,11 @@ __global__ void __launch_bounds__(kVerThreads, 4) verify_tile_kernel(VerifyParam
   if (p.parents[row] < -1) return;  // padding
   const char* x = static_cast<const char*>(p.logits) + (b * p.l_sb + n * p.l_sn) * ES;
   const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15) / ES;  // elements between a 16-byte boundary and the row
-  auto first = [&](int i) { return (tile * (kVerVecs * kVerThreads) + i * kVerThreads + tid) * EPC - off; };  // < 2^30 + a tile
+  const int k0 = tile * (kVerVecs * kVerThreads) * EPC - off;       // the tile's first element; < 2^30 + a tile
   uint4 r[kVerVecs];
 #pragma unroll
   for (int i = 0; i < kVerVecs; ++i) {
-    const int k = first(i);
+    const int k = k0 + (i * kVerThreads + tid) * EPC;
     if (k >= 0 && k + EPC <= p.V) {
       r[i] = ld_once_u4(x + (int64_t)k * ES);
     } else {  // the row's ends, element by element; -inf outside
@@ -193,117 +191,118 @@ __global__ void __launch_bounds__(kVerThreads, 4) verify_tile_kernel(VerifyParam
       r[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-  if (tid == 0) s_n = 0;
-  uint32_t mw = XT == kBF16 ? 0xff80ff80u : 0xff800000u;
+  if (tid == 0) s_n = s_vecs = 0;
+  float vm[kVerVecs], mx = ninf;
 #pragma unroll
   for (int i = 0; i < kVerVecs; ++i) {
-    r[i].x = clean_word<XT>(r[i].x); r[i].y = clean_word<XT>(r[i].y);
-    r[i].z = clean_word<XT>(r[i].z); r[i].w = clean_word<XT>(r[i].w);
-    mw = max_word<XT>(mw, max_word<XT>(max_word<XT>(r[i].x, r[i].y), max_word<XT>(r[i].z, r[i].w)));
+    const uint32_t w = max_word<XT>(max_word<XT>(r[i].x, r[i].y), max_word<XT>(r[i].z, r[i].w));
+    vm[i] = word_max<XT>(w);
+    mx = fmaxf(mx, vm[i]);
   }
-  float mx = __uint_as_float(mw);
-  if constexpr (XT == kBF16) mx = fmaxf(__uint_as_float(mw << 16), __uint_as_float(mw & 0xffff0000u));
   s_max[tid] = mx;
   __syncthreads();
   if (warp == 0) {
-    uint32_t key[kVerThreads / 32];
+    uint32_t key[kVerThreads / 32], hi = 0, lo = 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < kVerThreads / 32; ++i) key[i] = logit_key(s_max[lane + 32 * i]);
-    uint32_t t = 0;
-    for (int bit = 31; bit >= SH; --bit) {
+    for (int i = 0; i < kVerThreads / 32; ++i) {
+      key[i] = logit_key(s_max[lane + 32 * i]);
+      hi = max(hi, key[i]);
+      lo = min(lo, key[i]);
+    }
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    const int top = 31 - __clz((int)(hi ^ lo));  // first bit in which they differ; -1: they are all equal
+    uint32_t t = top < 0 ? lo : lo & ~((2u << top) - 1u);
+    int reach = kVerThreads;
+    for (int bit = top; bit >= SH && reach > p.K + (p.K >> 3); --bit) {
       const uint32_t c = t | (1u << bit);
       int cnt = 0;
 #pragma unroll
       for (int i = 0; i < kVerThreads / 32; ++i) cnt += __popc(__ballot_sync(0xffffffffu, key[i] >= c));
-      if (cnt >= p.K) t = c;
-      if (cnt == p.K) break;
+      if (cnt >= p.K) {
+        t = c;
+        reach = cnt;
+      }
     }
     if (lane == 0) s_t = t;
   }
   __syncthreads();
-  const float tf = s_t <= 0x007fffffu ? ninf : key_logit(s_t);  // at or below -inf's word
+  // just above -inf where T is not above it (fewer than K finite maxima)
+  const uint32_t t = max(s_t, 0x00800000u);
+  const float tf = key_logit(t);
   if (mx >= tf) {
 #pragma unroll
-    for (int i = 0; i < kVerVecs; ++i) {
-#pragma unroll
-      for (int e = 0; e < EPC; ++e) {
-        const float v = tile_value<XT>(r[i], e);
-        const int k = first(i) + e;
-        if (v >= tf && k >= 0 && k < p.V) {
-          const int at = atomicAdd(&s_n, 1);
-          if (at < kVerCap) s_list[at] = make_uint2(logit_key(v), (uint32_t)k);
-        }
-      }
+    for (int i = 0; i < kVerVecs; ++i)
+      if (vm[i] >= tf) s_vec[atomicAdd(&s_vecs, 1)] = i * kVerThreads + tid;
+  }
+  __syncthreads();
+  for (int j = tid; j < s_vecs * EPC; j += kVerThreads) {
+    const int k = k0 + s_vec[j / EPC] * EPC + j % EPC;
+    if (k < 0 || k >= p.V) continue;
+    const float v = load_f<XT>(x, k);
+    if (v >= tf) {
+      const int at = atomicAdd(&s_n, 1);
+      if (at < kVerCap) s_list[at] = make_uint2(logit_key(v), (uint32_t)k);
     }
   }
   __syncthreads();
   int found = s_n;
   if (found > kVerCap) {
-    // exactly the K largest of the tile: their smallest word by halving, all
-    // above it, and its first ties in order of ids
-    uint32_t t = 0;
+    // exactly the K largest of the tile, from its words in shared memory: their
+    // smallest by halving, all above it, and its first ties in order of ids
+    using Word = typename VerWord<XT>::type;
+    Word* words = reinterpret_cast<Word*>(s_tile);
+    constexpr int TILE = kVerThreads * kVerVecs * EPC;
+#pragma unroll 8
+    for (int j = tid; j < TILE; j += kVerThreads) {
+      const int k = k0 + j;
+      const uint32_t key = k >= 0 && k < p.V ? logit_key(load_f<XT>(x, k)) : 0u;
+      words[j] = (Word)(key >= t ? key >> SH : 0u);  // 0: not of interest
+    }
+    uint32_t kth = 0;
     int flip = 0;
-    for (int bit = 31; bit >= SH; --bit) {
-      const uint32_t c = t | (1u << bit);
+#pragma unroll 1
+    for (int bit = 31 - SH; bit >= 0; --bit) {
+      const uint32_t c = kth | (1u << bit);
       if (tid == 0) s_cnt[flip] = 0;
       __syncthreads();
       int cnt = 0;
-#pragma unroll
+#pragma unroll 2
       for (int i = 0; i < kVerVecs; ++i) {
+        const uint4 v = s_tile[i * kVerThreads + tid];
+        const uint32_t q[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < EPC; ++e) {
-          const int k = first(i) + e;
-          cnt += logit_key(tile_value<XT>(r[i], e)) >= c && k >= 0 && k < p.V;
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (XT == kBF16) cnt += ((q[e] & 0xffffu) >= c) + ((q[e] >> 16) >= c);
+          else cnt += q[e] >= c;
         }
       }
       cnt = __reduce_add_sync(0xffffffffu, cnt);
       if (lane == 0) atomicAdd(&s_cnt[flip], cnt);
       __syncthreads();
-      if (s_cnt[flip] >= p.K) t = c;
+      if (s_cnt[flip] >= p.K) kth = c;
       flip ^= 1;
     }
-    const uint32_t tk = t >> SH, tie_key = (XT == kBF16 && !(t >> 31)) ? t | 0xffffu : t;
     if (tid == 0) s_n = 0;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kVerVecs; ++i) {
-#pragma unroll
-      for (int e = 0; e < EPC; ++e) {
-        const uint32_t key = logit_key(tile_value<XT>(r[i], e));
-        const int k = first(i) + e;
-        if ((key >> SH) > tk && k >= 0 && k < p.V) s_list[atomicAdd(&s_n, 1)] = make_uint2(key, (uint32_t)k);
-      }
-    }
+    auto key_of = [](uint32_t w) {  // the whole word again
+      return XT == kBF16 ? (w & 0x8000u ? w << 16 : w << 16 | 0xffffu) : w;
+    };
+    for (int j = tid; j < TILE; j += kVerThreads)
+      if (words[j] > kth) s_list[atomicAdd(&s_n, 1)] = make_uint2(key_of(words[j]), (uint32_t)(k0 + j));
     __syncthreads();
     int base = s_n;  // fewer than K
-    for (int i = 0; i < kVerVecs; ++i) {
-      // this thread's ties in vector row i; ids rise with (i, thread, element)
-      uint32_t tie = 0;
-#pragma unroll
-      for (int j = 0; j < kVerVecs; ++j) {
-        if (j != i) continue;
-#pragma unroll
-        for (int e = 0; e < EPC; ++e) {
-          const int k = first(j) + e;
-          if ((logit_key(tile_value<XT>(r[j], e)) >> SH) == tk && k >= 0 && k < p.V) tie |= 1u << e;
-        }
-      }
-      const int mine = __popc(tie);
-      int pre = mine;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, pre, m);
-        if (lane >= m) pre += o;
-      }
-      if (lane == 31) s_warp[warp] = pre;
+#pragma unroll 1
+    for (int j0 = 0; j0 < TILE && base < p.K; j0 += kVerThreads) {
+      const unsigned vote = __ballot_sync(0xffffffffu, words[j0 + tid] == kth);
+      if (lane == 0) s_warp[warp] = __popc(vote);
       __syncthreads();
-      int at = base + pre - mine, all = 0;
+      int at = base + __popc(vote & ((1u << lane) - 1u)), all = 0;
       for (int w = 0; w < kVerThreads / 32; ++w) {
         if (w < warp) at += s_warp[w];
         all += s_warp[w];
       }
-      for (; tie; tie &= tie - 1, ++at)
-        if (at < p.K) s_list[at] = make_uint2(tie_key, (uint32_t)(first(i) + __ffs((int)tie) - 1));
+      if (((vote >> lane) & 1u) && at < p.K) s_list[at] = make_uint2(key_of(kth), (uint32_t)(k0 + j0 + tid));
       base += all;
       __syncthreads();
     }
@@ -379,14 +378,36 @@ __global__ void __launch_bounds__(kVerThreads) verify_row_kernel(VerifyParams p)
     const int total = s_off[32], want = min(p.K, total);
     int m = total;
     if (total > kVerThreads) {
-      uint32_t t = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = t | (1u << bit);
-        const int k = count([&](const uint2& v) { return v.x >= c; }, total);
-        if (k >= want) t = c;
-        if (k == want) break;
+      // cut down to between `want` and 256: T from the first bit in which the words differ
+      uint32_t hi = 0, lo = 0xffffffffu;
+      for (int e = tid; e < total; e += kVerThreads) {
+        hi = max(hi, s_c[e].x);
+        lo = min(lo, s_c[e].x);
       }
-      int k = count([&](const uint2& v) { return v.x >= t; }, total);
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      if (lane == 0) {
+        s_red[0][warp] = (int)hi;
+        s_red[1][warp] = (int)lo;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kVerThreads / 32; ++w) {
+        hi = max(hi, (uint32_t)s_red[0][w]);
+        lo = min(lo, (uint32_t)s_red[1][w]);
+      }
+      __syncthreads();
+      const int top = 31 - __clz((int)(hi ^ lo));
+      uint32_t t = top < 0 ? lo : lo & ~((2u << top) - 1u);
+      int k = total;
+      for (int bit = top; bit >= 0 && k > kVerThreads; --bit) {
+        const uint32_t c = t | (1u << bit);
+        const int kc = count([&](const uint2& v) { return v.x >= c; }, total);
+        if (kc >= want) {
+          t = c;
+          k = kc;
+        }
+      }
       uint32_t last = 0xffffffffu;  // highest id taken among the words equal to t
       if (k > kVerThreads) {
         const int ties = want - count([&](const uint2& v) { return v.x > t; }, total);
@@ -420,12 +441,13 @@ __global__ void __launch_bounds__(kVerThreads) verify_row_kernel(VerifyParams p)
   if (tid < kVerMaxK) {
     const uint2 v = tid < have ? s_sorted[tid] : make_uint2(0u, 0u);
     s_key[tid] = v.x;
-    s_id[tid] = (int)v.y;
-    if (p.draft != nullptr)
+    s_id[tid] = have > 0 ? (int)v.y : tid;  // nothing above -inf: the lowest ids share alike
+    if (p.draft != nullptr) {
+      const bool used = tid < have || (have == 0 && tid < p.K);
       p.q[row * kVerMaxK + tid] =
-          tid < have ? load_f<DT>(static_cast<const char*>(p.draft) + (b * p.d_sb + n * p.d_sn) * (DT == kBF16 ? 2 : 4),
-                                  (int)v.y)
-                     : 0.0f;
+          used ? load_f<DT>(static_cast<const char*>(p.draft) + (b * p.d_sb + n * p.d_sn) * (DT == kBF16 ? 2 : 4), s_id[tid])
+               : 0.0f;
+    }
   }
   if (tid == kVerMaxK && p.draft != nullptr) {
     const int64_t x = p.tokens[row];
@@ -435,7 +457,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_row_kernel(VerifyParams p)
                      : 0.0f;
   }
   __syncthreads();
-  if (warp == 0) node_weights(p, s_key, s_id, row, lane);
+  if (warp == 0) node_weights(p, s_key, s_id, have, row, lane);
 }
 
 // ------------------------------------------------------------------- walk --
