@@ -319,14 +319,17 @@ __global__ void __launch_bounds__(kVerThreads, 5) verify_tile_kernel(VerifyParam
 // left to fetch token by token).  The K-th largest word is found bit by bit
 // over the candidates in shared memory, what reaches it is put in order by
 // counting what stands before each.
-__device__ __forceinline__ bool cand_before(const uint2& a, const uint2& b) {  // larger logit, then lower id
-  return a.x > b.x || (a.x == b.x && a.y < b.y);
+constexpr int kVerRank = 128;  // candidates that are put in order by counting
+
+// One word whose order is larger logit, then lower id.
+__device__ __forceinline__ unsigned long long cand_word(const uint2& v) {
+  return (unsigned long long)v.x << 32 | (0xffffffffu - v.y);
 }
 
 template <int DT>
 __global__ void __launch_bounds__(kVerThreads) verify_row_kernel(VerifyParams p) {
   __shared__ uint2 s_c[kVerBatch];
-  __shared__ uint2 s_best[kVerThreads];
+  __shared__ unsigned long long s_best[kVerRank];
   __shared__ uint2 s_sorted[kVerMaxK];
   __shared__ uint32_t s_key[kVerMaxK];
   __shared__ int s_id[kVerMaxK];
@@ -377,8 +380,8 @@ __global__ void __launch_bounds__(kVerThreads) verify_row_kernel(VerifyParams p)
     __syncthreads();
     const int total = s_off[32], want = min(p.K, total);
     int m = total;
-    if (total > kVerThreads) {
-      // cut down to between `want` and 256: T from the first bit in which the words differ
+    if (total > kVerRank) {
+      // cut down to between `want` and kVerRank: T from the first bit in which the words differ
       uint32_t hi = 0, lo = 0xffffffffu;
       for (int e = tid; e < total; e += kVerThreads) {
         hi = max(hi, s_c[e].x);
@@ -400,7 +403,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_row_kernel(VerifyParams p)
       const int top = 31 - __clz((int)(hi ^ lo));
       uint32_t t = top < 0 ? lo : lo & ~((2u << top) - 1u);
       int k = total;
-      for (int bit = top; bit >= 0 && k > kVerThreads; --bit) {
+      for (int bit = top; bit >= 0 && k > kVerRank; --bit) {
         const uint32_t c = t | (1u << bit);
         const int kc = count([&](const uint2& v) { return v.x >= c; }, total);
         if (kc >= want) {
@@ -409,7 +412,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_row_kernel(VerifyParams p)
         }
       }
       uint32_t last = 0xffffffffu;  // highest id taken among the words equal to t
-      if (k > kVerThreads) {
+      if (k > kVerRank) {
         const int ties = want - count([&](const uint2& v) { return v.x > t; }, total);
         last = 0;
         for (int bit = 30; bit >= 0; --bit) {  // ids are below 2^30; last + 1 such that `ties` are below it
@@ -421,19 +424,20 @@ __global__ void __launch_bounds__(kVerThreads) verify_row_kernel(VerifyParams p)
       __syncthreads();
       for (int e = tid; e < total; e += kVerThreads) {
         const uint2 v = s_c[e];
-        if (v.x > t || (v.x == t && v.y <= last)) s_best[atomicAdd(&s_m, 1)] = v;
+        if (v.x > t || (v.x == t && v.y <= last)) s_best[atomicAdd(&s_m, 1)] = cand_word(v);
       }
       __syncthreads();
       m = s_m;
     } else {
-      if (tid < total) s_best[tid] = s_c[tid];
+      if (tid < total) s_best[tid] = cand_word(s_c[tid]);
       __syncthreads();
     }
     if (tid < m) {
-      const uint2 v = s_best[tid];
+      const unsigned long long v = s_best[tid];
       int r = 0;
-      for (int j = 0; j < m; ++j) r += cand_before(s_best[j], v);
-      if (r < want) s_sorted[r] = v;
+#pragma unroll 8
+      for (int j = 0; j < m; ++j) r += s_best[j] > v;
+      if (r < want) s_sorted[r] = make_uint2((uint32_t)(v >> 32), 0xffffffffu - (uint32_t)v);
     }
     __syncthreads();
     have = want;
