@@ -16,18 +16,21 @@
 //
 // Comparisons with a uniform decide which token comes out, so everything after
 // the selection (at most 64 values per node) is held in 64 bits.
+#include <cooperative_groups.h>
+
 #include "bulk.cuh"
 #include "common.cuh"
 #include "launch.cuh"
 
 namespace mb {
 
+namespace cg = cooperative_groups;
+
 constexpr int kVerMaxK = 64;
 constexpr int kVerMaxNodes = 64;
 constexpr int kVerThreads = 256;
 constexpr int kVerVecs = 8;      // 16-byte vectors per thread and tile
 constexpr int kVerCap = 128;     // candidates that a tile may hand on
-constexpr int kVerBatch = 4096;  // candidates that a row's selection holds at a time
 
 struct VerifyParams {
   const void* logits;     // [B, N, V], V contiguous
@@ -37,10 +40,6 @@ struct VerifyParams {
   const void* draft;      // [B, N, V] or null, V contiguous
   uint2* cand;            // [B * N, tiles, kVerCap] candidates: key, id
   int32_t* n_cand;        // [B * N, tiles]
-  double* w;              // [B * N, 64] kept weights, falling
-  int32_t* id;            // [B * N, 64] their token ids
-  float* q;               // [B * N, 64] the draft's probabilities of them
-  float* raw;             // [B * N] the draft's probability of the node's token at its parent
   int32_t* path;          // [B, N]
   int32_t* n_path;        // [B]
   int64_t* out;           // [B, N]
@@ -69,46 +68,16 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 // Inclusive prefixes of 64 values, value j in lane j % 32 of a[j / 32].
 __device__ __forceinline__ void warp_prefix_d(const double (&a)[2], double (&c)[2], int lane) {
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    c[u] = a[u];
+  for (int u = 0; u < 2; ++u) c[u] = a[u];
 #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-      const double o = __shfl_up_sync(0xffffffffu, c[u], m);
-      if (lane >= m) c[u] += o;
+  for (int m = 1; m < 32; m <<= 1) {
+    const double o0 = __shfl_up_sync(0xffffffffu, c[0], m), o1 = __shfl_up_sync(0xffffffffu, c[1], m);
+    if (lane >= m) {
+      c[0] += o0;
+      c[1] += o1;
     }
   }
   c[1] += __shfl_sync(0xffffffffu, c[0], 31);
-}
-
-// A node's distribution from its `have` <= K largest logits above -inf, in order
-// (none: all alike).
-__device__ __forceinline__ void node_weights(const VerifyParams& p, const uint32_t* key, const int* ids, int have,
-                                             int64_t row, int lane) {
-  const float v0 = have > 0 ? key_logit(key[0]) : 0.0f;
-  double w[2], c[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int j = lane + 32 * u;
-    w[u] = 0.0;
-    if (j < have || (have == 0 && j < p.K)) {
-      const float v = have > 0 ? key_logit(key[j]) : 0.0f;
-      w[u] = v == v0 ? 1.0 : exp(((double)v - (double)v0) * p.inv_t);
-    }
-  }
-  const double s = warp_sum_d(w[0] + w[1]);
-#pragma unroll
-  for (int u = 0; u < 2; ++u) w[u] /= s;
-  warp_prefix_d(w, c, lane);
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-    if (!(c[u] - w[u] <= p.top_p)) w[u] = 0.0;
-  const double t = warp_sum_d(w[0] + w[1]);
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int j = lane + 32 * u;
-    p.w[row * kVerMaxK + j] = w[u] / t;
-    p.id[row * kVerMaxK + j] = j < have || (have == 0 && j < p.K) ? ids[j] : -1;
-  }
 }
 
 // ------------------------------------------------------------- tile kernel --
@@ -116,13 +85,19 @@ __device__ __forceinline__ void node_weights(const VerifyParams& p, const uint32
 // per thread in flight together, and keeps each vector's maximum.  T, just
 // below the K-th largest of the 256 threads' maxima, is at most the tile's
 // K-th largest logit, and few logits reach it (about K of 16384: threads seldom
-// hold two); the vectors that do are looked at again, one element per thread.
-// T is found bit by bit, one warp counting the maxima with votes, from the
-// first bit in which they differ until close to K of them reach it: a T a
-// little too low only lets a few more through.  Where more than kVerCap come
-// through (ties, large logits side by side) the tile's K largest are selected
-// exactly, ties to the lowest ids.  -inf and NaN are not handed on: they have no weight, and a row
-// of nothing else is known by having no candidates.
+// hold two); a thread looks again into its own vectors that do.  T is found bit
+// by bit, one warp counting the maxima with votes, from the first bit in which
+// they differ until close to K of them reach it: a T a little too low only lets
+// a few more through.  Where more than kVerCap come through (ties, large logits
+// side by side) the tile's K largest are selected exactly, ties to the lowest
+// ids.  -inf and NaN are not handed on: they have no weight, and a row of
+// nothing else is known by having no candidates.  Five CTAs per SM: their loads
+// cover each other's search for T (a ring of tiles in shared memory with two
+// CTAs per SM measured slower, 45 against 40 us for 64 x 8 rows of 151936).
+// One word whose order is larger logit, then lower id.
+__device__ __forceinline__ unsigned long long cand_word(const uint2& v) {
+  return (unsigned long long)v.x << 32 | (0xffffffffu - v.y);
+}
 __device__ __forceinline__ uint4 ld_once_u4(const void* p) {  // written by the launch before: not the read-only path
   uint4 r;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
@@ -150,337 +125,397 @@ struct VerWord { using type = uint32_t; };
 template <>
 struct VerWord<kBF16> { using type = uint16_t; };
 
+// Exactly the K largest logits above -inf of a tile in shared memory (all of
+// them where there are fewer), in no order, into `list`; their number.  The
+// smallest one's word by halving, all above it, and its first ties in order of
+// ids.  The tile's words take the place of its logits.  For all threads of the
+// CTA at once.
+template <int XT>
+__device__ __noinline__ int verify_tile_exact(const VerifyParams& p, uint4* tile, int k0, uint2* list, int* s_cnt,
+                                              int* s_warp) {
+  constexpr int EPC = XT == kBF16 ? 8 : 4, SH = XT == kBF16 ? 16 : 0, TILE = kVerThreads * kVerVecs * EPC;
+  constexpr uint32_t kInf = 0x007fffffu >> SH;  // word of -inf
+  using Word = typename VerWord<XT>::type;
+  Word* words = reinterpret_cast<Word*>(tile);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int j = tid; j < TILE; j += kVerThreads) {
+    const int k = k0 + j;
+    words[j] = (Word)(k >= 0 && k < p.V ? logit_key(load_f<XT>(tile, j)) >> SH : 0u);
+  }
+  int flip = 0;
+  auto count = [&](uint32_t c) {  // words at or above c
+    if (tid == 0) s_cnt[flip] = 0;
+    __syncthreads();
+    int cnt = 0;
+    for (int i = 0; i < kVerVecs; ++i) {
+      const uint4 v = tile[i * kVerThreads + tid];
+      const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (XT == kBF16) cnt += ((q[e] & 0xffffu) >= c) + ((q[e] >> 16) >= c);
+        else cnt += q[e] >= c;
+      }
+    }
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+    if (lane == 0) atomicAdd(&s_cnt[flip], cnt);
+    __syncthreads();
+    cnt = s_cnt[flip];
+    flip ^= 1;
+    return cnt;
+  };
+  const int want = min(p.K, count(kInf + 1));
+  if (want == 0) return 0;
+  uint32_t kth = 0;
+  for (int bit = 31 - SH; bit >= 0; --bit)
+    if (count(kth | (1u << bit)) >= want) kth |= 1u << bit;
+  __syncthreads();  // everyone has the last count
+  if (tid == 0) s_cnt[0] = 0;
+  __syncthreads();
+  auto key_of = [](uint32_t w) {  // the whole word again
+    return XT == kBF16 ? (w & 0x8000u ? w << 16 : w << 16 | 0xffffu) : w;
+  };
+  for (int j = tid; j < TILE; j += kVerThreads)
+    if (words[j] > kth) list[atomicAdd(&s_cnt[0], 1)] = make_uint2(key_of(words[j]), (uint32_t)(k0 + j));
+  __syncthreads();
+  int base = s_cnt[0];  // fewer than `want`
+  for (int j0 = 0; j0 < TILE && base < want; j0 += kVerThreads) {
+    const unsigned vote = __ballot_sync(0xffffffffu, words[j0 + tid] == kth);
+    if (lane == 0) s_warp[warp] = __popc(vote);
+    __syncthreads();
+    int at = base + __popc(vote & ((1u << lane) - 1u)), all = 0;
+    for (int w = 0; w < kVerThreads / 32; ++w) {
+      if (w < warp) at += s_warp[w];
+      all += s_warp[w];
+    }
+    if (((vote >> lane) & 1u) && at < want) list[at] = make_uint2(key_of(kth), (uint32_t)(k0 + j0 + tid));
+    base += all;
+    __syncthreads();
+  }
+  return want;
+}
+
+// A word that at least K, and not many more, of 32 x PER words reach, for one
+// warp: bit by bit from the first bit in which they differ, counting with votes.
+template <int PER, typename At>
+__device__ __forceinline__ uint32_t warp_threshold(At at, int K, int last_bit, int lane) {
+  uint32_t key[PER], hi = 0, lo = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    key[i] = at(lane + 32 * i);
+    hi = max(hi, key[i]);
+    lo = min(lo, key[i]);
+  }
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  if (K == 1) return hi;
+  const int top = 31 - __clz((int)(hi ^ lo));  // -1: they are all equal
+  uint32_t t = top < 0 ? lo : lo & ~((2u << top) - 1u);
+  int reach = 32 * PER;
+  for (int bit = top; bit >= last_bit && reach > K + (K >> 3); --bit) {
+    const uint32_t c = t | (1u << bit);
+    int cnt = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) cnt += __popc(__ballot_sync(0xffffffffu, key[i] >= c));
+    if (cnt >= K) {
+      t = c;
+      reach = cnt;
+    }
+  }
+  return t;
+}
+
+// Vector v of a tile (its first element k of the row): the row's logits, -inf
+// outside of it.
+template <int XT>
+__device__ __forceinline__ uint4 edge_vector(const char* x, int k, int V) {
+  constexpr int EPC = XT == kBF16 ? 8 : 4;
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < EPC; ++e) {
+    const bool in = k + e >= 0 && k + e < V;
+    if constexpr (XT == kBF16) {
+      const uint32_t h = in ? reinterpret_cast<const uint16_t*>(x)[k + e] : 0xff80u;
+      w[e >> 1] |= h << (16 * (e & 1));
+    } else {
+      w[e] = in ? reinterpret_cast<const uint32_t*>(x)[k + e] : 0xff800000u;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <int XT>
 __global__ void __launch_bounds__(kVerThreads, 5) verify_tile_kernel(VerifyParams p) {
   constexpr int ES = XT == kBF16 ? 2 : 4, EPC = 16 / ES, SH = XT == kBF16 ? 16 : 0;  // SH: low key bits that say nothing
+  constexpr int VECS = kVerVecs * kVerThreads, TILE = VECS * EPC;
   __shared__ float s_max[kVerThreads];
   __shared__ uint32_t s_t;
-  __shared__ int s_n, s_vecs, s_cnt[2];
+  __shared__ int s_n, s_cnt[2];
   __shared__ int s_warp[kVerThreads / 32];
-  __shared__ uint4 s_tile[kVerThreads * kVerVecs];  // vectors of interest (their numbers), or the tile's words
-  int* s_vec = reinterpret_cast<int*>(s_tile);
   __shared__ uint2 s_list[kVerCap];
+  __shared__ uint4 s_tile[VECS];  // the exact selection's words
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tile = blockIdx.x, n = blockIdx.y, b = blockIdx.z;
-  const float ninf = __int_as_float(0xff800000);
   pdl_wait();
   pdl_trigger();
   const int64_t row = (int64_t)b * p.N + n;
-  if (p.parents[row] < -1) return;  // padding
   const char* x = static_cast<const char*>(p.logits) + (b * p.l_sb + n * p.l_sn) * ES;
   const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15) / ES;  // elements between a 16-byte boundary and the row
-  const int k0 = tile * (kVerVecs * kVerThreads) * EPC - off;       // the tile's first element; < 2^30 + a tile
+  const int k0 = tile * TILE - off;                                 // the tile's first element; < 2^30 + a tile
+  const bool inner = k0 >= 0 && k0 + TILE <= p.V;
+  if (p.parents[row] < -1) return;  // padding
+  const char* src = x + ((int64_t)k0 + tid * EPC) * ES;
   uint4 r[kVerVecs];
+  if (inner) {
 #pragma unroll
-  for (int i = 0; i < kVerVecs; ++i) {
-    const int k = k0 + (i * kVerThreads + tid) * EPC;
-    if (k >= 0 && k + EPC <= p.V) {
-      r[i] = ld_once_u4(x + (int64_t)k * ES);
-    } else {  // the row's ends, element by element; -inf outside
-      uint32_t w[4] = {0, 0, 0, 0};
+    for (int i = 0; i < kVerVecs; ++i) r[i] = ld_once_u4(src + i * kVerThreads * 16);
+  } else {
 #pragma unroll
-      for (int e = 0; e < EPC; ++e) {
-        const bool in = k + e >= 0 && k + e < p.V;
-        if constexpr (XT == kBF16) {
-          const uint32_t h = in ? reinterpret_cast<const uint16_t*>(x)[k + e] : 0xff80u;
-          w[e >> 1] |= h << (16 * (e & 1));
-        } else {
-          w[e] = in ? reinterpret_cast<const uint32_t*>(x)[k + e] : 0xff800000u;
-        }
-      }
-      r[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < kVerVecs; ++i) {
+      const int k = k0 + (i * kVerThreads + tid) * EPC;
+      r[i] = k >= 0 && k + EPC <= p.V ? ld_once_u4(src + i * kVerThreads * 16) : edge_vector<XT>(x, k, p.V);
     }
   }
-  if (tid == 0) s_n = s_vecs = 0;
-  float vm[kVerVecs], mx = ninf;
+  if (tid == 0) s_n = 0;
+  float vm[kVerVecs], mx = __int_as_float(0xff800000);
 #pragma unroll
   for (int i = 0; i < kVerVecs; ++i) {
-    const uint32_t w = max_word<XT>(max_word<XT>(r[i].x, r[i].y), max_word<XT>(r[i].z, r[i].w));
-    vm[i] = word_max<XT>(w);
+    vm[i] = word_max<XT>(max_word<XT>(max_word<XT>(r[i].x, r[i].y), max_word<XT>(r[i].z, r[i].w)));
     mx = fmaxf(mx, vm[i]);
   }
   s_max[tid] = mx;
   __syncthreads();
+  constexpr uint32_t kLowest = 0x00800000u;  // word of the lowest finite value
   if (warp == 0) {
-    uint32_t key[kVerThreads / 32], hi = 0, lo = 0xffffffffu;
+    const uint32_t t = warp_threshold<kVerThreads / 32>([&](int j) { return logit_key(s_max[j]); }, p.K, SH, lane);
+    if (lane == 0) s_t = max(t, kLowest);  // fewer than K finite maxima: all that is above -inf
+  }
+  __syncthreads();
+  const float tf = key_logit(s_t);
+  uint32_t in = 0;  // this thread's vectors that reach T; lanes go through theirs side by side
 #pragma unroll
-    for (int i = 0; i < kVerThreads / 32; ++i) {
-      key[i] = logit_key(s_max[lane + 32 * i]);
-      hi = max(hi, key[i]);
-      lo = min(lo, key[i]);
-    }
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    const int top = 31 - __clz((int)(hi ^ lo));  // first bit in which they differ; -1: they are all equal
-    uint32_t t = top < 0 ? lo : lo & ~((2u << top) - 1u);
-    int reach = kVerThreads;
-    for (int bit = top; bit >= SH && reach > p.K + (p.K >> 3); --bit) {
-      const uint32_t c = t | (1u << bit);
-      int cnt = 0;
+  for (int i = 0; i < kVerVecs; ++i) in |= (vm[i] >= tf ? 1u : 0u) << i;
+#pragma unroll 1
+  for (; in; in &= in - 1) {
+    const int i = __ffs((int)in) - 1, k = k0 + (i * kVerThreads + tid) * EPC;
+    const uint4 v = k >= 0 && k + EPC <= p.V ? ld_once_u4(src + i * kVerThreads * 16) : edge_vector<XT>(x, k, p.V);
+    const uint32_t q[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < kVerThreads / 32; ++i) cnt += __popc(__ballot_sync(0xffffffffu, key[i] >= c));
-      if (cnt >= p.K) {
-        t = c;
-        reach = cnt;
+    for (int e = 0; e < EPC; ++e) {
+      const uint32_t w = q[e * ES / 4];
+      const float y = __uint_as_float(XT == kBF16 ? (e & 1 ? w & 0xffff0000u : w << 16) : w);
+      if (y >= tf && k + e >= 0 && k + e < p.V) {
+        const int at = atomicAdd(&s_n, 1);
+        if (at < kVerCap) s_list[at] = make_uint2(logit_key(y), (uint32_t)(k + e));
       }
-    }
-    if (lane == 0) s_t = t;
-  }
-  __syncthreads();
-  // just above -inf where T is not above it (fewer than K finite maxima)
-  const uint32_t t = max(s_t, 0x00800000u);
-  const float tf = key_logit(t);
-  if (mx >= tf) {
-#pragma unroll
-    for (int i = 0; i < kVerVecs; ++i)
-      if (vm[i] >= tf) s_vec[atomicAdd(&s_vecs, 1)] = i * kVerThreads + tid;
-  }
-  __syncthreads();
-  for (int j = tid; j < s_vecs * EPC; j += kVerThreads) {
-    const int k = k0 + s_vec[j / EPC] * EPC + j % EPC;
-    if (k < 0 || k >= p.V) continue;
-    const float v = load_f<XT>(x, k);
-    if (v >= tf) {
-      const int at = atomicAdd(&s_n, 1);
-      if (at < kVerCap) s_list[at] = make_uint2(logit_key(v), (uint32_t)k);
     }
   }
   __syncthreads();
   int found = s_n;
   if (found > kVerCap) {
-    // exactly the K largest of the tile, from its words in shared memory: their
-    // smallest by halving, all above it, and its first ties in order of ids
-    using Word = typename VerWord<XT>::type;
-    Word* words = reinterpret_cast<Word*>(s_tile);
-    constexpr int TILE = kVerThreads * kVerVecs * EPC;
-#pragma unroll 8
-    for (int j = tid; j < TILE; j += kVerThreads) {
-      const int k = k0 + j;
-      const uint32_t key = k >= 0 && k < p.V ? logit_key(load_f<XT>(x, k)) : 0u;
-      words[j] = (Word)(key >= t ? key >> SH : 0u);  // 0: not of interest
-    }
-    uint32_t kth = 0;
-    int flip = 0;
 #pragma unroll 1
-    for (int bit = 31 - SH; bit >= 0; --bit) {
-      const uint32_t c = kth | (1u << bit);
-      if (tid == 0) s_cnt[flip] = 0;
-      __syncthreads();
-      int cnt = 0;
-#pragma unroll 2
-      for (int i = 0; i < kVerVecs; ++i) {
-        const uint4 v = s_tile[i * kVerThreads + tid];
-        const uint32_t q[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (XT == kBF16) cnt += ((q[e] & 0xffffu) >= c) + ((q[e] >> 16) >= c);
-          else cnt += q[e] >= c;
-        }
-      }
-      cnt = __reduce_add_sync(0xffffffffu, cnt);
-      if (lane == 0) atomicAdd(&s_cnt[flip], cnt);
-      __syncthreads();
-      if (s_cnt[flip] >= p.K) kth = c;
-      flip ^= 1;
-    }
-    if (tid == 0) s_n = 0;
+    for (int i = 0; i < kVerVecs; ++i) s_tile[i * kVerThreads + tid] = edge_vector<XT>(x, k0 + (i * kVerThreads + tid) * EPC, p.V);
     __syncthreads();
-    auto key_of = [](uint32_t w) {  // the whole word again
-      return XT == kBF16 ? (w & 0x8000u ? w << 16 : w << 16 | 0xffffu) : w;
-    };
-    for (int j = tid; j < TILE; j += kVerThreads)
-      if (words[j] > kth) s_list[atomicAdd(&s_n, 1)] = make_uint2(key_of(words[j]), (uint32_t)(k0 + j));
+    found = verify_tile_exact<XT>(p, s_tile, k0, s_list, s_cnt, s_warp);
     __syncthreads();
-    int base = s_n;  // fewer than K
-#pragma unroll 1
-    for (int j0 = 0; j0 < TILE && base < p.K; j0 += kVerThreads) {
-      const unsigned vote = __ballot_sync(0xffffffffu, words[j0 + tid] == kth);
-      if (lane == 0) s_warp[warp] = __popc(vote);
-      __syncthreads();
-      int at = base + __popc(vote & ((1u << lane) - 1u)), all = 0;
-      for (int w = 0; w < kVerThreads / 32; ++w) {
-        if (w < warp) at += s_warp[w];
-        all += s_warp[w];
-      }
-      if (((vote >> lane) & 1u) && at < p.K) s_list[at] = make_uint2(key_of(kth), (uint32_t)(k0 + j0 + tid));
-      base += all;
-      __syncthreads();
-    }
-    found = p.K;
   }
   const int64_t slot = row * p.tiles + tile;
   if (tid < found) p.cand[slot * kVerCap + tid] = s_list[tid];
   if (tid == 0) p.n_cand[slot] = found;
 }
 
-// -------------------------------------------------------------- row kernel --
-// One CTA per node: the K largest of the tiles' candidates in order, their
-// weights, and the draft's probabilities at them (so that the walk has nothing
-// left to fetch token by token).  The K-th largest word is found bit by bit
-// over the candidates in shared memory, what reaches it is put in order by
-// counting what stands before each.
-constexpr int kVerRank = 128;  // candidates that are put in order by counting
+// ------------------------------------------------------------------- walk --
+// One cluster of CTAs per sequence, four warps per node: the K largest of the
+// node's candidates in order, their weights, and the draft's probabilities at
+// them, into the shared memory of the cluster's first CTA, where one warp then
+// walks with nothing left to fetch.  Bound by latency, so the work is spread: a
+// thread per candidate of a tile (kVerCap = 128 of them), and per kept one that
+// counts what stands before it.  With one warp per node the same took 15 us
+// more (64 x 8, 50 kept of 590 candidates).
+constexpr int kVerBuf = 1024;                 // candidates of a node held at a time
+constexpr int kVerRank = kVerCap;             // of which at most so many are put in order by counting
+constexpr int kVerWalkThreads = 512;
+constexpr int kVerGroups = kVerWalkThreads / kVerCap;  // nodes at a time in a CTA
 
-// One word whose order is larger logit, then lower id.
-__device__ __forceinline__ unsigned long long cand_word(const uint2& v) {
-  return (unsigned long long)v.x << 32 | (0xffffffffu - v.y);
+struct VerGroup {
+  unsigned long long buf[kVerBuf];
+  unsigned long long lim[kVerCap / 32][2];
+  int cnt[2][kVerCap / 32];
+  int n;
+};
+
+__device__ __forceinline__ void group_sync(int group) {
+  asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(kVerCap) : "memory");
+}
+
+// The K best of a row's candidates, in order, in g.buf[0 ..]; their number.
+__device__ __forceinline__ int row_select(const VerifyParams& p, int64_t row, VerGroup& g, int group, int gt) {
+  constexpr int WARPS = kVerCap / 32;
+  const int lane = gt & 31, warp = gt >> 5;
+  static_assert(kVerMaxK + kVerCap <= kVerBuf, "a tile fits behind what is carried");
+  int have = 0, flip = 0;  // carried from the batches before
+  for (int t0 = 0; t0 < p.tiles;) {
+    // as many of the next 32 tiles as fit
+    const int c = t0 + lane < p.tiles ? __ldcg(&p.n_cand[row * p.tiles + t0 + lane]) : 0;
+    int pre = c;  // c and its prefixes: 0 and the total past the last tile
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, pre, m);
+      if (lane >= m) pre += o;
+    }
+    const int nt = min(__popc(__ballot_sync(0xffffffffu, have + pre <= kVerBuf)), p.tiles - t0);
+    const int total = have + __shfl_sync(0xffffffffu, pre, nt - 1);
+    const uint2* src = p.cand + (row * p.tiles + t0) * kVerCap + gt;
+#pragma unroll 1
+    for (int t = 0; t < nt; t += 8) {
+      uint2 v[8];
+      int at[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int cnt = __shfl_sync(0xffffffffu, c, (t + i) & 31), end = __shfl_sync(0xffffffffu, pre, (t + i) & 31);
+        at[i] = t + i < nt && gt < cnt ? have + end - cnt + gt : -1;
+        if (at[i] >= 0) v[i] = __ldcg(src + (t + i) * kVerCap);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (at[i] >= 0) g.buf[at[i]] = cand_word(v[i]);
+    }
+    group_sync(group);
+    const int want = min(p.K, total);
+    int m = total;
+    if (total > kVerRank) {
+      // a word that between `want` and kVerRank of them reach, from the first bit in which they differ
+      unsigned long long hi = 0, lo = ~0ull;
+      for (int e = gt; e < total; e += kVerCap) {
+        hi = max(hi, g.buf[e]);
+        lo = min(lo, g.buf[e]);
+      }
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) {
+        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      }
+      if (lane == 0) {
+        g.lim[warp][0] = hi;
+        g.lim[warp][1] = lo;
+      }
+      if (gt == 0) g.n = 0;
+      group_sync(group);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        hi = max(hi, g.lim[w][0]);
+        lo = min(lo, g.lim[w][1]);
+      }
+      const int top = 63 - __clzll((long long)(hi ^ lo));  // the words are all different
+      unsigned long long t = top == 63 ? 0ull : lo & ~((2ull << top) - 1ull);
+#pragma unroll 1
+      for (int bit = top; bit >= 0 && m > kVerRank; --bit) {
+        const unsigned long long d = t | (1ull << bit);
+        int cnt = 0;
+#pragma unroll 4
+        for (int e = gt; e < total; e += kVerCap) cnt += g.buf[e] >= d;
+        cnt = __reduce_add_sync(0xffffffffu, cnt);
+        if (lane == 0) g.cnt[flip][warp] = cnt;
+        group_sync(group);
+        cnt = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) cnt += g.cnt[flip][w];
+        flip ^= 1;
+        if (cnt >= want) {
+          t = d;
+          m = cnt;
+        }
+      }
+      unsigned long long v[kVerBuf / kVerCap];
+#pragma unroll
+      for (int i = 0; i < kVerBuf / kVerCap; ++i) v[i] = gt + i * kVerCap < total ? g.buf[gt + i * kVerCap] : 0ull;
+      group_sync(group);
+#pragma unroll
+      for (int i = 0; i < kVerBuf / kVerCap; ++i)
+        if (gt + i * kVerCap < total && v[i] >= t) g.buf[atomicAdd(&g.n, 1)] = v[i];
+      group_sync(group);
+    }
+    // in order: each counts what stands before it
+    const unsigned long long v = gt < m ? g.buf[gt] : 0ull;
+    int r = gt < m ? 0 : kVerMaxK;
+#pragma unroll 8
+    for (int j = 0; j < m; ++j) r += g.buf[j] > v;
+    group_sync(group);
+    if (r < want) g.buf[r] = v;
+    group_sync(group);
+    have = want;
+    t0 += nt;
+  }
+  return have;
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kVerThreads) verify_row_kernel(VerifyParams p) {
-  __shared__ uint2 s_c[kVerBatch];
-  __shared__ unsigned long long s_best[kVerRank];
-  __shared__ uint2 s_sorted[kVerMaxK];
-  __shared__ uint32_t s_key[kVerMaxK];
-  __shared__ int s_id[kVerMaxK];
-  __shared__ int s_red[2][kVerThreads / 32];
-  __shared__ int s_off[33];
-  __shared__ int s_m;
-  constexpr int PER = (kVerBatch - kVerMaxK) / kVerCap;  // tiles per batch
-  static_assert(PER <= 32, "a warp scans a batch's counts");
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int n = blockIdx.x, b = blockIdx.y;
-  pdl_wait();
-  pdl_trigger();
-  const int64_t row = (int64_t)b * p.N + n;
-  const int parent = p.parents[row];
-  if (parent < -1) return;
-  int flip = 0;
-  auto count = [&](auto pred, int m) {  // candidates of the batch for which pred holds
-    int c = 0;
-    for (int e = tid; e < m; e += kVerThreads) c += pred(s_c[e]);
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0) s_red[flip][warp] = c;
-    __syncthreads();
-    c = 0;
-#pragma unroll
-    for (int w = 0; w < kVerThreads / 32; ++w) c += s_red[flip][w];
-    flip ^= 1;
-    return c;
-  };
-  int have = 0;  // candidates carried from the batches before
-  for (int t0 = 0; t0 < p.tiles; t0 += PER) {
-    const int nt = min(PER, p.tiles - t0);
-    if (warp == 0) {
-      int c = lane < nt ? __ldcg(&p.n_cand[row * p.tiles + t0 + lane]) : 0, pre = c;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, pre, m);
-        if (lane >= m) pre += o;
-      }
-      s_off[lane] = have + pre - c;
-      if (lane == 31) s_off[32] = have + pre;
-    }
-    __syncthreads();
-    for (int t = warp; t < nt; t += kVerThreads / 32) {
-      const int at = s_off[t], c = s_off[t + 1] - at;
-      for (int e = lane; e < c; e += 32) s_c[at + e] = __ldcg(&p.cand[(row * p.tiles + t0 + t) * kVerCap + e]);
-    }
-    if (tid < have) s_c[tid] = s_sorted[tid];
-    __syncthreads();
-    const int total = s_off[32], want = min(p.K, total);
-    int m = total;
-    if (total > kVerRank) {
-      // cut down to between `want` and kVerRank: T from the first bit in which the words differ
-      uint32_t hi = 0, lo = 0xffffffffu;
-      for (int e = tid; e < total; e += kVerThreads) {
-        hi = max(hi, s_c[e].x);
-        lo = min(lo, s_c[e].x);
-      }
-      hi = __reduce_max_sync(0xffffffffu, hi);
-      lo = __reduce_min_sync(0xffffffffu, lo);
-      if (lane == 0) {
-        s_red[0][warp] = (int)hi;
-        s_red[1][warp] = (int)lo;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kVerThreads / 32; ++w) {
-        hi = max(hi, (uint32_t)s_red[0][w]);
-        lo = min(lo, (uint32_t)s_red[1][w]);
-      }
-      __syncthreads();
-      const int top = 31 - __clz((int)(hi ^ lo));
-      uint32_t t = top < 0 ? lo : lo & ~((2u << top) - 1u);
-      int k = total;
-      for (int bit = top; bit >= 0 && k > kVerRank; --bit) {
-        const uint32_t c = t | (1u << bit);
-        const int kc = count([&](const uint2& v) { return v.x >= c; }, total);
-        if (kc >= want) {
-          t = c;
-          k = kc;
-        }
-      }
-      uint32_t last = 0xffffffffu;  // highest id taken among the words equal to t
-      if (k > kVerRank) {
-        const int ties = want - count([&](const uint2& v) { return v.x > t; }, total);
-        last = 0;
-        for (int bit = 30; bit >= 0; --bit) {  // ids are below 2^30; last + 1 such that `ties` are below it
-          const uint32_t c = last | (1u << bit);
-          if (count([&](const uint2& v) { return v.x == t && v.y < c; }, total) < ties) last = c;
-        }
-      }
-      if (tid == 0) s_m = 0;
-      __syncthreads();
-      for (int e = tid; e < total; e += kVerThreads) {
-        const uint2 v = s_c[e];
-        if (v.x > t || (v.x == t && v.y <= last)) s_best[atomicAdd(&s_m, 1)] = cand_word(v);
-      }
-      __syncthreads();
-      m = s_m;
-    } else {
-      if (tid < total) s_best[tid] = cand_word(s_c[tid]);
-      __syncthreads();
-    }
-    if (tid < m) {
-      const unsigned long long v = s_best[tid];
-      int r = 0;
-#pragma unroll 8
-      for (int j = 0; j < m; ++j) r += s_best[j] > v;
-      if (r < want) s_sorted[r] = make_uint2((uint32_t)(v >> 32), 0xffffffffu - (uint32_t)v);
-    }
-    __syncthreads();
-    have = want;
-  }
-  if (tid < kVerMaxK) {
-    const uint2 v = tid < have ? s_sorted[tid] : make_uint2(0u, 0u);
-    s_key[tid] = v.x;
-    s_id[tid] = have > 0 ? (int)v.y : tid;  // nothing above -inf: the lowest ids share alike
-    if (p.draft != nullptr) {
-      const bool used = tid < have || (have == 0 && tid < p.K);
-      p.q[row * kVerMaxK + tid] =
-          used ? load_f<DT>(static_cast<const char*>(p.draft) + (b * p.d_sb + n * p.d_sn) * (DT == kBF16 ? 2 : 4), s_id[tid])
-               : 0.0f;
-    }
-  }
-  if (tid == kVerMaxK && p.draft != nullptr) {
-    const int64_t x = p.tokens[row];
-    p.raw[row] = parent >= 0 && parent < n && x >= 0 && x < p.V
-                     ? load_f<DT>(static_cast<const char*>(p.draft) +
-                                  (b * p.d_sb + parent * p.d_sn) * (DT == kBF16 ? 2 : 4), x)
-                     : 0.0f;
-  }
-  __syncthreads();
-  if (warp == 0) node_weights(p, s_key, s_id, have, row, lane);
-}
-
-// ------------------------------------------------------------------- walk --
-// One CTA per sequence: all of its nodes' distributions into shared memory at
-// once, then one warp walks, nodes and candidates two per lane.
-__global__ void __launch_bounds__(kVerThreads) verify_walk_kernel(VerifyParams p) {
+__global__ void __launch_bounds__(kVerWalkThreads) verify_walk_kernel(VerifyParams p) {
   extern __shared__ __align__(16) unsigned char dyn[];
-  double* s_w = reinterpret_cast<double*>(dyn);                 // [N][64]
-  int* s_id = reinterpret_cast<int*>(s_w + p.N * kVerMaxK);     // [N][64]
-  float* s_q = reinterpret_cast<float*>(s_id + p.N * kVerMaxK); // [N][64]
-  const int tid = threadIdx.x, lane = tid & 31, b = blockIdx.x;
+  VerGroup* s_group = reinterpret_cast<VerGroup*>(dyn);                     // [kVerGroups]
+  double* s_w = reinterpret_cast<double*>(s_group + kVerGroups);            // [N][64] weights, falling
+  int* s_id = reinterpret_cast<int*>(s_w + p.N * kVerMaxK);                 // [N][64] their token ids
+  float* s_q = reinterpret_cast<float*>(s_id + p.N * kVerMaxK);             // [N][64] the draft's probabilities of them
+  float* s_raw = s_q + p.N * kVerMaxK;                                      // [N] that of the node's token at its parent
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, group = tid / kVerCap, gt = tid % kVerCap;
+  const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks(), b = (int)(blockIdx.x / ranks);
   pdl_wait();
   pdl_trigger();
   const int64_t base = (int64_t)b * p.N;
-  for (int e = tid; e < p.N * kVerMaxK; e += kVerThreads) {
-    s_w[e] = __ldcg(p.w + base * kVerMaxK + e);  // a padding node's is never looked at
-    s_id[e] = __ldcg(p.id + base * kVerMaxK + e);
-    s_q[e] = p.draft != nullptr ? __ldcg(p.q + base * kVerMaxK + e) : 0.0f;
+  for (int n = rank * kVerGroups + group; n < p.N; n += ranks * kVerGroups) {
+    const int parent = p.parents[base + n];
+    const int64_t own = p.tokens[base + n];
+    if (parent < -1) continue;  // padding: never looked at
+    VerGroup& g = s_group[group];
+    const int have = row_select(p, base + n, g, group, gt);
+    if (gt < 32) {
+      // `have` of K logits above -inf (none: the lowest ids share alike)
+      constexpr int DS = DT == kBF16 ? 2 : 4;
+      float q[2] = {0.0f, 0.0f}, raw = 0.0f;
+      int id[2];
+      unsigned long long word[2];
+      if (p.draft != nullptr && parent >= 0 && parent < n && own >= 0 && own < p.V)
+        raw = load_f<DT>(static_cast<const char*>(p.draft) + (b * p.d_sb + parent * p.d_sn) * DS, own);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int j = lane + 32 * u;
+        word[u] = j < have ? g.buf[j] : 0ull;
+        id[u] = j < have ? (int)(0xffffffffu - (uint32_t)word[u]) : have == 0 && j < p.K ? j : -1;
+        if (p.draft != nullptr && id[u] >= 0)
+          q[u] = load_f<DT>(static_cast<const char*>(p.draft) + (b * p.d_sb + n * p.d_sn) * DS, id[u]);
+      }
+      const float v0 = key_logit((uint32_t)(g.buf[0] >> 32));
+      double w[2], c[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float v = key_logit((uint32_t)(word[u] >> 32));
+        w[u] = id[u] < 0 ? 0.0 : have == 0 || v == v0 ? 1.0 : exp(((double)v - (double)v0) * p.inv_t);
+      }
+      // the nucleus: falling weights are kept while the sum before them is at most top_p of all
+      warp_prefix_d(w, c, lane);
+      const double most = p.top_p * __shfl_sync(0xffffffffu, c[1], 31);
+      bool keep[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) keep[u] = c[u] - w[u] <= most;
+      const unsigned long long kept = ((unsigned long long)__ballot_sync(0xffffffffu, keep[1]) << 32) |
+                                      __ballot_sync(0xffffffffu, keep[0]);
+      const int last = 63 - __clzll((long long)kept);  // the first one always is
+      const double inv = 1.0 / __shfl_sync(0xffffffffu, last < 32 ? c[0] : c[1], last & 31);
+      double* l_w = cluster.map_shared_rank(s_w, 0) + n * kVerMaxK;
+      int* l_id = cluster.map_shared_rank(s_id, 0) + n * kVerMaxK;
+      float* l_q = cluster.map_shared_rank(s_q, 0) + n * kVerMaxK;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        l_w[lane + 32 * u] = keep[u] ? w[u] * inv : 0.0;
+        l_id[lane + 32 * u] = id[u];
+        l_q[lane + 32 * u] = q[u];
+      }
+      if (lane == 0) cluster.map_shared_rank(s_raw, 0)[n] = raw;
+    }
+    group_sync(group);  // the buffer is free again
   }
+  cluster.sync();
+  if (rank != 0 || tid >= 32) return;
   int par[2];
   int64_t tok[2];
   float un[2], rw[2];
@@ -490,10 +525,8 @@ __global__ void __launch_bounds__(kVerThreads) verify_walk_kernel(VerifyParams p
     par[u] = i < p.N ? p.parents[base + i] : -2;
     tok[u] = i < p.N ? p.tokens[base + i] : -1;
     un[u] = i < p.N ? p.uniform[base + i] : 0.0f;
-    rw[u] = i < p.N && p.draft != nullptr ? __ldcg(p.raw + base + i) : 0.0f;
+    rw[u] = i < p.N && p.draft != nullptr ? s_raw[i] : 0.0f;
   }
-  __syncthreads();
-  if (tid >= 32) return;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int i = lane + 32 * u;
@@ -539,7 +572,8 @@ __global__ void __launch_bounds__(kVerThreads) verify_walk_kernel(VerifyParams p
       bool hit[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) hit[u] = in && id[u] == (int)x;
-      const double px = warp_sum_d((hit[0] ? pr[0] : 0.0) + (hit[1] ? pr[1] : 0.0));
+      const unsigned h0 = __ballot_sync(0xffffffffu, hit[0]), h1 = __ballot_sync(0xffffffffu, hit[1]);  // one at most
+      const double px = (h0 | h1) ? __shfl_sync(0xffffffffu, h0 ? pr[0] : pr[1], __ffs((int)(h0 | h1)) - 1) : 0.0;
       double qx = 1.0, raw = 0.0;
       if (p.draft != nullptr) {
         // a token refused before is no longer there to draw
@@ -564,8 +598,9 @@ __global__ void __launch_bounds__(kVerThreads) verify_walk_kernel(VerifyParams p
       }
       const double total = warp_sum_d(r[0] + r[1]);
       if (total > 0.0) {
-        pr[0] = r[0] / total;
-        pr[1] = r[1] / total;
+        const double inv = 1.0 / total;
+        pr[0] = r[0] * inv;
+        pr[1] = r[1] * inv;
       }
       if (p.draft != nullptr && !p.replacement) {
 #pragma unroll
@@ -601,8 +636,7 @@ using namespace mb;
 
 extern "C" int64_t maple_verify_tree_workspace_bytes(int64_t batch, int64_t nodes, int64_t vocab, int64_t top_k) {
   if (batch < 0 || nodes <= 0 || nodes > kVerMaxNodes || vocab <= 0 || vocab > (1LL << 30) || top_k <= 0) return -1;
-  const int64_t tiles = verify_tiles(vocab, 4);  // fp32 rows have the more tiles
-  return batch * nodes * (tiles * (kVerCap * 8 + 4) + kVerMaxK * 16 + 8) + 64;
+  return batch * nodes * verify_tiles(vocab, 4) * (kVerCap * 8 + 4) + 16;  // fp32 rows have the more tiles
 }
 
 extern "C" int maple_verify_tree(const void* logits, int x_dtype, int64_t batch, int64_t nodes, int64_t vocab,
@@ -623,28 +657,37 @@ extern "C" int maple_verify_tree(const void* logits, int x_dtype, int64_t batch,
   p.logits = logits; p.tokens = tokens; p.parents = parents; p.uniform = uniform; p.draft = draft_probs;
   const int64_t rows = batch * nodes;
   p.tiles = (int)verify_tiles(vocab, x_dtype == kBF16 ? 8 : 4);
-  p.w = static_cast<double*>(workspace);
-  p.cand = reinterpret_cast<uint2*>(p.w + rows * kVerMaxK);
-  p.id = reinterpret_cast<int32_t*>(p.cand + rows * p.tiles * kVerCap);
-  p.q = reinterpret_cast<float*>(p.id + rows * kVerMaxK);
-  p.raw = p.q + rows * kVerMaxK;
-  p.n_cand = reinterpret_cast<int32_t*>(p.raw + rows);
+  p.cand = static_cast<uint2*>(workspace);
+  p.n_cand = reinterpret_cast<int32_t*>(p.cand + rows * p.tiles * kVerCap);
   p.path = path; p.n_path = n_path; p.out = out; p.err = err;
   p.l_sb = l_sb; p.l_sn = l_sn; p.d_sb = d_sb; p.d_sn = d_sn;
   p.inv_t = 1.0 / (double)temperature; p.top_p = (double)top_p;
   p.B = (int)batch; p.N = (int)nodes; p.V = (int)vocab; p.K = (int)(top_k < vocab ? top_k : vocab);
   p.replacement = replacement != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)p.tiles, (unsigned)nodes, (unsigned)batch), rgrid((unsigned)nodes, (unsigned)batch);
+  const dim3 grid((unsigned)p.tiles, (unsigned)nodes, (unsigned)batch);
   cudaError_t e = x_dtype == kBF16 ? launch_k(verify_tile_kernel<kBF16>, grid, dim3(kVerThreads), 0, st, p)
                                    : launch_k(verify_tile_kernel<kF32>, grid, dim3(kVerThreads), 0, st, p);
-  if (e == cudaSuccess)
-    e = (draft_probs && d_dtype == kBF16) ? launch_k(verify_row_kernel<kBF16>, rgrid, dim3(kVerThreads), 0, st, p)
-                                          : launch_k(verify_row_kernel<kF32>, rgrid, dim3(kVerThreads), 0, st, p);
   if (e == cudaSuccess) {
-    const int smem = (int)nodes * kVerMaxK * 16;
-    e = cudaFuncSetAttribute(verify_walk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) e = launch_k(verify_walk_kernel, dim3((unsigned)batch), dim3(kVerThreads), smem, st, p);
+    auto* walk = (draft_probs && d_dtype == kBF16) ? verify_walk_kernel<kBF16> : verify_walk_kernel<kF32>;
+    const unsigned want = (unsigned)((nodes + kVerGroups - 1) / kVerGroups), ranks = want < 8 ? want : 8;  // portable
+    const int smem = (int)(kVerGroups * sizeof(VerGroup)) + (int)nodes * kVerMaxK * 16 + kVerMaxNodes * 4;
+    e = cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)batch * ranks);
+    cfg.blockDim = dim3(kVerWalkThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, walk, p);
   }
   return e == cudaSuccess ? kOk : kErrCuda;
 }
