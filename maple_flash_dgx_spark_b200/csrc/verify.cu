@@ -299,13 +299,19 @@ __global__ void __launch_bounds__(kVerThreads, 5) verify_tile_kernel(VerifyParam
     const int i = __ffs((int)in) - 1, k = k0 + (i * kVerThreads + tid) * EPC;
     const uint4 v = k >= 0 && k + EPC <= p.V ? ld_once_u4(src + i * kVerThreads * 16) : edge_vector<XT>(x, k, p.V);
     const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+    auto value = [&](int e) {  // e a constant
+      const uint32_t w = q[e * ES / 4];
+      return __uint_as_float(XT == kBF16 ? (e & 1 ? w & 0xffff0000u : w << 16) : w);
+    };
+    uint32_t reach = 0;
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) reach |= (value(e) >= tf && k + e >= 0 && k + e < p.V ? 1u : 0u) << e;
+    int at = atomicAdd(&s_n, __popc(reach));
 #pragma unroll
     for (int e = 0; e < EPC; ++e) {
-      const uint32_t w = q[e * ES / 4];
-      const float y = __uint_as_float(XT == kBF16 ? (e & 1 ? w & 0xffff0000u : w << 16) : w);
-      if (y >= tf && k + e >= 0 && k + e < p.V) {
-        const int at = atomicAdd(&s_n, 1);
-        if (at < kVerCap) s_list[at] = make_uint2(logit_key(y), (uint32_t)(k + e));
+      if ((reach >> e) & 1u) {
+        if (at < kVerCap) s_list[at] = make_uint2(logit_key(value(e)), (uint32_t)(k + e));
+        ++at;
       }
     }
   }
