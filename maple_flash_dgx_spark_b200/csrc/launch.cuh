@@ -14,6 +14,9 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
 #include <cstdlib>
 
 namespace mb {
@@ -27,6 +30,18 @@ inline bool pdl_enabled() {
     return !(v && v[0] == '0');
   }();
   return on;
+}
+
+// Raises a kernel's dynamic shared memory limit to `bytes`, once per device
+// (`done`: a static of the caller's, one for each kernel and size).
+template <typename Kern>
+inline cudaError_t smem_once(std::atomic<uint64_t>& done, Kern kern, int bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  return e;
 }
 
 template <typename... KArgs, typename... Args>

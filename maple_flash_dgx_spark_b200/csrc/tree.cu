@@ -448,7 +448,8 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
 #define MB_TREE(XT, DD)                                                                                              \
   do {                                                                                                               \
     const size_t smem = (size_t)(kSimtRows * DD + kSimtKeys * (DD + 4) + kSimtKeys * DD) * 4;                        \
-    e = cudaFuncSetAttribute(tree_simt_kernel<XT, DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);      \
+    static std::atomic<uint64_t> done{0};                                                                            \
+    e = smem_once(done, tree_simt_kernel<XT, DD>, (int)smem);                                                        \
     if (e == cudaSuccess)                                                                                            \
       e = launch_k(tree_simt_kernel<XT, DD>, dim3((unsigned)p.NS, (unsigned)(num_kv_heads * tiles), (unsigned)batch), \
                    dim3(256), smem, st, p, (int)tiles);                                                              \

@@ -751,7 +751,8 @@ cudaError_t tree_tc_launch1(const TreeAttnParams& p, int groups, const CUtensorM
   constexpr int smem = TtShape<D, PAIR>::kSmem;
   static_assert(smem <= 232448, "shared memory of one SM");
   const int items = p.B * p.Hkv * p.NS * groups;
-  cudaError_t e = cudaFuncSetAttribute(tree_tc_kernel<D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = smem_once(done, tree_tc_kernel<D, PAIR>, smem);
   if (e == cudaSuccess)
     e = launch_k(tree_tc_kernel<D, PAIR>, dim3((unsigned)(items < 148 ? items : 148)), dim3(kTtThreads), smem, st, p,
                  groups, items, tmk, tmv);

@@ -678,7 +678,9 @@ extern "C" int maple_verify_tree(const void* logits, int x_dtype, int64_t batch,
     auto* walk = (draft_probs && d_dtype == kBF16) ? verify_walk_kernel<kBF16> : verify_walk_kernel<kF32>;
     const unsigned want = (unsigned)((nodes + kVerGroups - 1) / kVerGroups), ranks = want < 8 ? want : 8;  // portable
     const int smem = (int)(kVerGroups * sizeof(VerGroup)) + (int)nodes * kVerMaxK * 16 + kVerMaxNodes * 4;
-    e = cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done[2];
+    const int most = (int)(kVerGroups * sizeof(VerGroup)) + kVerMaxNodes * (kVerMaxK * 16 + 4);
+    e = smem_once(done[draft_probs && d_dtype == kBF16], walk, most);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)batch * ranks);
     cfg.blockDim = dim3(kVerWalkThreads);

@@ -9,6 +9,7 @@ runs unchanged.  All arithmetic happens in ``libmaple_b200.so``.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -932,38 +933,38 @@ def batched_sampler_workspace(vocab: int, top_k: int, batch: int, device):
 MAX_TREE_NODES = 64
 
 
-def _one_device(op, first, *tensors):
-    """Every tensor on the first one's GPU; returns it."""
-    require_cuda(op, first, *tensors)
-    for t in tensors:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{op}: tensors on {first.device} and {t.device}.")
-    return first.device
+def _device_error(op, *tensors):
+    """Raise for tensors off the GPU or on different GPUs."""
+    require_cuda(op, *tensors)
+    raise ValueError(f"{op}: tensors on different devices: "
+                     f"{sorted({str(t.device) for t in tensors if t is not None})}.")
 
 
-def _launch(fn, op, device, *args):
-    """``check(fn(*args, stream))`` with ``device`` current."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, stream_ptr(device)), op)
+def _launch(fn, op, d, *args):
+    """``check(fn(*args, stream))`` on GPU ``d``'s current stream, with that GPU current."""
+    if d == torch.cuda.current_device():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(d))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, stream_ptr(device)), op)
+        with torch.cuda.device(d):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(d))
+    if st:
+        check(st, op)
 
 
 def _as(t, dtype):
     return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
-def _tree_shape(op, t, what):
-    if t.ndim < 2 or not 1 <= t.shape[1] <= MAX_TREE_NODES:
-        raise ValueError(f"{op}: {what} must be [B, N, ...] with 1 to {MAX_TREE_NODES} nodes, got {tuple(t.shape)}.")
-    return int(t.shape[0]), int(t.shape[1])
+def _bad_nodes(op, n):
+    raise ValueError(f"{op}: a tree has 1 to {MAX_TREE_NODES} nodes, got {n}.")
 
 
 class TreePlan:
     """The trees of one step, shared by every layer's attention: ``parents``
     int32, ``mask`` int64 (bit j: the node sees node j) and ``depth`` int32
     (the node's ancestors), all ``[B, N]``."""
+
+    __slots__ = ("parents", "mask", "depth")
 
     def __init__(self, parents: torch.Tensor, mask: torch.Tensor, depth: torch.Tensor):
         self.parents = parents
@@ -978,17 +979,28 @@ def tree_plan(parents: torch.Tensor) -> TreePlan:
     (node 0: the last drawn token), less than -1 padding.  A parent that is not
     before its node sets the device error word; that branch becomes padding."""
     op = "tree_plan"
-    dev = _one_device(op, parents)
-    B, N = _tree_shape(op, parents, "parents")
     if parents.ndim != 2:
         raise ValueError(f"{op}: parents must be [B, N], got {tuple(parents.shape)}.")
-    if parents.is_floating_point() or parents.dtype == torch.bool:
+    B, N = parents.shape
+    if not 1 <= N <= MAX_TREE_NODES:
+        _bad_nodes(op, N)
+    d = parents.get_device()
+    if d < 0:
+        _device_error(op, parents)
+    if parents.dtype != torch.int32 and (parents.is_floating_point() or parents.dtype == torch.bool):
         raise TypeError(f"{op}: parents must be whole numbers, got {parents.dtype}.")
     par = _as(parents, torch.int32)
+    dev = par.device
     mask = torch.empty(B, N, dtype=torch.int64, device=dev)
     depth = torch.empty(B, N, dtype=torch.int32, device=dev)
-    _launch(lib().maple_tree_plan, op, dev, ptr(par), B, N, N, 1, ptr(mask), ptr(depth), ptr(_err(dev)))
+    _launch(lib().maple_tree_plan, op, d, par.data_ptr(), B, N, N, 1, mask.data_ptr(), depth.data_ptr(),
+            _err(dev).data_ptr())
     return TreePlan(par, mask, depth)
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_gqa_bytes(*shape) -> int:
+    return lib().maple_tree_gqa_workspace_bytes(*shape)
 
 
 def tree_gqa_attn(q, k_cache, v_cache, seqlen, tree_mask, *, row_map=None, scale: float, window: int | None = None):
@@ -1005,46 +1017,63 @@ def tree_gqa_attn(q, k_cache, v_cache, seqlen, tree_mask, *, row_map=None, scale
     op = "tree_gqa_attn"
     if q.ndim != 4:
         raise ValueError(f"{op} expects q [B, N, H, D], got {tuple(q.shape)}.")
-    dev = _one_device(op, q, k_cache, v_cache, seqlen, tree_mask, row_map)
-    B, N = _tree_shape(op, q, "q")
-    H, D = int(q.shape[2]), int(q.shape[3])
+    d = q.get_device()
+    if (d < 0 or k_cache.get_device() != d or v_cache.get_device() != d or seqlen.get_device() != d or
+            tree_mask.get_device() != d or (row_map is not None and row_map.get_device() != d)):
+        _device_error(op, q, k_cache, v_cache, seqlen, tree_mask, row_map)
+    B, N, H, D = q.shape
+    if not 1 <= N <= MAX_TREE_NODES:
+        _bad_nodes(op, N)
     if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != D:
         raise ValueError(f"{op}: caches must be [Bc, n_kv, T, {D}], got {tuple(k_cache.shape)} and "
                          f"{tuple(v_cache.shape)}.")
-    Bc, n_kv, T = int(k_cache.shape[0]), int(k_cache.shape[1]), int(k_cache.shape[2])
-    if H % n_kv:
+    Bc, n_kv, T, _ = k_cache.shape
+    if n_kv < 1 or H % n_kv:
         raise ValueError(f"n_q={H} not divisible by n_kv={n_kv}.")
-    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    dtype = q.dtype
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise TypeError("KV cache dtype must match q dtype.")
-    if row_map is None and Bc != B:
-        raise ValueError(f"KV cache batch {Bc} != q batch {B}.")
-    if seqlen.numel() != B or (row_map is not None and row_map.numel() != B):
-        raise ValueError(f"{op}: seqlen and row_map need {B} entries.")
-    if tuple(tree_mask.shape) != (B, N) or tree_mask.dtype != torch.int64:
+    if row_map is None:
+        if Bc != B:
+            raise ValueError(f"KV cache batch {Bc} != q batch {B}.")
+    elif row_map.numel() != B:
+        raise ValueError(f"{op}: row_map needs {B} entries, got {row_map.numel()}.")
+    if seqlen.numel() != B:
+        raise ValueError(f"{op}: seqlen needs {B} entries, got {seqlen.numel()}.")
+    if tree_mask.shape != (B, N) or tree_mask.dtype != torch.int64:
         raise ValueError(f"{op}: tree_mask must be int64 {(B, N)}, got {tree_mask.dtype} {tuple(tree_mask.shape)}.")
-    ks = k_cache.stride()
-    if ks[3] != 1 or ks[2] != D or ks != v_cache.stride():
+    sb, sh, st, sd = k_cache.stride()
+    if sd != 1 or st != D or v_cache.stride() != (sb, sh, st, sd):
         raise ValueError("KV caches must be [B, n_kv, T, D] with contiguous (T, D).")
-    if window is not None and window < 0:
+    if window is None:
+        window = 0
+    elif window < 0:
         raise ValueError(f"{op}: window must not be negative, got {window}.")
-    code, es = dtype_code(q, op), q.element_size()
-    if q.stride(3) != 1 or q.data_ptr() % 16 or any(s * es % 16 for s in q.stride()[:3]):
+    code = dtype_code(q, op)
+    per = 8 if code else 4  # elements in 16 bytes
+    qb, qn, qh, qd = q.stride()
+    if qd != 1 or qb % per or qn % per or qh % per or q.data_ptr() % 16:
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-    qs = q.stride()
+        qb, qn, qh, qd = q.stride()
     sl, tm = _as(seqlen, torch.int64), _as(tree_mask, torch.int64)
     rm = _as(row_map, torch.int32) if row_map is not None else None
-    out = torch.empty(B, N, H, D, dtype=q.dtype, device=dev)
+    dev = q.device
+    out = torch.empty(B, N, H, D, dtype=dtype, device=dev)
     if B == 0:
         return out
-    L = lib()
-    nbytes = L.maple_tree_gqa_workspace_bytes(B, N, H, n_kv, D, T, int(window or 0), code)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
-    _launch(L.maple_tree_gqa_attn, op, dev, ptr(q), code, B, N, H, qs[0], qs[1], qs[2], ptr(k_cache), ptr(v_cache),
-            Bc, n_kv, ks[0], ks[1], T, D, ptr(sl), ptr(tm), ptr(rm), float(scale), int(window or 0), ptr(out), ptr(ws),
-            max(nbytes, 0), ptr(_err(dev)))
+    nbytes = max(_tree_gqa_bytes(B, N, H, n_kv, D, T, window, code), 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch(lib().maple_tree_gqa_attn, op, d, q.data_ptr(), code, B, N, H, qb, qn, qh, k_cache.data_ptr(),
+            v_cache.data_ptr(), Bc, n_kv, sb, sh, T, D, sl.data_ptr(), tm.data_ptr(), ptr(rm), scale, window,
+            out.data_ptr(), ptr(ws), nbytes, _err(dev).data_ptr())
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _verify_bytes(*shape) -> int:
+    return lib().maple_verify_tree_workspace_bytes(*shape)
 
 
 def verify_tree(logits, tokens, parents, uniform, *, temperature: float, top_p: float, top_k: int, draft_probs=None,
@@ -1068,12 +1097,16 @@ def verify_tree(logits, tokens, parents, uniform, *, temperature: float, top_p: 
     op = "verify_tree"
     if logits.ndim != 3:
         raise ValueError(f"{op} expects logits [B, N, V], got {tuple(logits.shape)}.")
-    dev = _one_device(op, logits, tokens, parents, uniform, draft_probs)
-    B, N = _tree_shape(op, logits, "logits")
-    V = int(logits.shape[2])
-    for t, what in ((tokens, "tokens"), (parents, "parents"), (uniform, "uniform")):
-        if tuple(t.shape) != (B, N):
-            raise ValueError(f"{op}: {what} must be {(B, N)}, got {tuple(t.shape)}.")
+    d = logits.get_device()
+    if (d < 0 or tokens.get_device() != d or parents.get_device() != d or uniform.get_device() != d or
+            (draft_probs is not None and draft_probs.get_device() != d)):
+        _device_error(op, logits, tokens, parents, uniform, draft_probs)
+    B, N, V = logits.shape
+    if not 1 <= N <= MAX_TREE_NODES:
+        _bad_nodes(op, N)
+    if tokens.shape != (B, N) or parents.shape != (B, N) or uniform.shape != (B, N):
+        raise ValueError(f"{op}: tokens, parents and uniform must be {(B, N)}, got {tuple(tokens.shape)}, "
+                         f"{tuple(parents.shape)} and {tuple(uniform.shape)}.")
     if tokens.is_floating_point() or parents.is_floating_point():
         raise TypeError(f"{op}: tokens and parents must be whole numbers.")
     if V < 1:
@@ -1084,27 +1117,28 @@ def verify_tree(logits, tokens, parents, uniform, *, temperature: float, top_p: 
         raise ValueError(f"{op} needs temperature > 0 (greedy is top_k = 1).")
     if not top_p > 0:
         raise ValueError(f"{op} needs top_p > 0, got {top_p}.")
-    if draft_probs is not None and tuple(draft_probs.shape) != (B, N, V):
-        raise ValueError(f"{op}: draft_probs must be {(B, N, V)}, got {tuple(draft_probs.shape)}.")
     code = dtype_code(logits, op)
-    dcode = dtype_code(draft_probs, op) if draft_probs is not None else 0
     lg = logits if logits.stride(2) == 1 else logits.contiguous()
-    dp = draft_probs
-    if dp is not None and dp.stride(2) != 1:
-        dp = dp.contiguous()
+    dp, dcode, db, dn = None, 0, 0, 0
+    if draft_probs is not None:
+        if draft_probs.shape != (B, N, V):
+            raise ValueError(f"{op}: draft_probs must be {(B, N, V)}, got {tuple(draft_probs.shape)}.")
+        dcode = dtype_code(draft_probs, op)
+        dp = draft_probs if draft_probs.stride(2) == 1 else draft_probs.contiguous()
+        db, dn, _ = dp.stride()
     tok, par, u = _as(tokens, torch.int64), _as(parents, torch.int32), _as(uniform, torch.float32)
+    dev = lg.device
     path = torch.empty(B, N, dtype=torch.int32, device=dev)
     n_path = torch.empty(B, dtype=torch.int32, device=dev)
     ids = torch.empty(B, N, dtype=torch.int64, device=dev)
     if B == 0:
         return path, n_path, ids
-    L = lib()
-    nbytes = L.maple_verify_tree_workspace_bytes(B, N, V, top_k)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    _launch(L.maple_verify_tree, op, dev, ptr(lg), code, B, N, V, lg.stride(0), lg.stride(1), ptr(tok), ptr(par),
-            ptr(u), ptr(dp), dcode, dp.stride(0) if dp is not None else 0, dp.stride(1) if dp is not None else 0,
-            float(temperature), float(top_p), int(top_k), int(bool(replacement)), ptr(path), ptr(n_path), ptr(ids),
-            ptr(ws), ws.numel(), ptr(_err(dev)))
+    nbytes = max(_verify_bytes(B, N, V, top_k), 16)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    lb, ln, _ = lg.stride()
+    _launch(lib().maple_verify_tree, op, d, lg.data_ptr(), code, B, N, V, lb, ln, tok.data_ptr(), par.data_ptr(),
+            u.data_ptr(), ptr(dp), dcode, db, dn, temperature, top_p, top_k, 1 if replacement else 0, path.data_ptr(),
+            n_path.data_ptr(), ids.data_ptr(), ws.data_ptr(), nbytes, _err(dev).data_ptr())
     return path, n_path, ids
 
 
@@ -1121,7 +1155,10 @@ class CacheRows:
         first = k[0]
         if first.ndim != 4 or first.stride(3) != 1 or first.stride(2) != first.shape[3]:
             raise ValueError(f"{op}: KV caches must be [B, n_kv, T, D] with contiguous (T, D).")
-        self.device = _one_device(op, *k, *v)
+        self.index = first.get_device()
+        if self.index < 0 or any(t.get_device() != self.index for t in k + v):
+            _device_error(op, *k, *v)
+        self.device = first.device
         self.code = dtype_code(first, op)
         for t in k + v:
             if t.shape != first.shape or t.stride() != first.stride():
@@ -1142,19 +1179,27 @@ def commit_tree(rows: CacheRows, seqlen, path, n_path, *, row_map=None) -> None:
     n_path[b]`` (``path`` / ``n_path`` as :func:`verify_tree` returns them).
     ``seqlen`` is not advanced."""
     op = "commit_tree"
-    dev = rows.device
-    B, N = _tree_shape(op, path, "path")
+    d = rows.index
+    if path.ndim != 2:
+        raise ValueError(f"{op}: path must be [B, N], got {tuple(path.shape)}.")
+    if (path.get_device() != d or seqlen.get_device() != d or n_path.get_device() != d or
+            (row_map is not None and row_map.get_device() != d)):
+        _device_error(op, path, seqlen, n_path, row_map, rows.k[0])
+    B, N = path.shape
+    if not 1 <= N <= MAX_TREE_NODES:
+        _bad_nodes(op, N)
     Bc, n_kv, T, D = rows.shape
-    for t in (seqlen, path, n_path, row_map):
-        if t is not None and t.device != dev:
-            raise (ValueError if t.is_cuda else RuntimeError)(f"{op}: caches on {dev}, {t.device} given.")
-    if path.ndim != 2 or seqlen.numel() != B or n_path.numel() != B or (row_map is not None and row_map.numel() != B):
-        raise ValueError(f"{op}: path must be [B, N]; seqlen, n_path and row_map need {B} entries.")
-    if row_map is None and Bc < B:
-        raise ValueError(f"{op}: {B} sequences in a cache of {Bc} rows.")
+    if seqlen.numel() != B or n_path.numel() != B:
+        raise ValueError(f"{op}: seqlen and n_path need {B} entries.")
+    if row_map is None:
+        if Bc < B:
+            raise ValueError(f"{op}: {B} sequences in a cache of {Bc} rows.")
+    elif row_map.numel() != B:
+        raise ValueError(f"{op}: row_map needs {B} entries.")
     if B == 0:
         return
     sl, pa, n = _as(seqlen, torch.int64), _as(path, torch.int32), _as(n_path, torch.int32)
     rm = _as(row_map, torch.int32) if row_map is not None else None
-    _launch(lib().maple_commit_tree, op, dev, rows.k_ptrs, rows.v_ptrs, len(rows.k), rows.code, B, N, Bc, n_kv,
-            rows.strides[0], rows.strides[1], T, D, ptr(sl), ptr(pa), ptr(n), ptr(rm), ptr(_err(dev)))
+    _launch(lib().maple_commit_tree, op, d, rows.k_ptrs, rows.v_ptrs, len(rows.k), rows.code, B, N, Bc, n_kv,
+            rows.strides[0], rows.strides[1], T, D, sl.data_ptr(), pa.data_ptr(), n.data_ptr(), ptr(rm),
+            _err(rows.device).data_ptr())

@@ -46,10 +46,11 @@ def test_tree_attention_refuses_before_any_launch(L):
     assert _attn(L, k=ctypes.c_void_p(264)) == 7
     assert _attn(L, sb=4 * 1024 * 128 + 4) == 7
     assert _attn(L, qsh=132) == 7
-    need = L.maple_tree_gqa_workspace_bytes(2, 8, 32, 4, 128, 1024, 0, 1)
+    need = L.maple_tree_gqa_workspace_bytes(2, 8, 32, 4, 128, 65536, 0, 1)
     assert need > 0
-    assert _attn(L, ws=None) == 6
-    assert _attn(L, nbytes=need - 1) == 6
+    assert _attn(L, T=65536, ws=None) == 6
+    assert _attn(L, T=65536, nbytes=need - 1) == 6
+    assert _attn(L, dtype=0, ws=None) == 6           # fp32: splits of its own
     assert L.maple_tree_gqa_workspace_bytes(2, 65, 32, 4, 128, 1024, 0, 1) == -1
     assert L.maple_tree_gqa_workspace_bytes(2, 8, 30, 4, 128, 1024, 0, 1) == -1
 
