@@ -2,6 +2,8 @@
 // attention of every node over the cache and its branch, and the move of the
 // accepted rows.  No counterpart in the reference, which decodes one token per
 // step (generate.py:168-373).
+#include <type_traits>
+
 #include "bulk.cuh"
 #include "launch.cuh"
 #include "tree.cuh"
@@ -63,83 +65,114 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, 
 
 // -------------------------------------------------- attention, CUDA cores --
 // fp32 caches, and heads of 256: one CTA per (split of the keys, KV head and
-// tile of 32 query rows, sequence).  Row r of a KV head is node r / G, query
-// head h G + r % G, so the whole tree reads each K/V row once per 32 rows.
-// Tiles of 32 keys stand in shared memory as fp32; a warp owns four rows: its
-// lanes are the tile's keys for the scores (one K row per lane, row pitch D + 4
-// floats: 16-byte reads without bank conflicts) and the head's dimensions for
-// the products with V.  Softmax online: running maximum, sum and output in
-// fp32 registers.  A key that a row does not see never meets its sums (the
-// weight carries the sign as a mark), so NaN or infinities there stay out.
-constexpr int kSimtRows = 32;
-constexpr int kSimtKeys = 32;
+// tile of 64 query rows, sequence).  Row r of a KV head is node r / G, query
+// head h G + r % G, so the whole tree reads each K/V row once per 64 rows.
+// Tiles of 64 keys stand in shared memory as fp32.  A thread holds 4 rows x 4
+// keys of the scores and 4 rows x D / 16 dims of the output (packed fp32 FMAs,
+// two per instruction; bound by their pipes; K at a pitch of D + 4 floats
+// free of bank conflicts), the weights pass through shared memory key by key.
+// Softmax online: running maximum, sum and output in fp32 registers.  In a tile
+// that some row sees only in part the weight of a key that a row does not see
+// is marked (-1) and its product left out, so NaN or infinities there stay out.
+constexpr int kSimtRows = 64;
+constexpr int kSimtKeys = 64;
+constexpr int kSimtPitch = kSimtRows + 4;
 
 template <int XT, int D>
-__global__ void __launch_bounds__(256) tree_simt_kernel(TreeAttnParams p, int row_tiles) {
-  constexpr int U = D / 32, PITCH = D + 4;
-  constexpr int es = XT == kBF16 ? 2 : 4, EPC = 16 / es;
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) tree_simt_kernel(TreeAttnParams p, int row_tiles) {
+  constexpr int PITCH = D + 4, CB = D / 64;  // blocks of 64 dims
+  constexpr int es = XT == kBF16 ? 2 : 4, EPC = 16 / es, CH = D / EPC;
   extern __shared__ __align__(16) float sm[];
-  float* sq = sm;                        // [32][D]
-  float* sk = sq + kSimtRows * D;        // [32][PITCH]
-  float* sv = sk + kSimtKeys * PITCH;    // [32][D]
+  float* sq = sm;                          // [64 rows][D]
+  float* sk = sq + kSimtRows * D;          // [64 keys][PITCH]
+  float* sv = sk + kSimtKeys * PITCH;      // [64 keys][D]
+  float* sp_w = sv + kSimtKeys * D;        // [64 keys][kSimtPitch] weights
   __shared__ unsigned long long s_mask[kTreeMaxNodes];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ unsigned s_used[2];
+  __shared__ int s_dmax;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int sp = blockIdx.x, h = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles, b = blockIdx.z;
   const float ninf = __int_as_float(0xff800000);
   pdl_wait();
   pdl_trigger();
   const int64_t len = p.seqlen[b];
   const int cb = p.row_map != nullptr ? p.row_map[b] : b;
-  if (tid < kTreeMaxNodes) {
+  const int rows = p.N * p.G, r0 = rt * kSimtRows;
+  // q rows, zero past the last one; all of a thread's loads in flight together
+  {
+    constexpr int QN = kSimtRows * CH / 256;
+    static_assert(QN * 256 == kSimtRows * CH, "whole rounds");
+    uint4 v[QN];
+    const uint64_t per_g = (1ull << 32) / (unsigned)p.G + 1;  // row / G by a multiplication, exact while row x G < 2^32
+#pragma unroll
+    for (int e = 0; e < QN; ++e) {
+      const int c = tid + 256 * e, gr = r0 + c / CH;
+      v[e] = make_uint4(0u, 0u, 0u, 0u);
+      if (gr < rows) {
+        const int i = (int)((uint64_t)(unsigned)gr * per_g >> 32), g = gr - i * p.G;
+        v[e] = ld_u4(static_cast<const char*>(p.q) +
+                     (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + g) * p.q_sh + c % CH * EPC) * es);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < QN; ++e) {
+      const int c = tid + 256 * e;
+      float f[EPC];
+      widen_u4<XT>(v[e], f);
+#pragma unroll
+      for (int u = 0; u < EPC; u += 4)
+        *reinterpret_cast<float4*>(&sq[c / CH * D + c % CH * EPC + u]) = make_float4(f[u], f[u + 1], f[u + 2], f[u + 3]);
+    }
+  }
+  if (tid < 32) {
     const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
-    s_mask[tid] = tid < p.N ? p.mask[(int64_t)b * p.N + tid] & keep : 0ull;
+    unsigned long long used = 0;
+    int dm = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = tid + 32 * u;
+      const unsigned long long m = i < p.N ? p.mask[(int64_t)b * p.N + i] & keep : 0ull;
+      s_mask[i] = m;
+      used |= m | (m ? 1ull << i : 0ull);
+      dm = max(dm, __popcll(m) - 1);
+    }
+    const unsigned lo = __reduce_or_sync(0xffffffffu, (unsigned)used);
+    const unsigned hi = __reduce_or_sync(0xffffffffu, (unsigned)(used >> 32));
+    dm = __reduce_max_sync(0xffffffffu, dm);
+    if (tid == 0) {
+      s_used[0] = lo;
+      s_used[1] = hi;
+      s_dmax = dm;
+    }
   }
   __syncthreads();
-  unsigned long long used = 0;
-  for (int i = 0; i < p.N; ++i) used |= s_mask[i] | (s_mask[i] ? 1ull << i : 0ull);
-  const TreeRange rg = tree_range(p, len, cb, used);
+  const TreeRange rg = tree_range(p, len, cb, ((unsigned long long)s_used[1] << 32) | s_used[0]);
   if (rg.bad && tid == 0) atomicOr(p.err, kErrFlagBounds);
   int k0, k1;
   tree_split(rg.lo, rg.hi, kSimtKeys, p.NS, sp, k0, k1);
   if (sp > 0 && k0 >= k1) return;  // nothing here; split 0 always answers
-
-  const int rows = p.N * p.G, r0 = rt * kSimtRows + warp * 4;
-  // q rows, zero past the last one
-  for (int c = tid; c < kSimtRows * D / EPC; c += 256) {
-    const int r = c / (D / EPC), cc = c % (D / EPC), gr = rt * kSimtRows + r;
-    float f[EPC];
-    if (gr < rows) {
-      const int i = gr / p.G, g = gr - i * p.G;
-      widen_u4<XT>(ld_u4(static_cast<const char*>(p.q) +
-                         (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + g) * p.q_sh + cc * EPC) * es), f);
-    } else {
-#pragma unroll
-      for (int e = 0; e < EPC; ++e) f[e] = 0.0f;
-    }
-#pragma unroll
-    for (int e = 0; e < EPC; ++e) sq[r * D + cc * EPC + e] = f[e];
-  }
   const char* kb = static_cast<const char*>(p.kc) + (rg.cb * p.c_sb + h * p.c_sh) * es;
   const char* vb = static_cast<const char*>(p.vc) + (rg.cb * p.c_sb + h * p.c_sh) * es;
 
   unsigned long long mine[4];
-  int depth[4];
-  float m[4], l[4], acc[4][U];
+  float m[4], l[4];
+  uint64_t acc[4][2 * CB];  // pairs of dims
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
-    const int r = r0 + a;
+    const int r = r0 + ty * 4 + a;
     mine[a] = r < rows ? s_mask[r / p.G] : 0ull;
-    depth[a] = __popcll(mine[a]) - 1;
     m[a] = ninf;
     l[a] = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) acc[a][u] = 0.0f;
+    for (int u = 0; u < 2 * CB; ++u) acc[a][u] = 0;
   }
   for (int t0 = k0; t0 < k1; t0 += kSimtKeys) {
     const int n = min(kSimtKeys, k1 - t0);
+    const bool mixed = t0 + kSimtKeys > min(rg.s, k1) || (p.window > 0 && t0 <= rg.s + s_dmax - p.window);
     __syncthreads();  // the last tile's readers are done
-    for (int c = tid; c < kSimtKeys * D / EPC; c += 256) {
-      const int r = c / (D / EPC), cc = c % (D / EPC);
+#pragma unroll 4
+    for (int c = tid; c < kSimtKeys * CH; c += 256) {
+      const int r = c / CH, cc = c % CH;
       float f[EPC], g[EPC];
       if (r < n) {
         widen_u4<XT>(ld_u4(kb + ((int64_t)(t0 + r) * D + cc * EPC) * es), f);
@@ -149,78 +182,123 @@ __global__ void __launch_bounds__(256) tree_simt_kernel(TreeAttnParams p, int ro
         for (int e = 0; e < EPC; ++e) f[e] = g[e] = 0.0f;
       }
 #pragma unroll
-      for (int e = 0; e < EPC; ++e) {
-        sk[r * PITCH + cc * EPC + e] = f[e];
-        sv[r * D + cc * EPC + e] = g[e];
+      for (int e = 0; e < EPC; e += 4) {
+        *reinterpret_cast<float4*>(&sk[r * PITCH + cc * EPC + e]) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        *reinterpret_cast<float4*>(&sv[r * D + cc * EPC + e]) = make_float4(g[e], g[e + 1], g[e + 2], g[e + 3]);
       }
     }
     __syncthreads();
-    // scores: this lane's key against the warp's four rows
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
+    // scores: rows 4 ty .., keys tx + 16 j
+    uint64_t s2[4][4] = {};  // sums over even and odd dims
+#pragma unroll 4
     for (int d = 0; d < D; d += 4) {
-      const float4 kk = *reinterpret_cast<const float4*>(&sk[lane * PITCH + d]);
+      ulonglong2 qq[4], kk[4];
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const float4 qq = *reinterpret_cast<const float4*>(&sq[(warp * 4 + a) * D + d]);
-        s[a] = fmaf(qq.x, kk.x, s[a]);
-        s[a] = fmaf(qq.y, kk.y, s[a]);
-        s[a] = fmaf(qq.z, kk.z, s[a]);
-        s[a] = fmaf(qq.w, kk.w, s[a]);
-      }
+      for (int a = 0; a < 4; ++a) qq[a] = *reinterpret_cast<const ulonglong2*>(&sq[(ty * 4 + a) * D + d]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kk[j] = *reinterpret_cast<const ulonglong2*>(&sk[(tx + 16 * j) * PITCH + d]);
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s2[a][j] = f2_fma(qq[a].y, kk[j].y, f2_fma(qq[a].x, kk[j].x, s2[a][j]));
     }
-    const int t = t0 + lane;
-    const int j = t - rg.s;  // node of this key, below 0: a cached position
-    const int kpos = j < 0 ? t : (j < kTreeMaxNodes ? rg.s + __popcll(s_mask[j]) - 1 : 0);
-    float w[4];
+    unsigned seen = 0xffffu;  // bit 4 a + j
+    if (mixed) {
+      seen = 0;
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      bool vis = lane < n && mine[a] != 0 && (j < 0 || ((mine[a] >> (j & 63)) & 1));
-      if (p.window > 0) vis = vis && kpos > rg.s + depth[a] - p.window;
-      const float x = vis ? s[a] * p.scale : ninf;
-      const float mt = fmaxf(m[a], warp_max(x));
-      const float base = mt == ninf ? 0.0f : mt;
-      w[a] = vis ? mexp(x - base) : 0.0f;
-      const float fix = mexp(m[a] - base);
-      l[a] = fmaf(l[a], fix, warp_butterfly_sum(w[a]));
-      m[a] = mt;
+      for (int j = 0; j < 4; ++j) {
+        const int t = t0 + tx + 16 * j, x = t - rg.s;  // node of this key, below 0: a cached position
+        const int kpos = x < 0 ? t : x < kTreeMaxNodes ? rg.s + __popcll(s_mask[x]) - 1 : 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) acc[a][u] *= fix;
-      if (!vis) w[a] = -1.0f;  // mark: not this row's
-    }
-    for (int kx = 0; kx < n; ++kx) {
-      float vv[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) vv[u] = sv[kx * D + lane + 32 * u];
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const float wk = __shfl_sync(0xffffffffu, w[a], kx);
-        if (!(wk < 0.0f)) {
-#pragma unroll
-          for (int u = 0; u < U; ++u) acc[a][u] = fmaf(wk, vv[u], acc[a][u]);
+        for (int a = 0; a < 4; ++a) {
+          bool vis = tx + 16 * j < n && mine[a] != 0 && (x < 0 || ((mine[a] >> (x & 63)) & 1));
+          if (p.window > 0) vis = vis && kpos > rg.s + __popcll(mine[a]) - 1 - p.window;
+          seen |= (vis ? 1u : 0u) << (4 * a + j);
         }
       }
     }
+    float w[4][4];  // [key][row]
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      float x[4], mt = m[a];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float even, odd;
+        f2_get(s2[a][j], even, odd);
+        x[j] = (seen >> (4 * a + j)) & 1u ? (even + odd) * p.scale : ninf;
+        mt = fmaxf(mt, x[j]);
+      }
+#pragma unroll
+      for (int o = 8; o >= 1; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+      const float base = mt == ninf ? 0.0f : mt;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool vis = (seen >> (4 * a + j)) & 1u;
+        const float e = vis ? mexp(x[j] - base) : 0.0f;
+        sum += e;
+        w[j][a] = vis ? e : -1.0f;  // the mark: not this row's
+      }
+#pragma unroll
+      for (int o = 8; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float fix = mt == m[a] ? 1.0f : mexp(m[a] - base);
+      l[a] = fmaf(l[a], fix, sum);
+      m[a] = mt;
+      const uint64_t fix2 = f2(fix, fix);
+#pragma unroll
+      for (int u = 0; u < 2 * CB; ++u) acc[a][u] = f2_fma(acc[a][u], fix2, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<float4*>(&sp_w[(tx + 16 * j) * kSimtPitch + ty * 4]) = make_float4(w[j][0], w[j][1], w[j][2], w[j][3]);
+    __syncwarp();  // a row's weights come from the 16 threads of its own half-warp
+    auto product = [&](auto marks) {
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const float4 pw = *reinterpret_cast<const float4*>(&sp_w[k * kSimtPitch + ty * 4]);
+        const float pr[4] = {pw.x, pw.y, pw.z, pw.w};
+        const uint64_t p2[4] = {f2(pw.x, pw.x), f2(pw.y, pw.y), f2(pw.z, pw.z), f2(pw.w, pw.w)};
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+          const ulonglong2 vv = *reinterpret_cast<const ulonglong2*>(&sv[k * D + 64 * c + tx * 4]);
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            const uint64_t y0 = f2_fma(p2[a], vv.x, acc[a][2 * c]), y1 = f2_fma(p2[a], vv.y, acc[a][2 * c + 1]);
+            const bool out = decltype(marks)::value && pr[a] < 0.0f;
+            acc[a][2 * c] = out ? acc[a][2 * c] : y0;
+            acc[a][2 * c + 1] = out ? acc[a][2 * c + 1] : y1;
+          }
+        }
+      }
+    };
+    if (mixed) product(std::true_type{});
+    else product(std::false_type{});
   }
   const bool alone = tree_splits_used(rg.lo, rg.hi, kSimtKeys, p.NS) <= 1;
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
-    const int r = r0 + a;
+    const int r = r0 + ty * 4 + a;
     if (r >= rows) continue;
-    if (alone) {
-      const int i = r / p.G, g = r - i * p.G;
-      const int64_t o = (((int64_t)b * p.N + i) * p.H + h * p.G + g) * D;
+    const int i = r / p.G, g = r - i * p.G;
+    const int64_t o = (((int64_t)b * p.N + i) * p.H + h * p.G + g) * D, R = ((int64_t)b * p.Hkv + h) * rows + r;
+    if (mine[a] == 0) m[a] = ninf;  // padding, whatever it met in tiles that the others see whole
+    const float inv = m[a] == ninf ? 0.0f : 1.0f / l[a];
 #pragma unroll
-      for (int u = 0; u < U; ++u) store_f<XT>(p.out, o + lane + 32 * u, l[a] == 0.0f ? 0.0f : acc[a][u] / l[a]);
-    } else {
-      const int64_t R = ((int64_t)b * p.Hkv + h) * rows + r;
-      float* ac = p.ws_acc + (R * p.NS + sp) * D;
+    for (int c = 0; c < CB; ++c) {
+      float x[4];
+      f2_get(acc[a][2 * c], x[0], x[1]);
+      f2_get(acc[a][2 * c + 1], x[2], x[3]);
+      const int d = 64 * c + tx * 4;
+      if (!alone) {
+        *reinterpret_cast<float4*>(p.ws_acc + (R * p.NS + sp) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+      } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) ac[lane + 32 * u] = acc[a][u];
-      if (lane == 0) {
-        p.ws_ml[(R * p.NS + sp) * 2] = m[a];
-        p.ws_ml[(R * p.NS + sp) * 2 + 1] = l[a];
+        for (int e = 0; e < 4; ++e) store_f<XT>(p.out, o + d + e, m[a] == ninf ? 0.0f : x[e] * inv);
       }
+    }
+    if (!alone && tx == 0) {
+      p.ws_ml[(R * p.NS + sp) * 2] = m[a];
+      p.ws_ml[(R * p.NS + sp) * 2 + 1] = m[a] == ninf ? 0.0f : l[a];
     }
   }
 }
@@ -352,10 +430,10 @@ __global__ void __launch_bounds__(256) commit_kernel(const __grid_constant__ Com
   }
 }
 
-// How many splits a row's keys are cut into: enough CTAs for two per SM at
-// full length, no more than the join can hold.
+// How many splits a row's keys are cut into: as many as the 296 resident CTAs
+// (two per SM) take at once, no more than the join can hold.
 inline int tree_simt_splits(int64_t ctas, int64_t max_len) {
-  const int64_t want = (2 * 148 + ctas - 1) / ctas, most = (max_len + kSimtKeys - 1) / kSimtKeys;
+  const int64_t want = 2 * 148 / ctas, most = (max_len + kSimtKeys - 1) / kSimtKeys;
   const int64_t ns = want < most ? want : most;
   return (int)(ns < 1 ? 1 : ns > kTreeMaxSplits ? kTreeMaxSplits : ns);
 }
@@ -447,7 +525,7 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   cudaError_t e = cudaSuccess;
 #define MB_TREE(XT, DD)                                                                                              \
   do {                                                                                                               \
-    const size_t smem = (size_t)(kSimtRows * DD + kSimtKeys * (DD + 4) + kSimtKeys * DD) * 4;                        \
+    const size_t smem = (size_t)(kSimtRows * DD + kSimtKeys * (DD + 4) + kSimtKeys * DD + kSimtKeys * kSimtPitch) * 4; \
     static std::atomic<uint64_t> done{0};                                                                            \
     e = smem_once(done, tree_simt_kernel<XT, DD>, (int)smem);                                                        \
     if (e == cudaSuccess)                                                                                            \
