@@ -63,74 +63,98 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, 
   if (wrong) atomicOr(err, kErrFlagBounds);
 }
 
-// -------------------------------------------------- attention, CUDA cores --
-// fp32 caches, and heads of 256: one CTA per (split of the keys, KV head and
-// tile of 64 query rows, sequence).  Row r of a KV head is node r / G, query
-// head h G + r % G, so the whole tree reads each K/V row once per 64 rows.
-// Tiles of 64 keys stand in shared memory as fp32.  A thread holds 4 rows x 4
-// keys of the scores and 4 rows x D / 16 dims of the output (packed fp32 FMAs,
-// two per instruction; bound by their pipes; K at a pitch of D + 4 floats
-// free of bank conflicts), the weights pass through shared memory key by key.
-// Softmax online: running maximum, sum and output in fp32 registers.  In a tile
-// that some row sees only in part the weight of a key that a row does not see
-// is marked (-1) and its product left out, so NaN or infinities there stay out.
-constexpr int kSimtRows = 64;
-constexpr int kSimtKeys = 64;
-constexpr int kSimtPitch = kSimtRows + 4;
+// ------------------------------------- attention, fp32 and heads of 256 --
+// One CTA per (split of the keys, KV head and tile of 64 query rows, sequence).
+// Row r of a KV head is node r / G, query head h G + r % G; a warp has 16 rows.
+// Products on the tensor pipe as tf32 (mma.sync m16n8k8), each fp32 operand x
+// split into hi = x with its low 13 bits cleared and lo = x - hi (exact):
+// lo hi + hi lo + hi hi leaves out lo lo, 2^-22 of the product, so an fp32
+// result keeps its precision; bf16 values are their own hi, which saves two of
+// the three for the scores and one for the output.  Tiles of 32 keys stand in
+// shared memory as fp32 in two stages (cp.async under the tile before); a pitch
+// of D + 4 floats keeps ldmatrix (K, Q) and the V reads free of bank conflicts.
+// The weights stay in registers: key 2t of a block of eight takes the place of
+// the product's index t and key 2t + 1 that of t + 4, which is how the scores'
+// accumulators lie, and V's rows are read in that order.
+// Infinities do not survive the split (0 x inf), and a masked weight of 0 does
+// not keep NaN out: K and V are cleared of both as they arrive.  A score with a
+// cleared key is computed again from the cache (each such key by its threads);
+// cleared values of V are added at the end for the rows that see them.
+// Before, on the fp32 pipes: 33 us for 4 x 1500 with heads of 64, 17 nodes.
+constexpr int kMmaRows = 64;
+constexpr int kMmaKeys = 32;
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four 8 x 4 blocks of fp32, a lane's 32 bits as the tf32 fragments want them.
+__device__ __forceinline__ void ldsm4(const float* p, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(p)));
+}
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
+  hi = x & 0xffffe000u;
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+}
+__device__ __forceinline__ bool odd_f32(uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u; }  // NaN, infinity
 
 template <int XT, int D>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) tree_simt_kernel(TreeAttnParams p, int row_tiles) {
-  constexpr int PITCH = D + 4, CB = D / 64;  // blocks of 64 dims
-  constexpr int es = XT == kBF16 ? 2 : 4, EPC = 16 / es, CH = D / EPC;
+__global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row_tiles) {
+  constexpr int PITCH = D + 4, es = XT == kBF16 ? 2 : 4, EPC = 16 / es, CH = D / EPC;
+  constexpr int STAGE = 2 * kMmaKeys * PITCH;             // floats: K, then V
+  constexpr int PER = kMmaKeys * CH / 128;                // 16-byte chunks of K (and of V) per thread
   extern __shared__ __align__(16) float sm[];
-  float* sq = sm;                          // [64 rows][D]
-  float* sk = sq + kSimtRows * D;          // [64 keys][PITCH]
-  float* sv = sk + kSimtKeys * PITCH;      // [64 keys][D]
-  float* sp_w = sv + kSimtKeys * D;        // [64 keys][kSimtPitch] weights
+  float* sq = sm;                                         // [64][PITCH]
+  float* ring = sq + kMmaRows * PITCH;                    // [2][STAGE]
   __shared__ unsigned long long s_mask[kTreeMaxNodes];
   __shared__ unsigned s_used[2];
-  __shared__ int s_dmax;
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  __shared__ int s_dmax, s_fix;
+  __shared__ unsigned s_odd[2];                           // per stage: keys that were cleared
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int sp = blockIdx.x, h = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles, b = blockIdx.z;
   const float ninf = __int_as_float(0xff800000);
   pdl_wait();
   pdl_trigger();
   const int64_t len = p.seqlen[b];
   const int cb = p.row_map != nullptr ? p.row_map[b] : b;
-  const int rows = p.N * p.G, r0 = rt * kSimtRows;
-  // q rows, zero past the last one; all of a thread's loads in flight together
-  {
-    constexpr int QN = kSimtRows * CH / 256;
-    static_assert(QN * 256 == kSimtRows * CH, "whole rounds");
-    uint4 v[QN];
-    const uint64_t per_g = (1ull << 32) / (unsigned)p.G + 1;  // row / G by a multiplication, exact while row x G < 2^32
+  const int rows = p.N * p.G, r0 = rt * kMmaRows;
+  const uint64_t per_g = (1ull << 32) / (unsigned)p.G + 1;  // row / G by a multiplication, exact while row x G < 2^32
+  // q rows, zero past the last one; a thread's loads in flight together
+#pragma unroll 1
+  for (int e0 = 0; e0 < kMmaRows * CH / 128; e0 += 8) {
+    uint4 v[8];
 #pragma unroll
-    for (int e = 0; e < QN; ++e) {
-      const int c = tid + 256 * e, gr = r0 + c / CH;
+    for (int e = 0; e < 8; ++e) {
+      const int c = tid + 128 * (e0 + e), gr = r0 + c / CH;
       v[e] = make_uint4(0u, 0u, 0u, 0u);
       if (gr < rows) {
-        const int i = (int)((uint64_t)(unsigned)gr * per_g >> 32), g = gr - i * p.G;
+        const int i = (int)((uint64_t)(unsigned)gr * per_g >> 32), qg = gr - i * p.G;
         v[e] = ld_u4(static_cast<const char*>(p.q) +
-                     (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + g) * p.q_sh + c % CH * EPC) * es);
+                     (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + qg) * p.q_sh + c % CH * EPC) * es);
       }
     }
 #pragma unroll
-    for (int e = 0; e < QN; ++e) {
-      const int c = tid + 256 * e;
+    for (int e = 0; e < 8; ++e) {
+      const int c = tid + 128 * (e0 + e);
       float f[EPC];
       widen_u4<XT>(v[e], f);
 #pragma unroll
       for (int u = 0; u < EPC; u += 4)
-        *reinterpret_cast<float4*>(&sq[c / CH * D + c % CH * EPC + u]) = make_float4(f[u], f[u + 1], f[u + 2], f[u + 3]);
+        *reinterpret_cast<float4*>(&sq[c / CH * PITCH + c % CH * EPC + u]) = make_float4(f[u], f[u + 1], f[u + 2], f[u + 3]);
     }
   }
-  if (tid < 32) {
+  if (warp == 0) {
     const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
     unsigned long long used = 0;
     int dm = 0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int i = tid + 32 * u;
+      const int i = lane + 32 * u;
       const unsigned long long m = i < p.N ? p.mask[(int64_t)b * p.N + i] & keep : 0ull;
       s_mask[i] = m;
       used |= m | (m ? 1ull << i : 0ull);
@@ -139,164 +163,252 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) tree_simt_kernel(TreeAt
     const unsigned lo = __reduce_or_sync(0xffffffffu, (unsigned)used);
     const unsigned hi = __reduce_or_sync(0xffffffffu, (unsigned)(used >> 32));
     dm = __reduce_max_sync(0xffffffffu, dm);
-    if (tid == 0) {
+    if (lane == 0) {
       s_used[0] = lo;
       s_used[1] = hi;
       s_dmax = dm;
+      s_fix = 0;
+      s_odd[0] = s_odd[1] = 0;
     }
   }
   __syncthreads();
   const TreeRange rg = tree_range(p, len, cb, ((unsigned long long)s_used[1] << 32) | s_used[0]);
   if (rg.bad && tid == 0) atomicOr(p.err, kErrFlagBounds);
   int k0, k1;
-  tree_split(rg.lo, rg.hi, kSimtKeys, p.NS, sp, k0, k1);
+  tree_split(rg.lo, rg.hi, kMmaKeys, p.NS, sp, k0, k1);
   if (sp > 0 && k0 >= k1) return;  // nothing here; split 0 always answers
   const char* kb = static_cast<const char*>(p.kc) + (rg.cb * p.c_sb + h * p.c_sh) * es;
   const char* vb = static_cast<const char*>(p.vc) + (rg.cb * p.c_sb + h * p.c_sh) * es;
 
-  unsigned long long mine[4];
-  float m[4], l[4];
-  uint64_t acc[4][2 * CB];  // pairs of dims
+  // this thread's chunks of a tile (rows past the split's end as zeros)
+  auto load = [&](int t0, int stage) {
+    float* st = ring + stage * STAGE;
 #pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    const int r = r0 + ty * 4 + a;
-    mine[a] = r < rows ? s_mask[r / p.G] : 0ull;
-    m[a] = ninf;
-    l[a] = 0.0f;
+    for (int e = 0; e < PER; ++e) {
+      const int c = tid + 128 * e, r = c / CH, cc = c % CH * EPC;
+      const int64_t at = ((int64_t)(t0 + r) * D + cc) * es;
 #pragma unroll
-    for (int u = 0; u < 2 * CB; ++u) acc[a][u] = 0;
-  }
-  for (int t0 = k0; t0 < k1; t0 += kSimtKeys) {
-    const int n = min(kSimtKeys, k1 - t0);
-    const bool mixed = t0 + kSimtKeys > min(rg.s, k1) || (p.window > 0 && t0 <= rg.s + s_dmax - p.window);
-    __syncthreads();  // the last tile's readers are done
-#pragma unroll 4
-    for (int c = tid; c < kSimtKeys * CH; c += 256) {
-      const int r = c / CH, cc = c % CH;
-      float f[EPC], g[EPC];
-      if (r < n) {
-        widen_u4<XT>(ld_u4(kb + ((int64_t)(t0 + r) * D + cc * EPC) * es), f);
-        widen_u4<XT>(ld_u4(vb + ((int64_t)(t0 + r) * D + cc * EPC) * es), g);
-      } else {
-#pragma unroll
-        for (int e = 0; e < EPC; ++e) f[e] = g[e] = 0.0f;
-      }
-#pragma unroll
-      for (int e = 0; e < EPC; e += 4) {
-        *reinterpret_cast<float4*>(&sk[r * PITCH + cc * EPC + e]) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-        *reinterpret_cast<float4*>(&sv[r * D + cc * EPC + e]) = make_float4(g[e], g[e + 1], g[e + 2], g[e + 3]);
-      }
-    }
-    __syncthreads();
-    // scores: rows 4 ty .., keys tx + 16 j
-    uint64_t s2[4][4] = {};  // sums over even and odd dims
-#pragma unroll 4
-    for (int d = 0; d < D; d += 4) {
-      ulonglong2 qq[4], kk[4];
-#pragma unroll
-      for (int a = 0; a < 4; ++a) qq[a] = *reinterpret_cast<const ulonglong2*>(&sq[(ty * 4 + a) * D + d]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) kk[j] = *reinterpret_cast<const ulonglong2*>(&sk[(tx + 16 * j) * PITCH + d]);
-#pragma unroll
-      for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s2[a][j] = f2_fma(qq[a].y, kk[j].y, f2_fma(qq[a].x, kk[j].x, s2[a][j]));
-    }
-    unsigned seen = 0xffffu;  // bit 4 a + j
-    if (mixed) {
-      seen = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = t0 + tx + 16 * j, x = t - rg.s;  // node of this key, below 0: a cached position
-        const int kpos = x < 0 ? t : x < kTreeMaxNodes ? rg.s + __popcll(s_mask[x]) - 1 : 0;
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          bool vis = tx + 16 * j < n && mine[a] != 0 && (x < 0 || ((mine[a] >> (x & 63)) & 1));
-          if (p.window > 0) vis = vis && kpos > rg.s + __popcll(mine[a]) - 1 - p.window;
-          seen |= (vis ? 1u : 0u) << (4 * a + j);
+      for (int kv = 0; kv < 2; ++kv) {
+        float* dst = st + kv * kMmaKeys * PITCH + r * PITCH + cc;
+        const char* src = (kv ? vb : kb) + at;
+        if constexpr (XT == kF32) {
+          if (t0 + r < k1) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+          else *reinterpret_cast<float4*>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+          float f[8];
+          widen_u4<kBF16>(t0 + r < k1 ? ld_u4(src) : make_uint4(0u, 0u, 0u, 0u), f);
+          *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+          *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
         }
       }
     }
-    float w[4][4];  // [key][row]
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  };
+  // clears this thread's chunks of NaN and infinities
+  auto clear = [&](int stage) {
+    float* st = ring + stage * STAGE;
+    uint32_t any = 0;
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      float x[4], mt = m[a];
+    for (int e = 0; e < 2 * PER; ++e) {
+      const int c = tid + 128 * (e >> 1), r = c / CH, cc = c % CH * EPC;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float even, odd;
-        f2_get(s2[a][j], even, odd);
-        x[j] = (seen >> (4 * a + j)) & 1u ? (even + odd) * p.scale : ninf;
-        mt = fmaxf(mt, x[j]);
+      for (int u = 0; u < EPC; u += 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(st + (e & 1) * kMmaKeys * PITCH + r * PITCH + cc + u);
+        any |= odd_f32(x.x) | odd_f32(x.y) | odd_f32(x.z) | odd_f32(x.w);
       }
-#pragma unroll
-      for (int o = 8; o >= 1; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-      const float base = mt == ninf ? 0.0f : mt;
-      float sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool vis = (seen >> (4 * a + j)) & 1u;
-        const float e = vis ? mexp(x[j] - base) : 0.0f;
-        sum += e;
-        w[j][a] = vis ? e : -1.0f;  // the mark: not this row's
-      }
-#pragma unroll
-      for (int o = 8; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float fix = mt == m[a] ? 1.0f : mexp(m[a] - base);
-      l[a] = fmaf(l[a], fix, sum);
-      m[a] = mt;
-      const uint64_t fix2 = f2(fix, fix);
-#pragma unroll
-      for (int u = 0; u < 2 * CB; ++u) acc[a][u] = f2_fma(acc[a][u], fix2, 0);
     }
+    if (!any) return;
+#pragma unroll 1
+    for (int e = 0; e < 2 * PER; ++e) {  // rare
+      const int c = tid + 128 * (e >> 1), r = c / CH, cc = c % CH * EPC;
+      for (int u = 0; u < EPC; ++u) {
+        uint32_t* x = reinterpret_cast<uint32_t*>(st + (e & 1) * kMmaKeys * PITCH + r * PITCH + cc + u);
+        if (!odd_f32(*x)) continue;
+        *x = 0u;
+        if (e & 1) s_fix = 1;
+        else atomicOr(&s_odd[stage], 1u << r);
+      }
+    }
+  };
+
+  // rows g and g + 8 of the warp's 16
+  unsigned long long mine[2];
+  float m[2] = {ninf, ninf}, l[2] = {0.0f, 0.0f}, acc[D / 8][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<float4*>(&sp_w[(tx + 16 * j) * kSimtPitch + ty * 4]) = make_float4(w[j][0], w[j][1], w[j][2], w[j][3]);
-    __syncwarp();  // a row's weights come from the 16 threads of its own half-warp
-    auto product = [&](auto marks) {
+  for (int a = 0; a < 2; ++a) {
+    const int r = r0 + warp * 16 + g + 8 * a;
+    mine[a] = r < rows ? s_mask[(int)((uint64_t)(unsigned)r * per_g >> 32)] : 0ull;
+  }
+#pragma unroll
+  for (int j = 0; j < D / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+  auto sees = [&](int a, int key) {  // whether row a sees slot `key` of this split
+    const int x = key - rg.s;        // its node, below 0: a cached position
+    bool vis = key < k1 && mine[a] != 0 && (x < 0 || ((mine[a] >> (x & 63)) & 1));
+    if (p.window > 0) {
+      const int kpos = x < 0 ? key : x < kTreeMaxNodes ? rg.s + __popcll(s_mask[x]) - 1 : 0;
+      vis = vis && kpos > rg.s + __popcll(mine[a]) - 1 - p.window;
+    }
+    return vis;
+  };
+  auto is_mixed = [&](int t0) {
+    return t0 + kMmaKeys > min(rg.s, k1) || (p.window > 0 && t0 <= rg.s + s_dmax - p.window);
+  };
+  const bool idle = r0 + warp * 16 >= rows;  // a warp without rows only loads
+  const float* a_at = sq + (warp * 16 + (lane & 7) + (lane >> 3 & 1) * 8) * PITCH + (lane >> 4) * 4;
+  if (k0 < k1) load(k0, 0);
+  int stage = 0;
+  for (int t0 = k0; t0 < k1; t0 += kMmaKeys, stage ^= 1) {
+    if (t0 + kMmaKeys < k1) load(t0 + kMmaKeys, stage ^ 1);
+    else asm volatile("cp.async.commit_group;\n" ::: "memory");
+    asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+    clear(stage);
+    __syncthreads();
+    const float* sk = ring + stage * STAGE;
+    const float* sv = sk + kMmaKeys * PITCH;
+    if (!idle) {
+      float s[4][4] = {};  // 16 rows x 32 keys: block j, keys 8 j + 2 t, + 1 of rows g (0, 1) and g + 8 (2, 3)
+      const float* b_at = sk + ((lane & 7) + (lane >> 4) * 8) * PITCH + (lane >> 3 & 1) * 4;
 #pragma unroll 4
-      for (int k = 0; k < n; ++k) {
-        const float4 pw = *reinterpret_cast<const float4*>(&sp_w[k * kSimtPitch + ty * 4]);
-        const float pr[4] = {pw.x, pw.y, pw.z, pw.w};
-        const uint64_t p2[4] = {f2(pw.x, pw.x), f2(pw.y, pw.y), f2(pw.z, pw.z), f2(pw.w, pw.w)};
+      for (int kk = 0; kk < D / 8; ++kk) {
+        uint32_t a[4], ah[4], al[4];
+        ldsm4(a_at + 8 * kk, a);
 #pragma unroll
-        for (int c = 0; c < CB; ++c) {
-          const ulonglong2 vv = *reinterpret_cast<const ulonglong2*>(&sv[k * D + 64 * c + tx * 4]);
+        for (int i = 0; i < 4; ++i) split_tf32(a[i], ah[i], al[i]);
 #pragma unroll
-          for (int a = 0; a < 4; ++a) {
-            const uint64_t y0 = f2_fma(p2[a], vv.x, acc[a][2 * c]), y1 = f2_fma(p2[a], vv.y, acc[a][2 * c + 1]);
-            const bool out = decltype(marks)::value && pr[a] < 0.0f;
-            acc[a][2 * c] = out ? acc[a][2 * c] : y0;
-            acc[a][2 * c + 1] = out ? acc[a][2 * c + 1] : y1;
+        for (int j = 0; j < 4; j += 2) {
+          uint32_t y[4];
+          ldsm4(b_at + 8 * j * PITCH + 8 * kk, y);
+          if constexpr (XT == kBF16) {
+            mma_tf32(s[j], a, y[0], y[1]);
+            mma_tf32(s[j + 1], a, y[2], y[3]);
+          } else {
+            uint32_t yh[4], yl[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) split_tf32(y[i], yh[i], yl[i]);
+            mma_tf32(s[j], al, yh[0], yh[1]);
+            mma_tf32(s[j + 1], al, yh[2], yh[3]);
+            mma_tf32(s[j], ah, yl[0], yl[1]);
+            mma_tf32(s[j + 1], ah, yl[2], yl[3]);
+            mma_tf32(s[j], ah, yh[0], yh[1]);
+            mma_tf32(s[j + 1], ah, yh[2], yh[3]);
           }
         }
       }
-    };
-    if (mixed) product(std::true_type{});
-    else product(std::false_type{});
-  }
-  const bool alone = tree_splits_used(rg.lo, rg.hi, kSimtKeys, p.NS) <= 1;
+      if (const unsigned odd = s_odd[stage]; odd) {  // rare: keys with a NaN or an infinity, from the cache
 #pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    const int r = r0 + ty * 4 + a;
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int key = 8 * j + 2 * t + (c & 1);
+            if (!((odd >> key) & 1u)) continue;
+            float x = 0.0f;
+            const float* qr = sq + (warp * 16 + g + (c >> 1) * 8) * PITCH;
+#pragma unroll 1
+            for (int d = 0; d < D; ++d) x = fmaf(qr[d], load_f<XT>(kb, (int64_t)(t0 + key) * D + d), x);
+            s[j][c] = x;
+          }
+      }
+      const bool mixed = is_mixed(t0);
+      float fix[2];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        float mt = m[a];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float& x = s[j][2 * a + c];
+            x = mixed && !sees(a, t0 + 8 * j + 2 * t + c) ? ninf : x * p.scale;
+            mt = fmaxf(mt, x);
+          }
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+        const float base = mt == ninf ? 0.0f : mt;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float& x = s[j][2 * a + c];
+            x = x == ninf ? 0.0f : mexp(x - base);
+            sum += x;
+          }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        fix[a] = mt == m[a] ? 1.0f : mexp(m[a] - base);
+        l[a] = fmaf(l[a], fix[a], sum);
+        m[a] = mt;
+      }
+      if (__any_sync(0xffffffffu, fix[0] != 1.0f || fix[1] != 1.0f)) {
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[j][c] *= fix[c >> 1];
+      }
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        const uint32_t a[4] = {__float_as_uint(s[kk][0]), __float_as_uint(s[kk][2]), __float_as_uint(s[kk][1]),
+                               __float_as_uint(s[kk][3])};
+        uint32_t ah[4], al[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split_tf32(a[i], ah[i], al[i]);
+        const float* v_at = sv + (8 * kk + 2 * t) * PITCH + g;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          const uint32_t y0 = __float_as_uint(v_at[8 * j]), y1 = __float_as_uint(v_at[PITCH + 8 * j]);
+          if constexpr (XT == kBF16) {
+            mma_tf32(acc[j], al, y0, y1);
+            mma_tf32(acc[j], ah, y0, y1);
+          } else {
+            uint32_t h0, l0, h1, l1;
+            split_tf32(y0, h0, l0);
+            split_tf32(y1, h1, l1);
+            mma_tf32(acc[j], al, h0, h1);
+            mma_tf32(acc[j], ah, l0, l1);
+            mma_tf32(acc[j], ah, h0, h1);
+          }
+        }
+      }
+    }
+    __syncthreads();  // the stage may be written again
+    if (tid == 0) s_odd[stage] = 0;
+  }
+  if (s_fix && !idle) {  // rare: what was cleared from V, to the rows that see it
+    for (int key = k0; key < k1; ++key) {
+      const bool v0 = sees(0, key), v1 = sees(1, key);
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float y = load_f<XT>(vb, (int64_t)key * D + 8 * j + 2 * t + c);
+          if (odd_f32(__float_as_uint(y))) {
+            if (v0) acc[j][c] += y;
+            if (v1) acc[j][2 + c] += y;
+          }
+        }
+    }
+  }
+  const bool alone = tree_splits_used(rg.lo, rg.hi, kMmaKeys, p.NS) <= 1;
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    const int r = r0 + warp * 16 + g + 8 * a;
     if (r >= rows) continue;
-    const int i = r / p.G, g = r - i * p.G;
-    const int64_t o = (((int64_t)b * p.N + i) * p.H + h * p.G + g) * D, R = ((int64_t)b * p.Hkv + h) * rows + r;
+    const int i = (int)((uint64_t)(unsigned)r * per_g >> 32), qg = r - i * p.G;
+    const int64_t o = (((int64_t)b * p.N + i) * p.H + h * p.G + qg) * D, R = ((int64_t)b * p.Hkv + h) * rows + r;
     if (mine[a] == 0) m[a] = ninf;  // padding, whatever it met in tiles that the others see whole
     const float inv = m[a] == ninf ? 0.0f : 1.0f / l[a];
 #pragma unroll
-    for (int c = 0; c < CB; ++c) {
-      float x[4];
-      f2_get(acc[a][2 * c], x[0], x[1]);
-      f2_get(acc[a][2 * c + 1], x[2], x[3]);
-      const int d = 64 * c + tx * 4;
+    for (int j = 0; j < D / 8; ++j) {
+      const float x0 = acc[j][2 * a], x1 = acc[j][2 * a + 1];
+      const int d = 8 * j + 2 * t;
       if (!alone) {
-        *reinterpret_cast<float4*>(p.ws_acc + (R * p.NS + sp) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float2*>(p.ws_acc + (R * p.NS + sp) * D + d) = make_float2(x0, x1);
       } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) store_f<XT>(p.out, o + d + e, m[a] == ninf ? 0.0f : x[e] * inv);
+        store_f<XT>(p.out, o + d, m[a] == ninf ? 0.0f : x0 * inv);
+        store_f<XT>(p.out, o + d + 1, m[a] == ninf ? 0.0f : x1 * inv);
       }
     }
-    if (!alone && tx == 0) {
+    if (!alone && t == 0) {
       p.ws_ml[(R * p.NS + sp) * 2] = m[a];
       p.ws_ml[(R * p.NS + sp) * 2 + 1] = m[a] == ninf ? 0.0f : l[a];
     }
@@ -430,10 +542,10 @@ __global__ void __launch_bounds__(256) commit_kernel(const __grid_constant__ Com
   }
 }
 
-// How many splits a row's keys are cut into: as many as the 296 resident CTAs
-// (two per SM) take at once, no more than the join can hold.
-inline int tree_simt_splits(int64_t ctas, int64_t max_len) {
-  const int64_t want = 2 * 148 / ctas, most = (max_len + kSimtKeys - 1) / kSimtKeys;
+// How many splits a row's keys are cut into: as many as the resident CTAs
+// (three, two or one per SM) take at once, no more than the join can hold.
+inline int tree_mma_splits(int64_t ctas, int64_t max_len, int64_t head_dim) {
+  const int64_t want = (head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1) * 148 / ctas, most = (max_len + kMmaKeys - 1) / kMmaKeys;
   const int64_t ns = want < most ? want : most;
   return (int)(ns < 1 ? 1 : ns > kTreeMaxSplits ? kTreeMaxSplits : ns);
 }
@@ -447,8 +559,8 @@ inline int tree_splits(int64_t batch, int64_t nodes, int64_t num_heads, int64_t 
   if (window > 0 && window + nodes < max_len) max_len = window + nodes;  // no row's keys span more
   if (tree_use_tc(x_dtype, head_dim))
     return tree_tc_splits(batch * num_kv_heads * tree_tc_groups(nodes * (num_heads / num_kv_heads)), max_len);
-  const int64_t tiles = (nodes * (num_heads / num_kv_heads) + kSimtRows - 1) / kSimtRows;
-  return tree_simt_splits(batch * num_kv_heads * tiles, max_len);
+  const int64_t tiles = (nodes * (num_heads / num_kv_heads) + kMmaRows - 1) / kMmaRows;
+  return tree_mma_splits(batch * num_kv_heads * tiles, max_len, head_dim);
 }
 
 // Rows of partials per split and KV head, and the bytes of all of them.
@@ -513,7 +625,7 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   p.G = (int)(num_heads / num_kv_heads); p.Bc = (int)cache_batch; p.T = (int)max_len;
   p.window = (int)(window > max_len ? 0 : window);  // a window past the cache hides nothing
   p.scale = scale;
-  const int64_t rows = (int64_t)p.N * p.G, tiles = (rows + kSimtRows - 1) / kSimtRows;
+  const int64_t rows = (int64_t)p.N * p.G, tiles = (rows + kMmaRows - 1) / kMmaRows;
   if (num_kv_heads * tiles > 65535) return kErrShape;
   p.NS = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim, window);
   const int64_t prows = tree_partial_rows(rows, x_dtype, head_dim);
@@ -525,15 +637,15 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   cudaError_t e = cudaSuccess;
 #define MB_TREE(XT, DD)                                                                                              \
   do {                                                                                                               \
-    const size_t smem = (size_t)(kSimtRows * DD + kSimtKeys * (DD + 4) + kSimtKeys * DD + kSimtKeys * kSimtPitch) * 4; \
+    const size_t smem = (size_t)(kMmaRows + 4 * kMmaKeys) * (DD + 4) * 4; \
     static std::atomic<uint64_t> done{0};                                                                            \
-    e = smem_once(done, tree_simt_kernel<XT, DD>, (int)smem);                                                        \
+    e = smem_once(done, tree_mma_kernel<XT, DD>, (int)smem);                                                        \
     if (e == cudaSuccess)                                                                                            \
-      e = launch_k(tree_simt_kernel<XT, DD>, dim3((unsigned)p.NS, (unsigned)(num_kv_heads * tiles), (unsigned)batch), \
-                   dim3(256), smem, st, p, (int)tiles);                                                              \
+      e = launch_k(tree_mma_kernel<XT, DD>, dim3((unsigned)p.NS, (unsigned)(num_kv_heads * tiles), (unsigned)batch), \
+                   dim3(128), smem, st, p, (int)tiles);                                                              \
     if (e == cudaSuccess && p.NS > 1)                                                                                \
       e = launch_k(tree_merge_kernel<XT, DD>,                                                                        \
-                   dim3((unsigned)((num_kv_heads * rows + 7) / 8), (unsigned)batch), dim3(256), 0, st, p, kSimtKeys); \
+                   dim3((unsigned)((num_kv_heads * rows + 7) / 8), (unsigned)batch), dim3(256), 0, st, p, kMmaKeys); \
   } while (0)
   if (tree_use_tc(x_dtype, head_dim)) {
     if (batch * num_kv_heads * p.NS * tree_tc_groups(rows) > (1LL << 30)) return kErrShape;
