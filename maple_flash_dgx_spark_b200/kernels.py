@@ -991,8 +991,7 @@ def tree_plan(parents: torch.Tensor) -> TreePlan:
         raise TypeError(f"{op}: parents must be whole numbers, got {parents.dtype}.")
     par = _as(parents, torch.int32)
     dev = par.device
-    mask = torch.empty(B, N, dtype=torch.int64, device=dev)
-    depth = torch.empty(B, N, dtype=torch.int32, device=dev)
+    mask, depth = torch.empty_like(par, dtype=torch.int64), torch.empty_like(par)
     _launch(lib().maple_tree_plan, op, d, par.data_ptr(), B, N, N, 1, mask.data_ptr(), depth.data_ptr(),
             _err(dev).data_ptr())
     return TreePlan(par, mask, depth)
@@ -1060,7 +1059,7 @@ def tree_gqa_attn(q, k_cache, v_cache, seqlen, tree_mask, *, row_map=None, scale
     sl, tm = _as(seqlen, torch.int64), _as(tree_mask, torch.int64)
     rm = _as(row_map, torch.int32) if row_map is not None else None
     dev = q.device
-    out = torch.empty(B, N, H, D, dtype=dtype, device=dev)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0:
         return out
     nbytes = max(_tree_gqa_bytes(B, N, H, n_kv, D, T, window, code), 0)
@@ -1128,9 +1127,8 @@ def verify_tree(logits, tokens, parents, uniform, *, temperature: float, top_p: 
         db, dn, _ = dp.stride()
     tok, par, u = _as(tokens, torch.int64), _as(parents, torch.int32), _as(uniform, torch.float32)
     dev = lg.device
-    path = torch.empty(B, N, dtype=torch.int32, device=dev)
+    path, ids = torch.empty_like(par), torch.empty_like(tok)
     n_path = torch.empty(B, dtype=torch.int32, device=dev)
-    ids = torch.empty(B, N, dtype=torch.int64, device=dev)
     if B == 0:
         return path, n_path, ids
     nbytes = max(_verify_bytes(B, N, V, top_k), 16)
