@@ -354,14 +354,16 @@ __device__ __forceinline__ void group_sync(int group) {
 }
 
 // The K best of a row's candidates, in order, in g.buf[0 ..]; their number.
-__device__ __forceinline__ int row_select(const VerifyParams& p, int64_t row, VerGroup& g, int group, int gt) {
+// first_counts: lane's count among the first 32 tiles, fetched ahead.
+__device__ __forceinline__ int row_select(const VerifyParams& p, int64_t row, int first_counts, VerGroup& g, int group,
+                                          int gt) {
   constexpr int WARPS = kVerCap / 32;
   const int lane = gt & 31, warp = gt >> 5;
   static_assert(kVerMaxK + kVerCap <= kVerBuf, "a tile fits behind what is carried");
   int have = 0, flip = 0;  // carried from the batches before
   for (int t0 = 0; t0 < p.tiles;) {
     // as many of the next 32 tiles as fit
-    const int c = t0 + lane < p.tiles ? __ldcg(&p.n_cand[row * p.tiles + t0 + lane]) : 0;
+    const int c = t0 == 0 ? first_counts : t0 + lane < p.tiles ? __ldcg(&p.n_cand[row * p.tiles + t0 + lane]) : 0;
     int pre = c;  // c and its prefixes: 0 and the total past the last tile
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -443,8 +445,10 @@ __device__ __forceinline__ int row_select(const VerifyParams& p, int64_t row, Ve
     // in order: each counts what stands before it
     const unsigned long long v = gt < m ? g.buf[gt] : 0ull;
     int r = gt < m ? 0 : kVerMaxK;
+    if (gt < m) {
 #pragma unroll 8
-    for (int j = 0; j < m; ++j) r += g.buf[j] > v;
+      for (int j = 0; j < m; ++j) r += g.buf[j] > v;
+    }
     group_sync(group);
     if (r < want) g.buf[r] = v;
     group_sync(group);
@@ -471,9 +475,10 @@ __global__ void __launch_bounds__(kVerWalkThreads) verify_walk_kernel(VerifyPara
   for (int n = rank * kVerGroups + group; n < p.N; n += ranks * kVerGroups) {
     const int parent = p.parents[base + n];
     const int64_t own = p.tokens[base + n];
+    const int counts = lane < p.tiles ? __ldcg(&p.n_cand[(base + n) * p.tiles + lane]) : 0;
     if (parent < -1) continue;  // padding: never looked at
     VerGroup& g = s_group[group];
-    const int have = row_select(p, base + n, g, group, gt);
+    const int have = row_select(p, base + n, counts, g, group, gt);
     if (gt < 32) {
       // `have` of K logits above -inf (none: the lowest ids share alike)
       constexpr int DS = DT == kBF16 ? 2 : 4;
