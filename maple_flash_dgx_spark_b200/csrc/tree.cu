@@ -395,8 +395,12 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
     if (r >= rows) continue;
     const int i = (int)((uint64_t)(unsigned)r * per_g >> 32), qg = r - i * p.G;
     const int64_t o = (((int64_t)b * p.N + i) * p.H + h * p.G + qg) * D, R = ((int64_t)b * p.Hkv + h) * rows + r;
-    if (mine[a] == 0) m[a] = ninf;  // padding, whatever it met in tiles that the others see whole
-    const float inv = m[a] == ninf ? 0.0f : 1.0f / l[a];
+    if (mine[a] == 0) {  // padding, whatever it met in tiles that the others see whole
+      m[a] = ninf;
+      l[a] = 0.0f;
+    }
+    const bool none = m[a] == ninf && l[a] == 0.0f;  // sees nothing; NaN scores stay NaN
+    const float inv = none ? 0.0f : 1.0f / l[a];
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) {
       const float x0 = acc[j][2 * a], x1 = acc[j][2 * a + 1];
@@ -404,13 +408,13 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
       if (!alone) {
         *reinterpret_cast<float2*>(p.ws_acc + (R * p.NS + sp) * D + d) = make_float2(x0, x1);
       } else {
-        store_f<XT>(p.out, o + d, m[a] == ninf ? 0.0f : x0 * inv);
-        store_f<XT>(p.out, o + d + 1, m[a] == ninf ? 0.0f : x1 * inv);
+        store_f<XT>(p.out, o + d, none ? 0.0f : x0 * inv);
+        store_f<XT>(p.out, o + d + 1, none ? 0.0f : x1 * inv);
       }
     }
     if (!alone && t == 0) {
       p.ws_ml[(R * p.NS + sp) * 2] = m[a];
-      p.ws_ml[(R * p.NS + sp) * 2 + 1] = m[a] == ninf ? 0.0f : l[a];
+      p.ws_ml[(R * p.NS + sp) * 2 + 1] = l[a];
     }
   }
 }
@@ -604,7 +608,7 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
                                    const int32_t* row_map, float scale, int64_t window, void* out, void* workspace,
                                    int64_t workspace_bytes, int* err, void* stream) {
   if (batch < 0 || nodes <= 0 || nodes > kTreeMaxNodes || num_heads <= 0 || num_kv_heads <= 0 || max_len <= 0 ||
-      cache_batch < 0 || window < 0)
+      cache_batch < 0 || window < 0 || !(scale - scale == 0.0f))
     return kErrShape;
   if (batch == 0) return kOk;
   if (x_dtype != kF32 && x_dtype != kBF16) return kErrDtype;

@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       dm = __reduce_max_sync(0xffffffffu, dm);
       const TreeRange rg = tree_range(p, len, cb, ((unsigned long long)uh << 32) | ul);
       if (rg.bad && lane == 0) atomicOr(p.err, kErrFlagBounds);
+      const int mh = p.c_sh ? h : 0, mb = p.c_sb ? rg.cb : 0;  // a stride of 0 is a map of one
       int k0, k1;
       tree_split(rg.lo, rg.hi, kTtKeys, p.NS, sp, k0, k1);
       if (sp > 0 && k0 >= k1) continue;  // nothing here; split 0 always answers
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             mbar_expect_tx(&kfull[st], (unsigned)TILE);
 #pragma unroll
             for (int hf = 0; hf < HALVES; ++hf)
-              tma_load_4d(sk + st * TILE + hf * BOX, &tmk, 64 * hf, k0 + c * kTtKeys, h, rg.cb, &kfull[st]);
+              tma_load_4d(sk + st * TILE + hf * BOX, &tmk, 64 * hf, k0 + c * kTtKeys, mh, mb, &kfull[st]);
           }
           if (c >= AHEAD) {
             const int g = kt_all + c - AHEAD, st = g % NV;
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             mbar_expect_tx(&vfull[st], (unsigned)TILE);
 #pragma unroll
             for (int hf = 0; hf < HALVES; ++hf)
-              tma_load_4d(sv + st * TILE + hf * BOX, &tmv, 64 * hf, k0 + (c - AHEAD) * kTtKeys, h, rg.cb, &vfull[st]);
+              tma_load_4d(sv + st * TILE + hf * BOX, &tmv, 64 * hf, k0 + (c - AHEAD) * kTtKeys, mh, mb, &vfull[st]);
           }
         }
       }
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         l = la + lb;
         mc = M;
       }
-      const bool zero = !(row < rows && mine != 0) || mc == ninf;
+      const bool zero = !(row < rows && mine != 0) || (mc == ninf && l == 0.0f);  // sees nothing; NaN scores stay NaN
       const float inv = zero ? 0.0f : 1.0f / l;
       // partials [item][dim][row of the tile]: a warp's 32 rows store side by side
       const int64_t part = (((int64_t)b * p.Hkv + h) * p.NS + it.sp) * ((rows + kTtRows - 1) / kTtRows) + row / kTtRows;
@@ -744,9 +745,12 @@ cudaError_t tree_tc_launch1(const TreeAttnParams& p, int groups, const CUtensorM
 }
 
 cudaError_t tree_tc_launch(const TreeAttnParams& p, int D, cudaStream_t st) {
+  // (dim, position, KV head, cache row); heads or rows that share one are a map of one
   CUtensorMap tmk, tmv;
-  if (!tmap_bf16_4d(p.kc, D, p.T, p.Hkv, p.Bc, D, p.c_sh, p.c_sb, 64, kTtKeys, &tmk) ||
-      !tmap_bf16_4d(p.vc, D, p.T, p.Hkv, p.Bc, D, p.c_sh, p.c_sb, 64, kTtKeys, &tmv))
+  const int64_t heads = p.c_sh ? p.Hkv : 1, hs = p.c_sh ? p.c_sh : (int64_t)p.T * D;
+  const int64_t caches = p.c_sb ? p.Bc : 1, bs = p.c_sb ? p.c_sb : hs * heads;
+  if (!tmap_bf16_4d(p.kc, D, p.T, heads, caches, D, hs, bs, 64, kTtKeys, &tmk) ||
+      !tmap_bf16_4d(p.vc, D, p.T, heads, caches, D, hs, bs, 64, kTtKeys, &tmv))
     return cudaErrorInvalidValue;
   const int rows = p.N * p.G, groups = tree_tc_groups(rows);
   const bool pair = rows > kTtRows;

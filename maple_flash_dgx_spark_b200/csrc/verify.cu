@@ -85,23 +85,19 @@ __device__ __forceinline__ void warp_prefix_d(const double (&a)[2], double (&c)[
 // per thread in flight together, and keeps each vector's maximum.  T, just
 // below the K-th largest of the 256 threads' maxima, is at most the tile's
 // K-th largest logit, and few logits reach it (about K of 16384: threads seldom
-// hold two); a thread looks again into its own vectors that do.  T is found bit
+// hold two); the vectors that do are looked into again.  T is found bit
 // by bit, one warp counting the maxima with votes, from the first bit in which
 // they differ until close to K of them reach it: a T a little too low only lets
 // a few more through.  Where more than kVerCap come through (ties, large logits
 // side by side) the tile's K largest are selected exactly, ties to the lowest
 // ids.  -inf and NaN are not handed on: they have no weight, and a row of
 // nothing else is known by having no candidates.  Five CTAs per SM: their loads
-// cover each other's search for T (a ring of tiles in shared memory with two
+// cover each other's search for T, and their tiles stay in L1 for the second
+// look (read past L1 it cost 13 of 38 us at K = 50; a ring of tiles in shared memory with two
 // CTAs per SM measured slower, 45 against 40 us for 64 x 8 rows of 151936).
 // One word whose order is larger logit, then lower id.
 __device__ __forceinline__ unsigned long long cand_word(const uint2& v) {
   return (unsigned long long)v.x << 32 | (0xffffffffu - v.y);
-}
-__device__ __forceinline__ uint4 ld_once_u4(const void* p) {  // written by the launch before: not the read-only path
-  uint4 r;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
 }
 // Larger of two words of logits (two bf16, or one fp32), NaN giving way.
 template <int XT>
@@ -120,42 +116,28 @@ __device__ __forceinline__ float word_max(uint32_t w) {
   return __uint_as_float(w);
 }
 
+// Exactly the K largest logits above -inf of a tile (elements k0 .. of row x),
+// all of them where there are fewer, in no order, into `list`; their number.
+// The smallest one's word by halving, all above it, and its first ties in order
+// of ids, the tile read again each time (it fits L1 as the CTAs lie).  For all
+// threads of the CTA at once.
 template <int XT>
-struct VerWord { using type = uint32_t; };
-template <>
-struct VerWord<kBF16> { using type = uint16_t; };
-
-// Exactly the K largest logits above -inf of a tile in shared memory (all of
-// them where there are fewer), in no order, into `list`; their number.  The
-// smallest one's word by halving, all above it, and its first ties in order of
-// ids.  The tile's words take the place of its logits.  For all threads of the
-// CTA at once.
-template <int XT>
-__device__ __noinline__ int verify_tile_exact(const VerifyParams& p, uint4* tile, int k0, uint2* list, int* s_cnt,
+__device__ __noinline__ int verify_tile_exact(const VerifyParams& p, const char* x, int k0, uint2* list, int* s_cnt,
                                               int* s_warp) {
   constexpr int EPC = XT == kBF16 ? 8 : 4, SH = XT == kBF16 ? 16 : 0, TILE = kVerThreads * kVerVecs * EPC;
   constexpr uint32_t kInf = 0x007fffffu >> SH;  // word of -inf
-  using Word = typename VerWord<XT>::type;
-  Word* words = reinterpret_cast<Word*>(tile);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int j = tid; j < TILE; j += kVerThreads) {
+  auto word = [&](int j) -> uint32_t {  // 0 outside of the row
     const int k = k0 + j;
-    words[j] = (Word)(k >= 0 && k < p.V ? logit_key(load_f<XT>(tile, j)) >> SH : 0u);
-  }
+    return k >= 0 && k < p.V ? logit_key(load_f<XT>(x, k)) >> SH : 0u;
+  };
   int flip = 0;
   auto count = [&](uint32_t c) {  // words at or above c
     if (tid == 0) s_cnt[flip] = 0;
     __syncthreads();
     int cnt = 0;
-    for (int i = 0; i < kVerVecs; ++i) {
-      const uint4 v = tile[i * kVerThreads + tid];
-      const uint32_t q[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (XT == kBF16) cnt += ((q[e] & 0xffffu) >= c) + ((q[e] >> 16) >= c);
-        else cnt += q[e] >= c;
-      }
-    }
+#pragma unroll 8
+    for (int j = tid; j < TILE; j += kVerThreads) cnt += word(j) >= c;
     cnt = __reduce_add_sync(0xffffffffu, cnt);
     if (lane == 0) atomicAdd(&s_cnt[flip], cnt);
     __syncthreads();
@@ -174,12 +156,14 @@ __device__ __noinline__ int verify_tile_exact(const VerifyParams& p, uint4* tile
   auto key_of = [](uint32_t w) {  // the whole word again
     return XT == kBF16 ? (w & 0x8000u ? w << 16 : w << 16 | 0xffffu) : w;
   };
-  for (int j = tid; j < TILE; j += kVerThreads)
-    if (words[j] > kth) list[atomicAdd(&s_cnt[0], 1)] = make_uint2(key_of(words[j]), (uint32_t)(k0 + j));
+  for (int j = tid; j < TILE; j += kVerThreads) {
+    const uint32_t w = word(j);
+    if (w > kth) list[atomicAdd(&s_cnt[0], 1)] = make_uint2(key_of(w), (uint32_t)(k0 + j));
+  }
   __syncthreads();
   int base = s_cnt[0];  // fewer than `want`
   for (int j0 = 0; j0 < TILE && base < want; j0 += kVerThreads) {
-    const unsigned vote = __ballot_sync(0xffffffffu, words[j0 + tid] == kth);
+    const unsigned vote = __ballot_sync(0xffffffffu, word(j0 + tid) == kth);
     if (lane == 0) s_warp[warp] = __popc(vote);
     __syncthreads();
     int at = base + __popc(vote & ((1u << lane) - 1u)), all = 0;
@@ -249,10 +233,10 @@ __global__ void __launch_bounds__(kVerThreads, 5) verify_tile_kernel(VerifyParam
   constexpr int VECS = kVerVecs * kVerThreads, TILE = VECS * EPC;
   __shared__ float s_max[kVerThreads];
   __shared__ uint32_t s_t;
-  __shared__ int s_n, s_cnt[2];
+  __shared__ int s_n, s_vecs, s_cnt[2];
   __shared__ int s_warp[kVerThreads / 32];
+  __shared__ uint16_t s_vec[VECS];
   __shared__ uint2 s_list[kVerCap];
-  __shared__ uint4 s_tile[VECS];  // the exact selection's words
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tile = blockIdx.x, n = blockIdx.y, b = blockIdx.z;
   pdl_wait();
@@ -267,15 +251,15 @@ __global__ void __launch_bounds__(kVerThreads, 5) verify_tile_kernel(VerifyParam
   uint4 r[kVerVecs];
   if (inner) {
 #pragma unroll
-    for (int i = 0; i < kVerVecs; ++i) r[i] = ld_once_u4(src + i * kVerThreads * 16);
+    for (int i = 0; i < kVerVecs; ++i) r[i] = ld_u4(src + i * kVerThreads * 16);
   } else {
 #pragma unroll
     for (int i = 0; i < kVerVecs; ++i) {
       const int k = k0 + (i * kVerThreads + tid) * EPC;
-      r[i] = k >= 0 && k + EPC <= p.V ? ld_once_u4(src + i * kVerThreads * 16) : edge_vector<XT>(x, k, p.V);
+      r[i] = k >= 0 && k + EPC <= p.V ? ld_u4(src + i * kVerThreads * 16) : edge_vector<XT>(x, k, p.V);
     }
   }
-  if (tid == 0) s_n = 0;
+  if (tid == 0) s_n = s_vecs = 0;
   float vm[kVerVecs], mx = __int_as_float(0xff800000);
 #pragma unroll
   for (int i = 0; i < kVerVecs; ++i) {
@@ -291,13 +275,19 @@ __global__ void __launch_bounds__(kVerThreads, 5) verify_tile_kernel(VerifyParam
   }
   __syncthreads();
   const float tf = key_logit(s_t);
-  uint32_t in = 0;  // this thread's vectors that reach T; lanes go through theirs side by side
+  // the vectors that reach T, put together so that few warps look into them
+  uint32_t in = 0;
 #pragma unroll
   for (int i = 0; i < kVerVecs; ++i) in |= (vm[i] >= tf ? 1u : 0u) << i;
+  if (in) {
+    int at = atomicAdd(&s_vecs, __popc(in));
+    for (; in; in &= in - 1) s_vec[at++] = (uint16_t)((__ffs((int)in) - 1) * kVerThreads + tid);
+  }
+  __syncthreads();
 #pragma unroll 1
-  for (; in; in &= in - 1) {
-    const int i = __ffs((int)in) - 1, k = k0 + (i * kVerThreads + tid) * EPC;
-    const uint4 v = k >= 0 && k + EPC <= p.V ? ld_once_u4(src + i * kVerThreads * 16) : edge_vector<XT>(x, k, p.V);
+  for (int j = tid; j < s_vecs; j += kVerThreads) {
+    const int k = k0 + s_vec[j] * EPC;
+    const uint4 v = k >= 0 && k + EPC <= p.V ? ld_u4(x + (int64_t)k * ES) : edge_vector<XT>(x, k, p.V);
     const uint32_t q[4] = {v.x, v.y, v.z, v.w};
     auto value = [&](int e) {  // e a constant
       const uint32_t w = q[e * ES / 4];
@@ -318,10 +308,7 @@ __global__ void __launch_bounds__(kVerThreads, 5) verify_tile_kernel(VerifyParam
   __syncthreads();
   int found = s_n;
   if (found > kVerCap) {
-#pragma unroll 1
-    for (int i = 0; i < kVerVecs; ++i) s_tile[i * kVerThreads + tid] = edge_vector<XT>(x, k0 + (i * kVerThreads + tid) * EPC, p.V);
-    __syncthreads();
-    found = verify_tile_exact<XT>(p, s_tile, k0, s_list, s_cnt, s_warp);
+    found = verify_tile_exact<XT>(p, x, k0, s_list, s_cnt, s_warp);
     __syncthreads();
   }
   const int64_t slot = row * p.tiles + tile;

@@ -244,6 +244,64 @@ def test_attention_carries_what_a_row_sees(cuda, K, dtype):
     torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("L,T", [(300, 400), (3000, 8000)])  # one part, and several joined
+def test_attention_nan_queries_and_keys(cuda, K, dtype, L, T):
+    """A NaN in a query reaches its own row alone, though no score of it is a
+    number; a NaN key every row that sees it, and no other."""
+    par = [[-1, 0, 0, 1, 2, 3]]
+    c = attn_case(18, 1, 6, 8, 2, 128, T, [L], dtype, mask=ref.plan(par)[0])
+    clean = run_attn(K, c)
+    q, k = c["q"].clone(), c["k"].clone()
+    q[0, 4, 3, 17] = float("nan")
+    k[0, 1, L + 1, 5] = float("nan")  # node 1 of KV head 1: nodes 1, 3 and 5, heads 4 to 7
+    want = clean.float().clone()
+    want[0, 4, 3] = float("nan")
+    for i in (1, 3, 5):
+        want[0, i, 4:] = float("nan")
+    torch.testing.assert_close(run_attn(K, {**c, "q": q, "k": k}).float(), want, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_attention_infinite_keys(cuda, K, dtype):
+    """A key with an infinity: a score of -inf weighs nothing, one of +inf leaves
+    no number."""
+    c = attn_case(19, 1, 4, 4, 2, 64, 200, [150], dtype, chain=True)
+    q, k = c["q"].clone(), c["k"].clone()
+    q[0, :, :, 3] = torch.tensor([1.0, -1.0, 1.0, -1.0], device=cuda, dtype=dtype)  # per head
+    k[0, :, 20, 3] = float("inf")
+    got = run_attn(K, {**c, "q": q, "k": k})
+    assert torch.isnan(got[0, :, 0]).all() and torch.isnan(got[0, :, 2]).all()
+    kz = k.clone()
+    kz[0, :, 20] = 0
+    v0 = c["v"].clone()
+    want, mass, reach = ref.attention(q, torch.cat([kz[:, :, :20], kz[:, :, 21:]], 2), torch.cat([v0[:, :, :20], v0[:, :, 21:]], 2),
+                                      [149], c["mask"], None, c["scale"], 0)
+    check_attention(got[:, :, 1::2], want[:, :, 1::2], mass[:, :, 1::2], reach[:, :, 1::2], dtype, 154)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_attention_expanded_caches(cuda, K, dtype):
+    """One prefix for all sequences, one KV head for all groups: strides of 0."""
+    c = attn_case(20, 3, 5, 8, 4, 128, 300, [250, 250, 100], dtype)
+    k, v = c["k"][:1, :1].expand(3, 4, 300, 128), c["v"][:1, :1].expand(3, 4, 300, 128)
+    want = run_attn(K, {**c, "k": k.contiguous(), "v": v.contiguous()})
+    torch.testing.assert_close(run_attn(K, {**c, "k": k, "v": v}), want, rtol=0, atol=0)
+    k, v = c["k"][:1].expand(3, 4, 300, 128), c["v"][:1].expand(3, 4, 300, 128)
+    want = run_attn(K, {**c, "k": k.contiguous(), "v": v.contiguous()})
+    torch.testing.assert_close(run_attn(K, {**c, "k": k, "v": v}), want, rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_attention_scale_zero_and_negative(cuda, K, dtype, scale):
+    c = attn_case(23, 2, 6, 8, 2, 128, 400, [300, 17], dtype, ragged=True)
+    c["scale"] = scale
+    got = run_attn(K, c)
+    want, mass, reach = ref.attention(c["q"], c["k"], c["v"], c["lens"], c["mask"], None, scale, 0)
+    check_attention(got, want, mass, reach.abs(), dtype, 306)
+
+
 def test_attention_huge_scores(cuda, K):
     """Scores far apart (weights underflow) and negative maxima."""
     for scale in (1.0, 8.0):

@@ -26,18 +26,19 @@ def L():
     return _lib.lib()
 
 
-def _attn(L, *, q=P, dtype=1, B=2, N=8, H=32, Hkv=4, T=1024, D=128, k=P, out=P, ws=P, nbytes=1 << 40, err=P, sb=None,
+def _attn(L, *, scale=0.1, q=P, dtype=1, B=2, N=8, H=32, Hkv=4, T=1024, D=128, k=P, out=P, ws=P, nbytes=1 << 40, err=P, sb=None,
           window=0, qsh=None, Bc=2):
     qsh = D if qsh is None else qsh
     sb = Hkv * T * D if sb is None else sb
     return L.maple_tree_gqa_attn(q, dtype, B, N, H, N * H * D, H * D, qsh, k, k, Bc, Hkv, sb, T * D, T, D, P, P, None,
-                                 0.1, window, out, ws, nbytes, err, None)
+                                 scale, window, out, ws, nbytes, err, None)
 
 
 def test_tree_attention_refuses_before_any_launch(L):
     assert _attn(L, B=0) == 0                        # nothing to do
     for bad in (dict(B=-1), dict(N=0), dict(N=65), dict(H=0), dict(Hkv=0), dict(H=30), dict(D=96), dict(T=0),
-                dict(window=-1), dict(B=1 << 17), dict(Bc=0), dict(T=1 << 31)):
+                dict(window=-1), dict(B=1 << 17), dict(Bc=0), dict(T=1 << 31), dict(scale=float("nan")),
+                dict(scale=float("inf"))):
         assert _attn(L, **bad) == 1, bad
     for null in ("q", "k", "out", "err"):
         assert _attn(L, **{null: None}) == 1, null
