@@ -504,6 +504,28 @@ def test_verify_ties_and_special_logits(cuda, K, dtype):
             check_verify(K, logits, tok, [[-1, 0]] * B, u, None, temperature=1.0, top_p=0.9, top_k=k)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V,finite", [(600001, None), (100000, 30), (100000, 64), (40000, 500), (17000, 0)])
+def test_verify_masked_and_long_vocabularies(cuda, K, V, finite, dtype):
+    """Constrained decoding: all but a few logits -inf, none in the first tile;
+    and a vocabulary of more tiles than one pass of the selection takes."""
+    r = np.random.RandomState(V % 1000)
+    lg = (r.standard_normal((2, 2, V)) * 2.5).astype(np.float32)
+    tok = np.zeros((2, 2), np.int64)
+    if finite is not None:
+        keep = np.zeros((2, 2, V), bool)
+        for b in range(2):
+            for n in range(2):
+                keep[b, n, 16400 + r.permutation(V - 16400)[:finite]] = True
+        lg = np.where(keep, lg, -np.inf)
+    tok[:, 1] = lg[:, 0].argmax(-1)
+    logits = torch.from_numpy(lg).to(cuda, dtype)
+    for k in (1, 20, 64):
+        for seed in range(3):
+            u = np.random.RandomState(seed).random_sample((2, 2)).astype(np.float32)
+            check_verify(K, logits, tok, [[-1, 0]] * 2, u, None, temperature=0.9, top_p=0.97, top_k=k)
+
+
 def test_verify_border_uniforms(cuda, K):
     """0 accepts whatever the target gives weight to, and draws the first token;
     the largest value below 1 draws the last kept one."""
