@@ -67,10 +67,14 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, 
 // One CTA per (split of the keys, KV head and tile of 64 query rows, sequence).
 // Row r of a KV head is node r / G, query head h G + r % G; a warp has 16 rows.
 // Products on the tensor pipe as tf32 (mma.sync m16n8k8), each fp32 operand x
-// split into hi = x with its low 13 bits cleared and lo = x - hi (exact):
-// lo hi + hi lo + hi hi leaves out lo lo, 2^-22 of the product, so an fp32
-// result keeps its precision; bf16 values are their own hi, which saves two of
-// the three for the scores and one for the output.  Tiles of 32 keys stand in
+// split into hi (x in tf32) and lo = x - hi (exact, then rounded to tf32):
+// lo hi + hi lo + hi hi leaves out 2^-23 of a product.  The pipe cuts its sums
+// instead of rounding them, so an fp32 sum takes at most four steps on it
+// before it is added to the rest with fp32's own rounding: 8e-7 of error at
+// 4 x 1500, where straight sums had 2.6e-6 (and 31 us for 33; two steps 5e-7
+// and 3 % more time).  bf16 values are their own hi, which saves two of the
+// three products for the scores and one for the output; their results' rounding
+// to 2^-8 hides the cut sums, which stay straight.  Tiles of 32 keys stand in
 // shared memory as fp32 in two stages (cp.async under the tile before); a pitch
 // of D + 4 floats keeps ldmatrix (K, Q) and the V reads free of bank conflicts.
 // The weights stay in registers: key 2t of a block of eight takes the place of
@@ -80,7 +84,9 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, 
 // not keep NaN out: K and V are cleared of both as they arrive.  A score with a
 // cleared key is computed again from the cache (each such key by its threads);
 // cleared values of V are added at the end for the rows that see them.
-// Before, on the fp32 pipes: 33 us for 4 x 1500 with heads of 64, 17 nodes.
+// 8 nodes, 16 query heads of 256 on 4 KV heads, 4 x 4096 bf16: 115 us, 580 GB/s
+// of cache; 32 heads of 128 on 8 with 64 nodes, 8 x 4000 fp32: 1.16 ms, 29
+// TFLOP/s.  Bound by issue: splits, ldmatrix and V's 4-byte reads per product.
 constexpr int kMmaRows = 64;
 constexpr int kMmaKeys = 32;
 
@@ -97,11 +103,15 @@ __device__ __forceinline__ void ldsm4(const float* p, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(smem_u32(p)));
 }
+// hi is x rounded to tf32, or cut to it where x may be the largest fp32; lo is
+// half a step up, as the pipe ignores the low 13 bits.
+template <bool CUT>
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
-  hi = x & 0xffffe000u;
-  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+  hi = (CUT ? x : x + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi)) + 0x1000u;
 }
 __device__ __forceinline__ bool odd_f32(uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u; }  // NaN, infinity
+__device__ __forceinline__ bool huge_f32(uint32_t x) { return (x & 0x7fffffffu) >= 0x7f7ff000u; }  // or rounds to it
 
 template <int XT, int D>
 __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row_tiles) {
@@ -214,7 +224,7 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
 #pragma unroll
       for (int u = 0; u < EPC; u += 4) {
         const uint4 x = *reinterpret_cast<const uint4*>(st + (e & 1) * kMmaKeys * PITCH + r * PITCH + cc + u);
-        any |= odd_f32(x.x) | odd_f32(x.y) | odd_f32(x.z) | odd_f32(x.w);
+        any |= huge_f32(x.x) | huge_f32(x.y) | huge_f32(x.z) | huge_f32(x.w);
       }
     }
     if (!any) return;
@@ -223,7 +233,7 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
       const int c = tid + 128 * (e >> 1), r = c / CH, cc = c % CH * EPC;
       for (int u = 0; u < EPC; ++u) {
         uint32_t* x = reinterpret_cast<uint32_t*>(st + (e & 1) * kMmaKeys * PITCH + r * PITCH + cc + u);
-        if (!odd_f32(*x)) continue;
+        if (!(e & 1 ? odd_f32(*x) : huge_f32(*x))) continue;
         *x = 0u;
         if (e & 1) s_fix = 1;
         else atomicOr(&s_odd[stage], 1u << r);
@@ -268,30 +278,41 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
     if (!idle) {
       float s[4][4] = {};  // 16 rows x 32 keys: block j, keys 8 j + 2 t, + 1 of rows g (0, 1) and g + 8 (2, 3)
       const float* b_at = sk + ((lane & 7) + (lane >> 4) * 8) * PITCH + (lane >> 3 & 1) * 4;
-#pragma unroll 4
-      for (int kk = 0; kk < D / 8; ++kk) {
-        uint32_t a[4], ah[4], al[4];
-        ldsm4(a_at + 8 * kk, a);
+#pragma unroll 2
+      for (int k4 = 0; k4 < D / 8; k4 += 4) {
+        float fresh[4][4] = {};
+        float(&part)[4][4] = XT == kBF16 ? s : fresh;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_tf32(a[i], ah[i], al[i]);
+        for (int kk = k4; kk < k4 + 4; ++kk) {
+          uint32_t a[4], ah[4], al[4];
+          ldsm4(a_at + 8 * kk, a);
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-          uint32_t y[4];
-          ldsm4(b_at + 8 * j * PITCH + 8 * kk, y);
-          if constexpr (XT == kBF16) {
-            mma_tf32(s[j], a, y[0], y[1]);
-            mma_tf32(s[j + 1], a, y[2], y[3]);
-          } else {
-            uint32_t yh[4], yl[4];
+          for (int i = 0; i < 4; ++i) split_tf32<true>(a[i], ah[i], al[i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) split_tf32(y[i], yh[i], yl[i]);
-            mma_tf32(s[j], al, yh[0], yh[1]);
-            mma_tf32(s[j + 1], al, yh[2], yh[3]);
-            mma_tf32(s[j], ah, yl[0], yl[1]);
-            mma_tf32(s[j + 1], ah, yl[2], yl[3]);
-            mma_tf32(s[j], ah, yh[0], yh[1]);
-            mma_tf32(s[j + 1], ah, yh[2], yh[3]);
+          for (int j = 0; j < 4; j += 2) {
+            uint32_t y[4];
+            ldsm4(b_at + 8 * j * PITCH + 8 * kk, y);
+            if constexpr (XT == kBF16) {
+              mma_tf32(part[j], a, y[0], y[1]);
+              mma_tf32(part[j + 1], a, y[2], y[3]);
+            } else {
+              uint32_t yh[4], yl[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) split_tf32<false>(y[i], yh[i], yl[i]);
+              mma_tf32(part[j], al, yh[0], yh[1]);
+              mma_tf32(part[j + 1], al, yh[2], yh[3]);
+              mma_tf32(part[j], ah, yl[0], yl[1]);
+              mma_tf32(part[j + 1], ah, yl[2], yl[3]);
+              mma_tf32(part[j], ah, yh[0], yh[1]);
+              mma_tf32(part[j + 1], ah, yh[2], yh[3]);
+            }
           }
+        }
+        if constexpr (XT != kBF16) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[j][c] += fresh[j][c];
         }
       }
       if (const unsigned odd = s_odd[stage]; odd) {  // rare: keys with a NaN or an infinity, from the cache
@@ -345,28 +366,37 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
 #pragma unroll
           for (int c = 0; c < 4; ++c) acc[j][c] *= fix[c >> 1];
       }
+      uint32_t ah[4][4], al[4][4];
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
-        const uint32_t a[4] = {__float_as_uint(s[kk][0]), __float_as_uint(s[kk][2]), __float_as_uint(s[kk][1]),
-                               __float_as_uint(s[kk][3])};
-        uint32_t ah[4], al[4];
+        const int order[4] = {0, 2, 1, 3};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_tf32(a[i], ah[i], al[i]);
-        const float* v_at = sv + (8 * kk + 2 * t) * PITCH + g;
+        for (int i = 0; i < 4; ++i) split_tf32<false>(__float_as_uint(s[kk][order[i]]), ah[kk][i], al[kk][i]);
+      }
+      const float* v_at = sv + 2 * t * PITCH + g;
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-          const uint32_t y0 = __float_as_uint(v_at[8 * j]), y1 = __float_as_uint(v_at[PITCH + 8 * j]);
+      for (int j = 0; j < D / 8; ++j) {
+        float fresh[4] = {};
+        float(&part)[4] = XT == kBF16 ? acc[j] : fresh;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint32_t y0 = __float_as_uint(v_at[8 * kk * PITCH + 8 * j]);
+          const uint32_t y1 = __float_as_uint(v_at[(8 * kk + 1) * PITCH + 8 * j]);
           if constexpr (XT == kBF16) {
-            mma_tf32(acc[j], al, y0, y1);
-            mma_tf32(acc[j], ah, y0, y1);
+            mma_tf32(part, al[kk], y0, y1);
+            mma_tf32(part, ah[kk], y0, y1);
           } else {
             uint32_t h0, l0, h1, l1;
-            split_tf32(y0, h0, l0);
-            split_tf32(y1, h1, l1);
-            mma_tf32(acc[j], al, h0, h1);
-            mma_tf32(acc[j], ah, l0, l1);
-            mma_tf32(acc[j], ah, h0, h1);
+            split_tf32<true>(y0, h0, l0);
+            split_tf32<true>(y1, h1, l1);
+            mma_tf32(part, al[kk], h0, h1);
+            mma_tf32(part, ah[kk], l0, l1);
+            mma_tf32(part, ah[kk], h0, h1);
           }
+        }
+        if constexpr (XT != kBF16) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[j][c] += fresh[c];
         }
       }
     }

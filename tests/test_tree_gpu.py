@@ -280,6 +280,40 @@ def test_attention_infinite_keys(cuda, K, dtype):
     check_attention(got[:, :, 1::2], want[:, :, 1::2], mass[:, :, 1::2], reach[:, :, 1::2], dtype, 154)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, F32), (128, F32), (256, F32), (128, BF), (256, BF)])
+def test_attention_largest_keys_and_values(cuda, K, D, dtype):
+    """The type's largest number in a key (scores near 1) and in a value, where
+    rounding it up on the way would leave the type."""
+    c = attn_case(24, 1, 6, 4, 2, D, 200, [150], dtype)
+    big = torch.finfo(dtype).max
+    c["q"] = c["q"].clone()
+    c["q"][..., 3] = c["q"][..., 3] * (4.0 / big)
+    c["k"][0, 0, [5, 77], 3] = big
+    c["k"][0, 1, 151, 3] = -big
+    c["v"][0, 0, 9, 1] = big
+    verify_attn(K, c)
+
+
+@pytest.mark.parametrize("D,L", [(64, 1500), (128, 1500), (256, 700)])
+def test_attention_fp32_is_as_close_as_a_plain_one(cuda, K, D, L):
+    """Not worse than fp32 products, softmax and sums one after the other, whose
+    own error varies by less than twice from one order of summing to another."""
+    c = attn_case(25, 2, 8, 8, 2, D, L + 20, [L, L - 9], F32)
+    got = run_attn(K, c).double()
+    want, _, _ = ref.attention(c["q"], c["k"], c["v"], c["lens"], c["mask"], None, c["scale"], 0)
+    k, v = (c[x].repeat_interleave(4, 1)[:, :, :L + 8] for x in "kv")
+    s = (c["q"].transpose(1, 2) @ k.transpose(2, 3)) * c["scale"]
+    for b, n in enumerate(c["lens"]):
+        sees = torch.arange(L + 8, device=cuda) < n
+        sees = sees.repeat(8, 1)
+        for i in range(8):
+            for j in range(8):
+                sees[i, n + j] = bool(int(c["mask"][b, i]) >> j & 1)
+        s[b].masked_fill_(~sees, float("-inf"))
+    plain = (s.softmax(-1) @ v).transpose(1, 2).double()
+    assert (got - want).norm() <= 2 * (plain - want).norm()
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_attention_expanded_caches(cuda, K, dtype):
     """One prefix for all sequences, one KV head for all groups: strides of 0."""
