@@ -64,15 +64,15 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, 
 }
 
 // ------------------------------------- attention, fp32 and heads of 256 --
-// One CTA per (split of the keys, KV head and tile of 64 query rows, sequence).
-// Row r of a KV head is node r / G, query head h G + r % G; a warp has 16 rows.
+// One CTA per (split of the keys, KV head and tile of query rows, sequence).
+// Row r of a KV head is node r / G, query head h G + r % G; a warp has 16 rows
+// and a part of each tile's keys; the parts are joined in shared memory.
 // Products on the tensor pipe as tf32 (mma.sync m16n8k8), each fp32 operand x
 // split into hi (x in tf32) and lo = x - hi (exact, then rounded to tf32):
 // lo hi + hi lo + hi hi leaves out 2^-23 of a product.  The pipe cuts its sums
 // instead of rounding them, so an fp32 sum takes at most four steps on it
-// before it is added to the rest with fp32's own rounding: 8e-7 of error at
-// 4 x 1500, where straight sums had 2.6e-6 (and 31 us for 33; two steps 5e-7
-// and 3 % more time).  bf16 values are their own hi, which saves two of the
+// before it is added to the rest with fp32's own rounding: 7e-7 of error at
+// 4 x 1500, where straight sums had 2.6e-6 (and 8 % less time).  bf16 values are their own hi, which saves two of the
 // three products for the scores and one for the output; their results' rounding
 // to 2^-8 hides the cut sums, which stay straight.  Tiles of 32 keys stand in
 // shared memory as fp32 in two stages (cp.async under the tile before); a pitch
@@ -84,14 +84,17 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, 
 // not keep NaN out: K and V are cleared of both as they arrive.  A score with a
 // cleared key is computed again from the cache (each such key by its threads);
 // cleared values of V are added at the end for the rows that see them.
-// 8 nodes, 16 query heads of 256 on 4 KV heads, 4 x 4096 bf16: 115 us, 580 GB/s
-// of cache; 32 heads of 128 on 8 with 64 nodes, 8 x 4000 fp32: 1.16 ms, 29
-// TFLOP/s.  Bound by issue: splits, ldmatrix and V's 4-byte reads per product.
-constexpr int kMmaRows = 64;
+// 16 query heads of 256 on 4 KV heads, 8 nodes, 4 x 4096 bf16: 80 us, 840 GB/s
+// of cache (115 with four warps that shared no keys); 32 heads of 128 on 8 with
+// 64 nodes, 8 x 4000 fp32: 975 us, 34 TFLOP/s (1160).  Bound by the latency of
+// its instructions: a scheduler issues in two cycles of five at 8 x 4000, eight
+// instructions per product (splits, ldmatrix, V's 4-byte reads), and the
+// registers hold no more than four warps on it.
 constexpr int kMmaKeys = 32;
+constexpr int kMmaWarps = 8, kMmaThreads = 32 * kMmaWarps;
 
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -112,35 +115,44 @@ __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& l
 }
 __device__ __forceinline__ bool odd_f32(uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u; }  // NaN, infinity
 __device__ __forceinline__ bool huge_f32(uint32_t x) { return (x & 0x7fffffffu) >= 0x7f7ff000u; }  // or rounds to it
+// Without the two bits by which lo would round hi + lo up past fp32 (2^-22 of it).
+__device__ __forceinline__ uint32_t cut_huge(uint32_t x) { return huge_f32(x) && !odd_f32(x) ? x & ~3u : x; }
 
-template <int XT, int D>
-__global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row_tiles) {
+// RW warps of 16 rows beside each other, KW = 8 / RW groups of them with 32 / KW
+// keys of each tile, joined at the end.
+template <int XT, int D, int RW>
+__global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
+    tree_mma_kernel(TreeAttnParams p, int row_tiles) {
+  constexpr int JG = 4;  // products of V side by side, for their latency
+  constexpr int ROWS = 16 * RW, KW = kMmaWarps / RW, JW = 4 / KW;  // JW: blocks of eight keys per warp and tile
   constexpr int PITCH = D + 4, es = XT == kBF16 ? 2 : 4, EPC = 16 / es, CH = D / EPC;
   constexpr int STAGE = 2 * kMmaKeys * PITCH;             // floats: K, then V
-  constexpr int PER = kMmaKeys * CH / 128;                // 16-byte chunks of K (and of V) per thread
+  constexpr int PER = kMmaKeys * CH / kMmaThreads;                // 16-byte chunks of K (and of V) per thread
   extern __shared__ __align__(16) float sm[];
-  float* sq = sm;                                         // [64][PITCH]
-  float* ring = sq + kMmaRows * PITCH;                    // [2][STAGE]
+  float* sq = sm;                                         // [ROWS][PITCH]
+  float* ring = sq + ROWS * PITCH;                    // [2][STAGE]
   __shared__ unsigned long long s_mask[kTreeMaxNodes];
   __shared__ unsigned s_used[2];
   __shared__ int s_dmax, s_fix;
   __shared__ unsigned s_odd[2];                           // per stage: keys that were cleared
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) % RW, kw = (tid >> 5) / RW;
+  const int g = lane >> 2, t = lane & 3;
   const int sp = blockIdx.x, h = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles, b = blockIdx.z;
   const float ninf = __int_as_float(0xff800000);
   pdl_wait();
   pdl_trigger();
   const int64_t len = p.seqlen[b];
   const int cb = p.row_map != nullptr ? p.row_map[b] : b;
-  const int rows = p.N * p.G, r0 = rt * kMmaRows;
+  const int rows = p.N * p.G, r0 = rt * ROWS;
   const uint64_t per_g = (1ull << 32) / (unsigned)p.G + 1;  // row / G by a multiplication, exact while row x G < 2^32
   // q rows, zero past the last one; a thread's loads in flight together
+  constexpr int QN = ROWS * CH / kMmaThreads, QU = QN < 8 ? QN : 8;
 #pragma unroll 1
-  for (int e0 = 0; e0 < kMmaRows * CH / 128; e0 += 8) {
-    uint4 v[8];
+  for (int e0 = 0; e0 < QN; e0 += QU) {
+    uint4 v[QU];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = tid + 128 * (e0 + e), gr = r0 + c / CH;
+    for (int e = 0; e < QU; ++e) {
+      const int c = tid + kMmaThreads * (e0 + e), gr = r0 + c / CH;
       v[e] = make_uint4(0u, 0u, 0u, 0u);
       if (gr < rows) {
         const int i = (int)((uint64_t)(unsigned)gr * per_g >> 32), qg = gr - i * p.G;
@@ -149,16 +161,20 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = tid + 128 * (e0 + e);
+    for (int e = 0; e < QU; ++e) {
+      const int c = tid + kMmaThreads * (e0 + e);
       float f[EPC];
       widen_u4<XT>(v[e], f);
+      if constexpr (XT == kF32) {
+#pragma unroll
+        for (int u = 0; u < EPC; ++u) f[u] = __uint_as_float(cut_huge(__float_as_uint(f[u])));
+      }
 #pragma unroll
       for (int u = 0; u < EPC; u += 4)
         *reinterpret_cast<float4*>(&sq[c / CH * PITCH + c % CH * EPC + u]) = make_float4(f[u], f[u + 1], f[u + 2], f[u + 3]);
     }
   }
-  if (warp == 0) {
+  if (tid < 32) {
     const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
     unsigned long long used = 0;
     int dm = 0;
@@ -195,7 +211,7 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
     float* st = ring + stage * STAGE;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const int c = tid + 128 * e, r = c / CH, cc = c % CH * EPC;
+      const int c = tid + kMmaThreads * e, r = c / CH, cc = c % CH * EPC;
       const int64_t at = ((int64_t)(t0 + r) * D + cc) * es;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
@@ -220,7 +236,7 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
     uint32_t any = 0;
 #pragma unroll
     for (int e = 0; e < 2 * PER; ++e) {
-      const int c = tid + 128 * (e >> 1), r = c / CH, cc = c % CH * EPC;
+      const int c = tid + kMmaThreads * (e >> 1), r = c / CH, cc = c % CH * EPC;
 #pragma unroll
       for (int u = 0; u < EPC; u += 4) {
         const uint4 x = *reinterpret_cast<const uint4*>(st + (e & 1) * kMmaKeys * PITCH + r * PITCH + cc + u);
@@ -230,10 +246,14 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
     if (!any) return;
 #pragma unroll 1
     for (int e = 0; e < 2 * PER; ++e) {  // rare
-      const int c = tid + 128 * (e >> 1), r = c / CH, cc = c % CH * EPC;
+      const int c = tid + kMmaThreads * (e >> 1), r = c / CH, cc = c % CH * EPC;
       for (int u = 0; u < EPC; ++u) {
         uint32_t* x = reinterpret_cast<uint32_t*>(st + (e & 1) * kMmaKeys * PITCH + r * PITCH + cc + u);
-        if (!(e & 1 ? odd_f32(*x) : huge_f32(*x))) continue;
+        if (!huge_f32(*x)) continue;
+        if ((e & 1) && !odd_f32(*x)) {
+          *x = cut_huge(*x);
+          continue;
+        }
         *x = 0u;
         if (e & 1) s_fix = 1;
         else atomicOr(&s_odd[stage], 1u << r);
@@ -276,51 +296,62 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
     const float* sk = ring + stage * STAGE;
     const float* sv = sk + kMmaKeys * PITCH;
     if (!idle) {
-      float s[4][4] = {};  // 16 rows x 32 keys: block j, keys 8 j + 2 t, + 1 of rows g (0, 1) and g + 8 (2, 3)
-      const float* b_at = sk + ((lane & 7) + (lane >> 4) * 8) * PITCH + (lane >> 3 & 1) * 4;
+      // 16 rows x 8 JW keys: block j, keys 8 j + 2 t, + 1 of rows g (0, 1) and g + 8 (2, 3)
+      float s[JW][4] = {};
+      const float* b_at = JW == 1 ? sk + (8 * kw + (lane & 7)) * PITCH + (lane >> 3) * 4
+                                  : sk + (8 * JW * kw + (lane & 7) + (lane >> 4) * 8) * PITCH + (lane >> 3 & 1) * 4;
 #pragma unroll 2
       for (int k4 = 0; k4 < D / 8; k4 += 4) {
-        float fresh[4][4] = {};
-        float(&part)[4][4] = XT == kBF16 ? s : fresh;
+        float fresh[JW][4] = {};
+        float(&part)[JW][4] = XT == kBF16 ? s : fresh;
+        uint32_t y[4];
 #pragma unroll
         for (int kk = k4; kk < k4 + 4; ++kk) {
-          uint32_t a[4], ah[4], al[4];
+          uint32_t a[4], ah[4], al[4], yh[JW][2], yl[JW][2];
           ldsm4(a_at + 8 * kk, a);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) split_tf32<true>(a[i], ah[i], al[i]);
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (XT == kBF16) ah[i] = a[i];
+            else split_tf32<true>(a[i], ah[i], al[i]);
+          }
+          auto part_of = [&](int j, int i, uint32_t x) {
+            if constexpr (XT == kBF16) yh[j][i] = x;
+            else split_tf32<false>(x, yh[j][i], yl[j][i]);
+          };
+          if constexpr (JW == 1) {
+            if (!(kk & 1)) ldsm4(b_at + 8 * kk, y);  // eight keys, two steps
+            part_of(0, 0, y[2 * (kk & 1)]);
+            part_of(0, 1, y[2 * (kk & 1) + 1]);
+          } else {
 #pragma unroll
-          for (int j = 0; j < 4; j += 2) {
-            uint32_t y[4];
-            ldsm4(b_at + 8 * j * PITCH + 8 * kk, y);
-            if constexpr (XT == kBF16) {
-              mma_tf32(part[j], a, y[0], y[1]);
-              mma_tf32(part[j + 1], a, y[2], y[3]);
-            } else {
-              uint32_t yh[4], yl[4];
+            for (int j = 0; j < JW; j += 2) {
+              ldsm4(b_at + 8 * j * PITCH + 8 * kk, y);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) split_tf32<false>(y[i], yh[i], yl[i]);
-              mma_tf32(part[j], al, yh[0], yh[1]);
-              mma_tf32(part[j + 1], al, yh[2], yh[3]);
-              mma_tf32(part[j], ah, yl[0], yl[1]);
-              mma_tf32(part[j + 1], ah, yl[2], yl[3]);
-              mma_tf32(part[j], ah, yh[0], yh[1]);
-              mma_tf32(part[j + 1], ah, yh[2], yh[3]);
+              for (int i = 0; i < 4; ++i) part_of(j + i / 2, i & 1, y[i]);
             }
           }
+          if constexpr (XT != kBF16) {
+#pragma unroll
+            for (int j = 0; j < JW; ++j) mma_tf32(part[j], al, yh[j][0], yh[j][1]);
+#pragma unroll
+            for (int j = 0; j < JW; ++j) mma_tf32(part[j], ah, yl[j][0], yl[j][1]);
+          }
+#pragma unroll
+          for (int j = 0; j < JW; ++j) mma_tf32(part[j], ah, yh[j][0], yh[j][1]);
         }
         if constexpr (XT != kBF16) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < JW; ++j)
 #pragma unroll
             for (int c = 0; c < 4; ++c) s[j][c] += fresh[j][c];
         }
       }
       if (const unsigned odd = s_odd[stage]; odd) {  // rare: keys with a NaN or an infinity, from the cache
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < JW; ++j)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int key = 8 * j + 2 * t + (c & 1);
+            const int key = 8 * (JW * kw + j) + 2 * t + (c & 1);
             if (!((odd >> key) & 1u)) continue;
             float x = 0.0f;
             const float* qr = sq + (warp * 16 + g + (c >> 1) * 8) * PITCH;
@@ -335,11 +366,11 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
       for (int a = 0; a < 2; ++a) {
         float mt = m[a];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < JW; ++j)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float& x = s[j][2 * a + c];
-            x = mixed && !sees(a, t0 + 8 * j + 2 * t + c) ? ninf : x * p.scale;
+            x = mixed && !sees(a, t0 + 8 * (JW * kw + j) + 2 * t + c) ? ninf : x * p.scale;
             mt = fmaxf(mt, x);
           }
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
@@ -347,7 +378,7 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
         const float base = mt == ninf ? 0.0f : mt;
         float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < JW; ++j)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float& x = s[j][2 * a + c];
@@ -366,44 +397,84 @@ __global__ void __launch_bounds__(128) tree_mma_kernel(TreeAttnParams p, int row
 #pragma unroll
           for (int c = 0; c < 4; ++c) acc[j][c] *= fix[c >> 1];
       }
-      uint32_t ah[4][4], al[4][4];
+      uint32_t ah[JW][4], al[JW][4];
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
+      for (int kk = 0; kk < JW; ++kk) {
         const int order[4] = {0, 2, 1, 3};
 #pragma unroll
         for (int i = 0; i < 4; ++i) split_tf32<false>(__float_as_uint(s[kk][order[i]]), ah[kk][i], al[kk][i]);
       }
-      const float* v_at = sv + 2 * t * PITCH + g;
+      const float* v_at = sv + (8 * JW * kw + 2 * t) * PITCH + g;
 #pragma unroll
-      for (int j = 0; j < D / 8; ++j) {
-        float fresh[4] = {};
-        float(&part)[4] = XT == kBF16 ? acc[j] : fresh;
+      for (int j0 = 0; j0 < D / 8; j0 += JG) {
+        float part[JG][4];
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const uint32_t y0 = __float_as_uint(v_at[8 * kk * PITCH + 8 * j]);
-          const uint32_t y1 = __float_as_uint(v_at[(8 * kk + 1) * PITCH + 8 * j]);
-          if constexpr (XT == kBF16) {
-            mma_tf32(part, al[kk], y0, y1);
-            mma_tf32(part, ah[kk], y0, y1);
-          } else {
-            uint32_t h0, l0, h1, l1;
-            split_tf32<true>(y0, h0, l0);
-            split_tf32<true>(y1, h1, l1);
-            mma_tf32(part, al[kk], h0, h1);
-            mma_tf32(part, ah[kk], l0, l1);
-            mma_tf32(part, ah[kk], h0, h1);
+        for (int j = 0; j < JG; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) part[j][c] = XT == kBF16 ? acc[j0 + j][c] : 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < JW; ++kk) {
+          uint32_t yh[JG][2], yl[JG][2];
+#pragma unroll
+          for (int j = 0; j < JG; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t y = __float_as_uint(v_at[(8 * kk + u) * PITCH + 8 * (j0 + j)]);
+              if constexpr (XT == kBF16) yh[j][u] = y;
+              else split_tf32<true>(y, yh[j][u], yl[j][u]);
+            }
+#pragma unroll
+          for (int j = 0; j < JG; ++j) mma_tf32(part[j], al[kk], yh[j][0], yh[j][1]);
+          if constexpr (XT != kBF16) {
+#pragma unroll
+            for (int j = 0; j < JG; ++j) mma_tf32(part[j], ah[kk], yl[j][0], yl[j][1]);
           }
-        }
-        if constexpr (XT != kBF16) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) acc[j][c] += fresh[c];
+          for (int j = 0; j < JG; ++j) mma_tf32(part[j], ah[kk], yh[j][0], yh[j][1]);
         }
+#pragma unroll
+        for (int j = 0; j < JG; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[j0 + j][c] = XT == kBF16 ? part[j][c] : acc[j0 + j][c] + part[j][c];
       }
     }
     __syncthreads();  // the stage may be written again
     if (tid == 0) s_odd[stage] = 0;
   }
-  if (s_fix && !idle) {  // rare: what was cleared from V, to the rows that see it
+  // the groups' parts of each row, in their order
+  float* join = ring;  // [KW - 1][RW][D / 2 + 4][32]
+  if (kw > 0 && !idle) {
+    float* at = join + ((kw - 1) * RW + warp) * (D / 2 + 4) * 32 + lane;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) at[(4 * j + c) * 32] = acc[j][c];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      at[(D / 2 + a) * 32] = m[a];
+      at[(D / 2 + 2 + a) * 32] = l[a];
+    }
+  }
+  __syncthreads();
+  if (kw > 0 || idle) return;
+#pragma unroll 1
+  for (int k = 0; k < KW - 1; ++k) {
+    const float* at = join + (k * RW + warp) * (D / 2 + 4) * 32 + lane;
+    float w0[2], w1[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const float mo = at[(D / 2 + a) * 32], mt = fmaxf(m[a], mo), base = mt == ninf ? 0.0f : mt;
+      w0[a] = mexp(m[a] - base);
+      w1[a] = mexp(mo - base);
+      l[a] = l[a] * w0[a] + at[(D / 2 + 2 + a) * 32] * w1[a];
+      m[a] = mt;
+    }
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[j][c] = acc[j][c] * w0[c >> 1] + at[(4 * j + c) * 32] * w1[c >> 1];
+  }
+  if (s_fix) {  // rare: what was cleared from V, to the rows that see it
     for (int key = k0; key < k1; ++key) {
       const bool v0 = sees(0, key), v1 = sees(1, key);
 #pragma unroll
@@ -577,12 +648,16 @@ __global__ void __launch_bounds__(256) commit_kernel(const __grid_constant__ Com
 }
 
 // How many splits a row's keys are cut into: as many as the resident CTAs
-// (three, two or one per SM) take at once, no more than the join can hold.
+// (two or one per SM) take at once, no more than the join can hold.
 inline int tree_mma_splits(int64_t ctas, int64_t max_len, int64_t head_dim) {
-  const int64_t want = (head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1) * 148 / ctas, most = (max_len + kMmaKeys - 1) / kMmaKeys;
+  const int64_t want = (head_dim == 256 ? 1 : 2) * 148 / ctas, most = (max_len + kMmaKeys - 1) / kMmaKeys;
   const int64_t ns = want < most ? want : most;
   return (int)(ns < 1 ? 1 : ns > kTreeMaxSplits ? kTreeMaxSplits : ns);
 }
+// Rows per CTA: 32 with four groups of warps on a tile's keys, or 64 with two.
+// Four rows, 16 x 1500 fp32 with heads of 128: 72 us with 32, 105 with 64; more
+// rows than 32 would read each key again: 512 rows, 8 x 4000, 1219 us and 975.
+inline int tree_mma_rows(int64_t rows) { return rows <= 32 ? 32 : 64; }
 
 inline bool tree_use_tc(int x_dtype, int64_t head_dim) {
   return x_dtype == kBF16 && (head_dim == 64 || head_dim == 128);
@@ -593,7 +668,7 @@ inline int tree_splits(int64_t batch, int64_t nodes, int64_t num_heads, int64_t 
   if (window > 0 && window + nodes < max_len) max_len = window + nodes;  // no row's keys span more
   if (tree_use_tc(x_dtype, head_dim))
     return tree_tc_splits(batch * num_kv_heads * tree_tc_groups(nodes * (num_heads / num_kv_heads)), max_len);
-  const int64_t tiles = (nodes * (num_heads / num_kv_heads) + kMmaRows - 1) / kMmaRows;
+  const int64_t rows = nodes * (num_heads / num_kv_heads), per = tree_mma_rows(rows), tiles = (rows + per - 1) / per;
   return tree_mma_splits(batch * num_kv_heads * tiles, max_len, head_dim);
 }
 
@@ -659,7 +734,7 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   p.G = (int)(num_heads / num_kv_heads); p.Bc = (int)cache_batch; p.T = (int)max_len;
   p.window = (int)(window > max_len ? 0 : window);  // a window past the cache hides nothing
   p.scale = scale;
-  const int64_t rows = (int64_t)p.N * p.G, tiles = (rows + kMmaRows - 1) / kMmaRows;
+  const int64_t rows = (int64_t)p.N * p.G, per = tree_mma_rows(rows), tiles = (rows + per - 1) / per;
   if (num_kv_heads * tiles > 65535) return kErrShape;
   p.NS = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim, window);
   const int64_t prows = tree_partial_rows(rows, x_dtype, head_dim);
@@ -669,14 +744,19 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   p.ws_ml = p.ws_acc ? p.ws_acc + batch * num_kv_heads * prows * p.NS * head_dim : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
+#define MB_TREE_MMA(XT, DD, RW)                                                                             \
+  do {                                                                                                      \
+    const size_t smem = (size_t)(16 * RW + 4 * kMmaKeys) * (DD + 4) * 4;                                     \
+    static std::atomic<uint64_t> done{0};                                                                   \
+    e = smem_once(done, tree_mma_kernel<XT, DD, RW>, (int)smem);                                            \
+    if (e == cudaSuccess)                                                                                   \
+      e = launch_k(tree_mma_kernel<XT, DD, RW>,                                                             \
+                   dim3((unsigned)p.NS, (unsigned)(num_kv_heads * tiles), (unsigned)batch), dim3(kMmaThreads), \
+                   smem, st, p, (int)tiles);                                                                \
+  } while (0)
 #define MB_TREE(XT, DD)                                                                                              \
   do {                                                                                                               \
-    const size_t smem = (size_t)(kMmaRows + 4 * kMmaKeys) * (DD + 4) * 4; \
-    static std::atomic<uint64_t> done{0};                                                                            \
-    e = smem_once(done, tree_mma_kernel<XT, DD>, (int)smem);                                                        \
-    if (e == cudaSuccess)                                                                                            \
-      e = launch_k(tree_mma_kernel<XT, DD>, dim3((unsigned)p.NS, (unsigned)(num_kv_heads * tiles), (unsigned)batch), \
-                   dim3(128), smem, st, p, (int)tiles);                                                              \
+    if (per == 32) MB_TREE_MMA(XT, DD, 2); else MB_TREE_MMA(XT, DD, 4);                                              \
     if (e == cudaSuccess && p.NS > 1)                                                                                \
       e = launch_k(tree_merge_kernel<XT, DD>,                                                                        \
                    dim3((unsigned)((num_kv_heads * rows + 7) / 8), (unsigned)batch), dim3(256), 0, st, p, kMmaKeys); \
@@ -690,6 +770,7 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
     if (head_dim == 64) MB_TREE(kF32, 64); else if (head_dim == 128) MB_TREE(kF32, 128); else MB_TREE(kF32, 256);
   }
 #undef MB_TREE
+#undef MB_TREE_MMA
   return e == cudaSuccess ? kOk : kErrCuda;
 }
 
