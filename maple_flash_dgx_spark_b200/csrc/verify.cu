@@ -17,6 +17,7 @@
 // Comparisons with a uniform decide which token comes out, so everything after
 // the selection (at most 64 values per node) is held in 64 bits.
 #include <cooperative_groups.h>
+#include <utility>
 
 #include "bulk.cuh"
 #include "common.cuh"
@@ -456,8 +457,10 @@ __global__ void __launch_bounds__(kVerWalkThreads) verify_walk_kernel(VerifyPara
   const cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, group = tid / kVerCap, gt = tid % kVerCap;
   const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks(), b = (int)(blockIdx.x / ranks);
+  auto here = cluster.barrier_arrive();  // every CTA has begun before one writes to another's shared memory
   pdl_wait();
   pdl_trigger();
+  cluster.barrier_wait(std::move(here));
   const int64_t base = (int64_t)b * p.N;
   for (int n = rank * kVerGroups + group; n < p.N; n += ranks * kVerGroups) {
     const int parent = p.parents[base + n];
