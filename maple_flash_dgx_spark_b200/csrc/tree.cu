@@ -15,7 +15,7 @@ namespace mb {
 // mask holds its ancestors within 2^r steps and `up` points 2^r steps up, so
 // six rounds cover 64 nodes.  One warp per sequence, nodes `lane` and
 // `lane + 32` in registers: no shared memory, no barrier; the 16 bytes per
-// node make the launch itself the bound (latency).
+// node make the launch itself the bound: 1.5 us for 1 x 8, 1.6 for 256 x 64.
 __global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, int64_t sb, int64_t sn, int B, int N,
                                                         unsigned long long* mask, int32_t* depth, int* err) {
   const int lane = threadIdx.x & 31, b = blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -522,7 +522,8 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
 
 // Joins the splits of each row: M = max m_j, out = sum e^(m_j - M) acc_j / sum
 // e^(m_j - M) l_j, in split order.  A warp per row, its lanes the dimensions;
-// the partials were just written and come from L2.
+// the partials were just written and come from L2.  7 us cold for 4 x 272 rows of
+// 64 in 12 splits, bound by latency.
 template <int XT, int D>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeAttnParams p, int tile) {
   constexpr int U = D / 32;
@@ -593,7 +594,9 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeAttnParams p, int t
 // every layer's K and V in one launch.  path rises (path[d] >= d), so one
 // thread that walks d upwards with its own 16-byte column may move in place:
 // what it overwrites at d it has read already.  Batches of eight loads keep the
-// column's reads in flight; bound by latency at the sizes of a draft.
+// column's reads in flight.  Bound by latency at the sizes of a draft: 48 layers
+// of 4 heads of 128, one sequence 2.3 us, 16 with up to 32 nodes 3.9 us for up
+// to 10.4 MB (2.7 TB/s); a launch alone takes 1.5.
 constexpr int kCommitLayers = 128;
 
 struct CommitParams {
@@ -666,9 +669,10 @@ inline bool tree_use_tc(int x_dtype, int64_t head_dim) {
 inline int tree_splits(int64_t batch, int64_t nodes, int64_t num_heads, int64_t num_kv_heads, int64_t max_len,
                        int x_dtype, int64_t head_dim, int64_t window) {
   if (window > 0 && window + nodes < max_len) max_len = window + nodes;  // no row's keys span more
+  const int64_t rows = nodes * (num_heads / num_kv_heads);
   if (tree_use_tc(x_dtype, head_dim))
-    return tree_tc_splits(batch * num_kv_heads * tree_tc_groups(nodes * (num_heads / num_kv_heads)), max_len);
-  const int64_t rows = nodes * (num_heads / num_kv_heads), per = tree_mma_rows(rows), tiles = (rows + per - 1) / per;
+    return tree_tc_splits(batch * num_kv_heads * tree_tc_groups(rows), max_len, rows > tree_tc_partial_rows(1));
+  const int64_t per = tree_mma_rows(rows), tiles = (rows + per - 1) / per;
   return tree_mma_splits(batch * num_kv_heads * tiles, max_len, head_dim);
 }
 

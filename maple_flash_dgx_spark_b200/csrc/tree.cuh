@@ -98,7 +98,7 @@ __device__ __forceinline__ int tree_splits_used(int lo, int hi, int tile, int ns
 }
 
 // tree_tc.cu: the tcgen05 kernel (bf16, heads of 64 or 128).
-int tree_tc_splits(int64_t ctas, int64_t max_len);
+int tree_tc_splits(int64_t ctas, int64_t max_len, bool pair);  // pair: two row tiles per CTA
 int tree_tc_groups(int64_t rows);
 int64_t tree_tc_partial_rows(int64_t rows);  // rows that a split's partials take
 cudaError_t tree_tc_launch(const TreeAttnParams& p, int D, cudaStream_t st);

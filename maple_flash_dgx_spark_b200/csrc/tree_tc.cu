@@ -28,6 +28,15 @@
 // NaN), and where a visible one was cleared the item's end adds it back to the
 // rows that see it.
 //
+// Up to 128 rows HBM bounds it: 64 sequences x 8150 with eight nodes (32 heads
+// on 4 of 128), 1.08 GB in 164 us = 6.57 TB/s, what a plain copy reaches; held
+// for seconds the power limit makes it 181.  With more rows the softmax does:
+// 64 nodes x 65440, 68.7 GFLOP in 72 us = 950 TFLOP/s; a warpgroup's loads from
+// tensor memory, exponentials (a thread's 128 per unit at 16 per cycle and SM
+// for four warps) and stores take longer than its two MMAs.  Exponentials by a
+// polynomial on the FMA pipes gave 280 to 316 us for 273 (37 x 8192, 64 nodes),
+// units of 64 keys with their scores a unit ahead 320.
+//
 // Waits are bounded: one that gives up sets the error word; every role then
 // leaves, waits (bounded) for its copies and MMAs in flight, frees the tensor
 // memory and returns.  Loads read this GPU's own memory, without multicast.
@@ -638,7 +647,9 @@ __global__ void __launch_bounds__(kTtThreads, 1)
 
 // Joins the splits: M = max m_j, out = sum e^(m_j - M) acc_j / sum e^(m_j - M)
 // l_j, in split order.  A CTA takes 32 rows (the lanes, as the partials lie) x
-// 32 dims (four per warp); eight splits' loads are in flight at a time.
+// 32 dims (four per warp); eight splits' loads are in flight at a time.  Bound
+// by latency: 13 us for 18 splits of 4 x 512 rows with nothing in L2, where the
+// partials are when they are read.
 template <int D>
 __global__ void __launch_bounds__(256) tree_tc_merge_kernel(TreeAttnParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -704,19 +715,32 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(TreeAttnParams p) {
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (((int64_t)b * p.N + node) * p.H + h * p.G + g) * D + col) = out;
 }
 
-// Splits of a sequence's keys.  Few items leave SMs idle, more splits cost a
-// join: time in key tiles (1.4 us each at 44 GB/s per SM) ~ waves x (tiles per
-// split + 4 of start and end), + 6 for the join's launch, + the partials'
-// traffic (a split writes and reads 128 KB per 128 rows: 2 tiles' worth).
-int tree_tc_splits(int64_t ctas, int64_t max_len) {
+// Splits of a sequence's keys: the number with the least expected time.  A key
+// tile takes 0.95 us while few SMs read (1.9 with two row tiles), 1.4 when all
+// share the HBM; an item 4 us to start and end, a launch 3, the join's 4 and
+// 0.19 per split that it walks through, an item's partials 0.02 per 128 rows.
+// Measured (8 nodes, 8 heads per KV head; in brackets what the rule takes), us:
+//   splits               1     2     3     5     9    18    37
+//   1 x 600   [1]     12.3  12.4  11.6  11.2  (and a second launch on the host)
+//   1 x 8192  [13]    67.5  40.3  30.4  22.9  18.8  16.7  19.7
+//   4 x 4000  [6]     37.4  25.9  20.9  18.0  17.0  22.2  33.7
+//   16 x 8192 [2]     70.0  55.0  71.3  73.1  67.9  89.8   135
+//   37 x 4096 [1]     55.0  71.7  75.5  81.5   103   157   249
+//   1 x 65440, 64 nodes [18]  941   479   327   204   122  74.8  87.8
+int tree_tc_splits(int64_t ctas, int64_t max_len, bool pair) {
   const int64_t tiles = (max_len + kTtKeys - 1) / kTtKeys;
   int64_t best = 1;
-  double cost = 1e30;
+  double least = 1e30;
   for (int64_t ns = 1; ns <= kTreeMaxSplits && ns <= tiles; ++ns) {
-    const int64_t waves = (ctas * ns + 147) / 148, per = (tiles + ns - 1) / ns;
-    const double t = (double)waves * ((double)per + 4.0 + (ns > 1 ? 2.0 : 0.0)) + (ns > 1 ? 6.0 : 0.0);
-    if (t < cost) {
-      cost = t;
+    const int64_t items = ctas * ns, per = (tiles + ns - 1) / ns;
+    auto wave = [&](int64_t n) {  // n items side by side
+      const double alone = pair ? 1.9 : 0.95, shared = 1.4 / 148 * (double)n;
+      return n == 0 ? 0.0 : (double)per * (alone > shared ? alone : shared) + 4.0;
+    };
+    double t = (double)(items / 148) * wave(148) + wave(items % 148) + 3.0;
+    if (ns > 1) t += 4.0 + 0.19 * (double)ns + (pair ? 0.04 : 0.02) * (double)items;
+    if (t < least) {
+      least = t;
       best = ns;
     }
   }

@@ -94,8 +94,10 @@ __device__ __forceinline__ void warp_prefix_d(const double (&a)[2], double (&c)[
 // ids.  -inf and NaN are not handed on: they have no weight, and a row of
 // nothing else is known by having no candidates.  Five CTAs per SM: their loads
 // cover each other's search for T, and their tiles stay in L1 for the second
-// look (read past L1 it cost 13 of 38 us at K = 50; a ring of tiles in shared memory with two
-// CTAs per SM measured slower, 45 against 40 us for 64 x 8 rows of 151936).
+// look.  64 x 8 rows of 151936 bf16 at K = 50: 33 us, 4.7 TB/s, 25 without the
+// second look; past L1 it took 37, with each thread looking at its own vectors
+// instead of the CTA's put together 37 as well, from a ring of tiles in shared
+// memory with two CTAs per SM 45.  16 x 24 rows at K = 20: 25 us.
 // One word whose order is larger logit, then lower id.
 __device__ __forceinline__ unsigned long long cand_word(const uint2& v) {
   return (unsigned long long)v.x << 32 | (0xffffffffu - v.y);
@@ -323,8 +325,9 @@ __global__ void __launch_bounds__(kVerThreads, 5) verify_tile_kernel(VerifyParam
 // them, into the shared memory of the cluster's first CTA, where one warp then
 // walks with nothing left to fetch.  Bound by latency, so the work is spread: a
 // thread per candidate of a tile (kVerCap = 128 of them), and per kept one that
-// counts what stands before it.  With one warp per node the same took 15 us
-// more (64 x 8, 50 kept of 590 candidates).
+// counts what stands before it.  64 x 8, 50 kept of 600 candidates: 13 us, of
+// which the candidates take 3, their limit and order 3.5, weights and draft 1,
+// the cluster 1 and the walk down eight nodes 3.5; with one warp per node 28.
 constexpr int kVerBuf = 1024;                 // candidates of a node held at a time
 constexpr int kVerRank = kVerCap;             // of which at most so many are put in order by counting
 constexpr int kVerWalkThreads = 512;
