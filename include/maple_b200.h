@@ -482,7 +482,8 @@ int maple_tree_plan(const int32_t* parents, int64_t batch, int64_t nodes, int64_
  * q [batch, nodes, H, D] with D contiguous (element strides q_sb, q_sn, q_sh),
  * out [batch, nodes, H, D] contiguous; caches [cache_batch, Hkv, max_len, D],
  * (max_len, D) contiguous, cache row row_map[b] (b when NULL).  f32 or bf16,
- * D in {64, 128, 256}; pointers and strides multiples of 16 bytes.  With nodes
+ * D in {64, 128, 256}, H / Hkv at most 4096; pointers and strides multiples of
+ * 16 bytes.  With nodes
  * = 1 and mask 1 this is maple_decode_gqa_attn.  A length or cache row outside
  * the cache sets bit 2 of *err (that sequence gets zeros); a bounded wait that
  * gives up sets bit 1.  A row's result depends on no other sequence's length

@@ -703,7 +703,7 @@ extern "C" int64_t maple_tree_gqa_workspace_bytes(int64_t batch, int64_t nodes, 
                                                   int64_t num_kv_heads, int64_t head_dim, int64_t max_len,
                                                   int64_t window, int x_dtype) {
   if (batch <= 0 || nodes <= 0 || nodes > kTreeMaxNodes || num_heads <= 0 || num_kv_heads <= 0 ||
-      num_heads % num_kv_heads || head_dim <= 0 || max_len <= 0 || window < 0)
+      num_heads % num_kv_heads || num_heads / num_kv_heads > kTreeMaxGroup || head_dim <= 0 || max_len <= 0 || window < 0)
     return -1;
   const int64_t ns = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim, window);
   const int64_t rows = tree_partial_rows(nodes * (num_heads / num_kv_heads), x_dtype, head_dim);
@@ -722,6 +722,7 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   if (batch == 0) return kOk;
   if (x_dtype != kF32 && x_dtype != kBF16) return kErrDtype;
   if (num_heads % num_kv_heads != 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return kErrShape;
+  if (num_heads / num_kv_heads > kTreeMaxGroup) return kErrShape;
   if (!q || !k_cache || !v_cache || !seqlen || !tree_mask || !out || !err || batch > 65535 || cache_batch < 1 ||
       num_heads > 65535 || max_len > (1LL << 30) || cache_batch > (1LL << 30))
     return kErrShape;

@@ -38,6 +38,7 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
 }
 constexpr int kTreeMaxNodes = 64;
 constexpr int kTreeMaxSplits = 64;
+constexpr int kTreeMaxGroup = 4096;  // query heads per KV head: (row of 64 nodes) x group stays below 2^32
 
 struct TreeAttnParams {
   const void* q;              // [B, N, H, D], D contiguous
