@@ -527,7 +527,7 @@ int maple_verify_tree(const void* logits, int x_dtype, int64_t batch, int64_t no
  * pointers to [cache_batch, Hkv, max_len, D] caches of one geometry, 16-byte
  * aligned.  A path that does not rise, or a slot or cache row outside the
  * cache, moves nothing of that sequence and sets bit 2 of *err.  Two sequences
- * on one cache row are not ordered. */
+ * on one cache row, or two pointers to one cache, are not ordered. */
 int maple_commit_tree(void* const* k_caches, void* const* v_caches, int64_t layers, int x_dtype, int64_t batch,
                       int64_t nodes, int64_t cache_batch, int64_t num_kv_heads, int64_t cache_sb, int64_t cache_sh,
                       int64_t max_len, int64_t head_dim, const int64_t* seqlen, const int32_t* path,

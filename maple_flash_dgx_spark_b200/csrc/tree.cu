@@ -790,6 +790,7 @@ extern "C" int maple_commit_tree(void* const* k_caches, void* const* v_caches, i
   if (layers == 0 || batch == 0) return kOk;
   if (x_dtype != kF32 && x_dtype != kBF16) return kErrDtype;
   if (!k_caches || !v_caches || !seqlen || !path || !n_path || !err || cache_batch < 1) return kErrShape;
+  if ((num_kv_heads > 1 && cache_sh == 0) || (cache_batch > 1 && cache_sb == 0)) return kErrShape;  // shared rows
   const int64_t epu = x_dtype == kBF16 ? 8 : 4;  // elements per 16 bytes
   if (head_dim % epu || cache_sb % epu || cache_sh % epu) return kErrAlign;
   for (int64_t i = 0; i < layers; ++i) {

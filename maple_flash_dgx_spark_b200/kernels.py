@@ -1164,6 +1164,10 @@ class CacheRows:
                                  f"{tuple(first.shape)}.")
             if t.dtype != first.dtype:
                 raise TypeError(f"{op}: caches of {first.dtype} and {t.dtype}.")
+        # rows are moved in place, so none may be another's: nor one tensor's twice (expanded), nor two tensors'
+        if any(n > 1 and s < first.shape[2] * first.shape[3] for n, s in zip(first.shape[:2], first.stride()[:2])) or \
+                len({t.data_ptr() for t in k + v}) < len(k + v):
+            raise ValueError(f"{op}: the caches' rows overlap.")
         self.k, self.v = k, v
         self.shape = tuple(int(x) for x in first.shape)
         self.strides = first.stride()
@@ -1175,7 +1179,7 @@ def commit_tree(rows: CacheRows, seqlen, path, n_path, *, row_map=None) -> None:
     """Keep the accepted nodes' K/V rows, in every layer and in place: slot
     ``seqlen[b] + d`` takes slot ``seqlen[b] + path[b, d]`` for ``d <
     n_path[b]`` (``path`` / ``n_path`` as :func:`verify_tree` returns them).
-    ``seqlen`` is not advanced."""
+    ``seqlen`` is not advanced.  The sequences' cache rows differ."""
     op = "commit_tree"
     d = rows.index
     if path.ndim != 2:

@@ -612,7 +612,7 @@ class MapleForCausalLM:
         ``verify_tree`` accepts.  The lengths stay as they are."""
         plan = parents if isinstance(parents, TreePlan) else tree_plan(parents)
         bsz, n = plan.mask.shape
-        if tuple(tokens.shape) != (bsz, n):
+        if bsz < 1 or tuple(tokens.shape) != (bsz, n):
             raise ValueError(f"forward_tree: tokens {tuple(tokens.shape)} and trees {(bsz, n)}.")
         first = 0 if cache.slot is None else cache.slot
         if first + bsz > (cache.batch if cache.slot is None else first + 1):

@@ -716,6 +716,11 @@ def test_commit_refusals(cuda, K):
         K.CacheRows([c[0], c[0][:1]], c)
     with pytest.raises(TypeError):
         K.CacheRows([c[0], c[1].half()], c)
+    for k, v in (([c[0]], [c[0]]), ([c[0], c[0]], [c[1], c[1].clone()]),
+                 ([c[0][:1].expand(2, 2, 30, 64)], [c[1][:1].expand(2, 2, 30, 64)]),
+                 ([c[0][:, :1].expand(2, 2, 30, 64)], [c[1][:, :1].expand(2, 2, 30, 64)])):
+        with pytest.raises(ValueError, match="overlap"):
+            K.CacheRows(k, v)
     h = K.CacheRows(c[:1], c[1:])
     path, n, s = (torch.zeros(3, 4, dtype=torch.int32, device=cuda), torch.ones(3, dtype=torch.int32, device=cuda),
                   torch.zeros(3, dtype=torch.int64, device=cuda))
@@ -896,6 +901,8 @@ def test_forward_tree_refusals(cuda):
     tok = torch.zeros(2, 3, dtype=torch.int64, device=cuda)
     with pytest.raises(ValueError):
         model.forward_tree(tok[:, :2], par, cache)
+    with pytest.raises(ValueError):
+        model.forward_tree(tok[:0], par[:0], cache)
     with pytest.raises(ValueError):
         model.forward_tree(tok.repeat(2, 1), par.repeat(2, 1), cache)
     cache.seen[1] = 14

@@ -104,7 +104,7 @@ def test_commit_refuses_before_any_launch(L):
 
     assert call(layers=0) == 0 and call(B=0) == 0
     for bad in (dict(layers=-1), dict(B=-1), dict(N=0), dict(N=65), dict(Hkv=0), dict(T=0), dict(D=0),
-                dict(ptrs=(256, 0))):
+                dict(ptrs=(256, 0)), dict(sb=0)):
         assert call(**bad) == 1, bad
     for name in ("seqlen", "path", "n_path", "err"):
         assert call(null=name) == 1, name
