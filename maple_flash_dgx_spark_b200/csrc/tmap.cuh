@@ -38,12 +38,31 @@ struct TmapKeyHash {
   }
 };
 
+// Encodes a map (a fraction of a microsecond); false if the driver refuses it.
+inline bool tmap_encode_bf16_4d(const void* base, int64_t d0, int64_t d1, int64_t d2, int64_t d3, int64_t s1,
+                                int64_t s2, int64_t s3, int b0, int b1, CUtensorMap* out) {
+  static const PFN_cuTensorMapEncodeTiled encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess;
+    return found ? reinterpret_cast<PFN_cuTensorMapEncodeTiled>(fn) : nullptr;
+  }();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2, (cuuint64_t)d3};
+  const cuuint64_t strides[3] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2, (cuuint64_t)s3 * 2};
+  const cuuint32_t box[4] = {(cuuint32_t)b0, (cuuint32_t)b1, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Encodes (or returns the cached) map; false if the driver refuses it.
 inline bool tmap_bf16_4d(const void* base, int64_t d0, int64_t d1, int64_t d2, int64_t d3, int64_t s1, int64_t s2,
                          int64_t s3, int b0, int b1, CUtensorMap* out) {
   static std::mutex mu;
   static std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> cache;
-  static PFN_cuTensorMapEncodeTiled encode = nullptr;
   TmapKey key{};
   key.addr = reinterpret_cast<uintptr_t>(base);
   key.d0 = d0; key.d1 = d1; key.d2 = d2; key.d3 = d3; key.s1 = s1; key.s2 = s2; key.s3 = s3;
@@ -54,23 +73,8 @@ inline bool tmap_bf16_4d(const void* base, int64_t d0, int64_t d1, int64_t d2, i
     *out = it->second;
     return true;
   }
-  if (encode == nullptr) {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess || fn == nullptr)
-      return false;
-    encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(fn);
-  }
-  const cuuint64_t dims[4] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2, (cuuint64_t)d3};
-  const cuuint64_t strides[3] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2, (cuuint64_t)s3 * 2};
-  const cuuint32_t box[4] = {(cuuint32_t)b0, (cuuint32_t)b1, 1, 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
   CUtensorMap m;
-  const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
-                            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return false;
+  if (!tmap_encode_bf16_4d(base, d0, d1, d2, d3, s1, s2, s3, b0, b1, &m)) return false;
   if (cache.size() > 4096) cache.clear();
   cache.emplace(key, m);
   *out = m;

@@ -773,8 +773,8 @@ cudaError_t tree_tc_launch(const TreeAttnParams& p, int D, cudaStream_t st) {
   CUtensorMap tmk, tmv;
   const int64_t heads = p.c_sh ? p.Hkv : 1, hs = p.c_sh ? p.c_sh : (int64_t)p.T * D;
   const int64_t caches = p.c_sb ? p.Bc : 1, bs = p.c_sb ? p.c_sb : hs * heads;
-  if (!tmap_bf16_4d(p.kc, D, p.T, heads, caches, D, hs, bs, 64, kTtKeys, &tmk) ||
-      !tmap_bf16_4d(p.vc, D, p.T, heads, caches, D, hs, bs, 64, kTtKeys, &tmv))
+  if (!tmap_encode_bf16_4d(p.kc, D, p.T, heads, caches, D, hs, bs, 64, kTtKeys, &tmk) ||
+      !tmap_encode_bf16_4d(p.vc, D, p.T, heads, caches, D, hs, bs, 64, kTtKeys, &tmv))
     return cudaErrorInvalidValue;
   const int rows = p.N * p.G, groups = tree_tc_groups(rows);
   const bool pair = rows > kTtRows;
