@@ -667,11 +667,12 @@ inline bool tree_use_tc(int x_dtype, int64_t head_dim) {
 }
 
 inline int tree_splits(int64_t batch, int64_t nodes, int64_t num_heads, int64_t num_kv_heads, int64_t max_len,
-                       int x_dtype, int64_t head_dim, int64_t window) {
+                       int x_dtype, int64_t head_dim, int64_t window, bool* join) {
+  *join = false;
   if (window > 0 && window + nodes < max_len) max_len = window + nodes;  // no row's keys span more
   const int64_t rows = nodes * (num_heads / num_kv_heads);
   if (tree_use_tc(x_dtype, head_dim))
-    return tree_tc_splits(batch * num_kv_heads * tree_tc_groups(rows), max_len, rows > tree_tc_partial_rows(1));
+    return tree_tc_splits(batch * num_kv_heads * tree_tc_groups(rows), max_len, rows > tree_tc_partial_rows(1), join);
   const int64_t per = tree_mma_rows(rows), tiles = (rows + per - 1) / per;
   return tree_mma_splits(batch * num_kv_heads * tiles, max_len, head_dim);
 }
@@ -680,8 +681,9 @@ inline int tree_splits(int64_t batch, int64_t nodes, int64_t num_heads, int64_t 
 inline int64_t tree_partial_rows(int64_t rows, int x_dtype, int64_t head_dim) {
   return tree_use_tc(x_dtype, head_dim) ? tree_tc_partial_rows(rows) : rows;
 }
-inline int64_t tree_partial_bytes(int64_t batch, int64_t num_kv_heads, int64_t rows, int64_t ns, int64_t head_dim) {
-  return ns <= 1 ? 0 : batch * num_kv_heads * rows * ns * (head_dim + 2) * 4;
+inline int64_t tree_partial_bytes(int64_t batch, int64_t num_kv_heads, int64_t rows, int64_t ns, bool join,
+                                  int64_t head_dim) {
+  return ns <= 1 || join ? 0 : batch * num_kv_heads * rows * ns * (head_dim + 2) * 4;
 }
 
 }  // namespace mb
@@ -705,9 +707,10 @@ extern "C" int64_t maple_tree_gqa_workspace_bytes(int64_t batch, int64_t nodes, 
   if (batch <= 0 || nodes <= 0 || nodes > kTreeMaxNodes || num_heads <= 0 || num_kv_heads <= 0 ||
       num_heads % num_kv_heads || num_heads / num_kv_heads > kTreeMaxGroup || head_dim <= 0 || max_len <= 0 || window < 0)
     return -1;
-  const int64_t ns = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim, window);
+  bool join;
+  const int64_t ns = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim, window, &join);
   const int64_t rows = tree_partial_rows(nodes * (num_heads / num_kv_heads), x_dtype, head_dim);
-  return tree_partial_bytes(batch, num_kv_heads, rows, ns, head_dim);
+  return tree_partial_bytes(batch, num_kv_heads, rows, ns, join, head_dim);
 }
 
 extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, int64_t nodes, int64_t num_heads,
@@ -741,9 +744,11 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   p.scale = scale;
   const int64_t rows = (int64_t)p.N * p.G, per = tree_mma_rows(rows), tiles = (rows + per - 1) / per;
   if (num_kv_heads * tiles > 65535) return kErrShape;
-  p.NS = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim, window);
+  bool join;
+  p.NS = tree_splits(batch, nodes, num_heads, num_kv_heads, max_len, x_dtype, head_dim, window, &join);
+  p.join = join;
   const int64_t prows = tree_partial_rows(rows, x_dtype, head_dim);
-  const int64_t need = tree_partial_bytes(batch, num_kv_heads, prows, p.NS, head_dim);
+  const int64_t need = tree_partial_bytes(batch, num_kv_heads, prows, p.NS, join, head_dim);
   if (need > 0 && (!workspace || workspace_bytes < need)) return kErrWorkspace;
   p.ws_acc = static_cast<float*>(workspace);
   p.ws_ml = p.ws_acc ? p.ws_acc + batch * num_kv_heads * prows * p.NS * head_dim : nullptr;

@@ -52,7 +52,7 @@ struct TreeAttnParams {
   float* ws_ml;               // maximum and sum of weights of each row and split
   int* err;
   int64_t q_sb, q_sn, q_sh, c_sb, c_sh;
-  int B, N, H, Hkv, G, Bc, T, NS, window;
+  int B, N, H, Hkv, G, Bc, T, NS, window, join;
   float scale;
 };
 
@@ -99,7 +99,8 @@ __device__ __forceinline__ int tree_splits_used(int lo, int hi, int tile, int ns
 }
 
 // tree_tc.cu: the tcgen05 kernel (bf16, heads of 64 or 128).
-int tree_tc_splits(int64_t ctas, int64_t max_len, bool pair);  // pair: two row tiles per CTA
+// pair: two row tiles per CTA; join: the splits are joined by their cluster, without partials in memory
+int tree_tc_splits(int64_t ctas, int64_t max_len, bool pair, bool* join);
 int tree_tc_groups(int64_t rows);
 int64_t tree_tc_partial_rows(int64_t rows);  // rows that a split's partials take
 cudaError_t tree_tc_launch(const TreeAttnParams& p, int D, cudaStream_t st);

@@ -23,7 +23,8 @@
 // then still fit fp32 and bf16 many times over).
 //
 // An item is one split of one sequence's keys for one KV head and row tile (or
-// pair).  A tile that some row sees only in part is masked in registers; its
+// pair).  With JOIN a CTA has one item, and the splits of a row tile form a
+// cluster, which joins their parts through its shared memory.  A tile that some row sees only in part is masked in registers; its
 // V tile is cleared of NaN and infinities in shared memory first (0 x NaN is
 // NaN), and where a visible one was cleared the item's end adds it back to the
 // rows that see it.
@@ -40,6 +41,8 @@
 // Waits are bounded: one that gives up sets the error word; every role then
 // leaves, waits (bounded) for its copies and MMAs in flight, frees the tensor
 // memory and returns.  Loads read this GPU's own memory, without multicast.
+#include <cooperative_groups.h>
+
 #include "bulk.cuh"
 #include "launch.cuh"
 #include "tcgen05.cuh"
@@ -48,16 +51,19 @@
 
 namespace mb {
 
+namespace cg = cooperative_groups;
+
 constexpr int kTtKeys = 128;   // keys per tile: MMA N of the scores, K of the output
 constexpr int kTtRows = 128;   // rows per tile: MMA M
 constexpr int kTtThreads = 384;
 constexpr int kTtInfo = 2;     // items known ahead
+constexpr int kTtCluster = 8;  // splits that a cluster joins (the portable size)
 constexpr float kTtGrow = 8.0f;  // log2 growth of a row's maximum that rescales
 
 struct TtItem {
   int b, h, rt, sp;     // sequence, KV head, row tile (pair), split
   int s, lo, k0, k1;    // cached positions, the row's first key, this split's keys
-  int item, tiles, alone, fix, dmax;  // key tiles; the only split; V was cleared; largest depth
+  int item, tiles, used, fix, dmax;  // key tiles; splits that hold keys; V was cleared; largest depth
   unsigned long long mask[kTreeMaxNodes];
 };
 
@@ -125,7 +131,57 @@ __device__ __forceinline__ uint32_t tt_bits(const TtView& v, int s, int k1, int 
   return v.real ? (cached | nb) & tt_low(k1 - t) : 0u;  // past the split's end: the next split's
 }
 
+// A cluster's join, one split per CTA: M = max m_j, out = sum 2^(m_j - M) acc_j
+// / sum 2^(m_j - M) l_j in split order.  The warps of the CTAs with keys each
+// take 32 rows, whose weights they form once, and every so many blocks of four
+// dims of them: loads from the other CTAs take some 0.5 us, so few may wait on
+// one another.
 template <int D, bool PAIR>
+__device__ __forceinline__ void tt_join(const TreeAttnParams& p, const TtItem& it, float* part, float2* part_ml, int warp,
+                                        int lane) {
+  const cg::cluster_group cluster = cg::this_cluster();
+  constexpr int R = PAIR ? 2 * kTtRows : kTtRows;
+  const float ninf = __int_as_float(0xff800000);
+  const int used = it.used, first = it.rt * R, rows = min(p.N * p.G - first, R);
+  const int blocks = (rows + 31) / 32, at = it.sp * 8 + warp;  // at most 8 blocks for 16 warps or more
+  const int row = at % blocks * 32 + lane, step = (used * 8 - at % blocks + blocks - 1) / blocks;
+  if (row >= rows) return;
+  float w[kTtCluster], M = ninf, den = 0.0f;
+  {
+    float2 y[kTtCluster];
+#pragma unroll
+    for (int j = 0; j < kTtCluster; ++j) {
+      y[j] = j < used ? cluster.map_shared_rank(part_ml, j)[row] : make_float2(ninf, 0.0f);
+      M = fmaxf(M, y[j].x);
+    }
+    const float base = M == ninf ? 0.0f : M;
+#pragma unroll
+    for (int j = 0; j < kTtCluster; ++j) {  // none for a split that this row sees nothing of; NaN scores stay NaN
+      w[j] = y[j].x == ninf && y[j].y == 0.0f ? 0.0f : ex2(y[j].x - base);
+      if (w[j] != 0.0f || y[j].y != 0.0f) den = fmaf(w[j], y[j].y, den);
+    }
+  }
+  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+  const int node = (first + row) / p.G, g = first + row - node * p.G;
+  uint16_t* out = static_cast<uint16_t*>(p.out) + (((int64_t)it.b * p.N + node) * p.H + it.h * p.G + g) * D;
+  const int src = row / kTtRows * D * kTtRows + row % kTtRows;
+#pragma unroll 2
+  for (int col = at / blocks * 4; col < D; col += step * 4) {
+    float num[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < kTtCluster; ++j) {
+      if (j < used) {
+        const float* a = cluster.map_shared_rank(part, j) + src + col * kTtRows;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) num[i] = fmaf(w[j], a[i * kTtRows], num[i]);
+      }
+    }
+    *reinterpret_cast<uint2*>(out + col) = den == 0.0f ? make_uint2(0u, 0u) : make_uint2(bf16x2(num[0] * inv, num[1] * inv),
+                                                                                         bf16x2(num[2] * inv, num[3] * inv));
+  }
+}
+
+template <int D, bool PAIR, bool JOIN>
 __global__ void __launch_bounds__(kTtThreads, 1)
     tree_tc_kernel(TreeAttnParams p, int row_groups, int items, const __grid_constant__ CUtensorMap tmk,
                    const __grid_constant__ CUtensorMap tmv) {
@@ -137,6 +193,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   unsigned char* sv = sk + NK * TILE;
   TtItem* info = reinterpret_cast<TtItem*>(sv + NV * TILE);
   float2* s_ml = reinterpret_cast<float2*>(sq);  // [2][128] maximum and sum, once the queries are done with
+  // JOIN: this split's part for the cluster, once the tiles are done with: [dim][128] per row tile, [row]
+  float* s_part = reinterpret_cast<float*>(sk);
+  float2* s_part_ml = s_ml + 2 * kTtRows;
+  static_assert(Sh::kQ * kTtRows * D * 4 <= (NK + NV) * TILE && (2 + Sh::kQ) * kTtRows * 8 <= TILE, "parts in the tiles' place");
   uint64_t* bars = reinterpret_cast<uint64_t*>(info + kTtInfo);
   uint64_t *kfull = bars, *kempty = kfull + NK, *vfull = kempty + NK, *vempty = vfull + NV, *sfull = vempty + NV,
            *phalf = sfull + 2, *pready = phalf + 2, *ofull = pready + 2, *oempty = ofull + 2, *qfull = oempty + 1, *ifull = qfull + 1,
@@ -155,6 +215,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     mbar_init(both, 8);
     for (int i = 0; i < 2; ++i) mbar_init(&each[i], 4);
     mbar_init(drain, 1);
+    if (JOIN) info[0].tiles = -1;  // stays where this split has no keys
   }
   tc_fence_before();
   __syncthreads();
@@ -172,7 +233,9 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
     int n_items = 0, kt_all = 0;
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const int rt = item % row_groups, sp = item / row_groups % p.NS, bh = item / row_groups / p.NS;
+      // a cluster's CTAs lie side by side: the splits of one row tile
+      const int rt = JOIN ? item / p.NS % row_groups : item % row_groups;
+      const int sp = JOIN ? item % p.NS : item / row_groups % p.NS, bh = item / row_groups / p.NS;
       const int h = bh % p.Hkv, b = bh / p.Hkv;
       const int64_t len = p.seqlen[b];
       const int cb = p.row_map != nullptr ? p.row_map[b] : b;
@@ -203,7 +266,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       if (lane == 0) {
         it.item = item; it.b = b; it.h = h; it.rt = rt; it.sp = sp;
         it.s = rg.s; it.lo = rg.lo; it.k0 = k0; it.k1 = k1; it.tiles = tiles; it.fix = 0; it.dmax = dm;
-        it.alone = tree_splits_used(rg.lo, rg.hi, kTtKeys, p.NS) <= 1;
+        it.used = tree_splits_used(rg.lo, rg.hi, kTtKeys, p.NS);
       }
       __syncwarp();
       if (lane == 0) {
@@ -362,10 +425,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     for (int n = 0; ok; ++n) {
       // the guessed item's Q rows come near under the wait: they depend on its number alone
       if (guess < items) {
-        const int bh = guess / row_groups / p.NS;
+        const int bh = guess / row_groups / p.NS, rt = JOIN ? guess / p.NS % row_groups : guess % row_groups;
         constexpr int LINES = D / 64;  // 128 bytes each
         for (int x = PAIR ? r : tid; x < kTtRows * LINES; x += QT) {
-          const int gr = (PAIR ? 2 * (guess % row_groups) + w : guess % row_groups) * kTtRows + x / LINES;
+          const int gr = (PAIR ? 2 * rt + w : rt) * kTtRows + x / LINES;
           if (gr < rows) {
             const int i = tt_node(gr), g = gr - i * p.G;
             asm volatile("prefetch.global.L1 [%0];\n" ::"l"(
@@ -607,7 +670,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           }
         }
         if (row < rows) {
-          if (it.alone) {
+          if (it.used <= 1) {
             uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + out + col);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -618,15 +681,19 @@ __global__ void __launch_bounds__(kTtThreads, 1)
               dst[i] = make_uint4(y[0], y[1], y[2], y[3]);
             }
           } else {
-            float* dst = p.ws_acc + (part * D + col) * kTtRows + r;
+            float* dst = JOIN ? s_part + ((PAIR ? w * D : 0) + col) * kTtRows + r : p.ws_acc + (part * D + col) * kTtRows + r;
 #pragma unroll
             for (int i = 0; i < 32; ++i) dst[i * kTtRows] = zero ? 0.0f : v[i];
           }
         }
       }
-      if (!it.alone && row < rows && (PAIR || w == 0))
-        reinterpret_cast<float2*>(p.ws_ml)[part * kTtRows + r] =
-            zero ? make_float2(ninf, 0.0f) : make_float2(mc * 0.693147180559945309f, l);
+      if (it.used > 1 && row < rows && (PAIR || w == 0)) {
+        if (JOIN)
+          s_part_ml[(PAIR ? w * kTtRows : 0) + r] = zero ? make_float2(ninf, 0.0f) : make_float2(mc, l);
+        else
+          reinterpret_cast<float2*>(p.ws_ml)[part * kTtRows + r] =
+              zero ? make_float2(ninf, 0.0f) : make_float2(mc * 0.693147180559945309f, l);
+      }
       tc_fence_before();
       __syncwarp();
       if (tiles > 0) {
@@ -643,6 +710,14 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 8) tmem_dealloc(tmem, 512);
+  if constexpr (JOIN) {
+    // every thread of the cluster comes here, whatever gave up before
+    const cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const TtItem& it = info[0];
+    if (warp < 8 && it.tiles > 0 && it.used > 1) tt_join<D, PAIR>(p, it, s_part, s_part_ml, warp, lane);
+    cluster.sync();  // nobody leaves while its part is read
+  }
 }
 
 // Joins the splits: M = max m_j, out = sum e^(m_j - M) acc_j / sum e^(m_j - M)
@@ -717,20 +792,29 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(TreeAttnParams p) {
 
 // Splits of a sequence's keys: the number with the least expected time.  A key
 // tile takes 0.95 us while few SMs read (1.9 with two row tiles), 1.4 when all
-// share the HBM; an item 4 us to start and end, a launch 3, the join's 4 and
-// 0.19 per split that it walks through, an item's partials 0.02 per 128 rows.
-// Measured (8 nodes, 8 heads per KV head; in brackets what the rule takes), us:
-//   splits               1     2     3     5     9    18    37
-//   1 x 600   [1]     12.3  12.4  11.6  11.2  (and a second launch on the host)
-//   1 x 8192  [13]    67.5  40.3  30.4  22.9  18.8  16.7  19.7
-//   4 x 4000  [6]     37.4  25.9  20.9  18.0  17.0  22.2  33.7
-//   16 x 8192 [2]     70.0  55.0  71.3  73.1  67.9  89.8   135
-//   37 x 4096 [1]     55.0  71.7  75.5  81.5   103   157   249
-//   1 x 65440, 64 nodes [18]  941   479   327   204   122  74.8  87.8
-int tree_tc_splits(int64_t ctas, int64_t max_len, bool pair) {
+// share the HBM; an item 4 us to start and end, a launch 3.  Up to 8 splits, as
+// far as such clusters fit the GPU at once, are joined by their cluster in 2.5
+// us; otherwise a second launch takes 4 and 0.19 per split that it walks
+// through, an item's partials 0.02 per 128 rows.
+// Measured (8 nodes, 8 heads per KV head), us, joined by a second launch:
+//   splits            1     2     3     5     9    18    37
+//   1 x 600        12.3  12.4  11.6  11.2
+//   1 x 8192       67.5  40.3  30.4  22.9  18.8  16.7  19.7
+//   4 x 4000       37.4  25.9  20.9  18.0  17.0  22.2  33.7
+//   16 x 8192      70.0  55.0  71.3  73.1  67.9  89.8   135
+//   37 x 4096      55.0  71.7  75.5  81.5   103   157   249
+//   1 x 65440, 64 nodes  941   479   327   204   122  74.8  87.8
+// and as the rule takes them: 1 x 600 in a cluster of 5 10.4, 4 x 1000 11.3 (one
+// split 15.2), 4 x 4000 16.5, 16 x 8192 in clusters of 2 51, 1 x 8192 in one of 8
+// 17.8 (a launch and an allocation fewer on the host: 4 us), 37 x 4096 54.5 in
+// one split, 1 x 65440 75 in 18.
+int tree_tc_splits(int64_t ctas, int64_t max_len, bool pair, bool* join) {
   const int64_t tiles = (max_len + kTtKeys - 1) / kTtKeys;
   int64_t best = 1;
   double least = 1e30;
+  *join = false;
+  // clusters of 2 to 8 CTAs that 148 SMs hold at once (74, 45, 33, 26, 22, 15, 15), less some
+  constexpr int kFit[kTtCluster + 1] = {0, 0, 70, 42, 31, 24, 20, 14, 14};
   for (int64_t ns = 1; ns <= kTreeMaxSplits && ns <= tiles; ++ns) {
     const int64_t items = ctas * ns, per = (tiles + ns - 1) / ns;
     auto wave = [&](int64_t n) {  // n items side by side
@@ -738,10 +822,13 @@ int tree_tc_splits(int64_t ctas, int64_t max_len, bool pair) {
       return n == 0 ? 0.0 : (double)per * (alone > shared ? alone : shared) + 4.0;
     };
     double t = (double)(items / 148) * wave(148) + wave(items % 148) + 3.0;
-    if (ns > 1) t += 4.0 + 0.19 * (double)ns + (pair ? 0.04 : 0.02) * (double)items;
+    const bool cluster = ns > 1 && ns <= kTtCluster && ctas <= kFit[ns];
+    if (cluster) t += pair ? 4.5 : 2.5;
+    else if (ns > 1) t += 4.0 + 0.19 * (double)ns + (pair ? 0.04 : 0.02) * (double)items;
     if (t < least) {
       least = t;
       best = ns;
+      *join = cluster;
     }
   }
   return (int)best;
@@ -757,10 +844,29 @@ cudaError_t tree_tc_launch1(const TreeAttnParams& p, int groups, const CUtensorM
   constexpr int smem = TtShape<D, PAIR>::kSmem;
   static_assert(smem <= 232448, "shared memory of one SM");
   const int items = p.B * p.Hkv * p.NS * groups;
+  if (p.join) {
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = smem_once(done, tree_tc_kernel<D, PAIR, true>, smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)items);
+    cfg.blockDim = dim3(kTtThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.NS;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    return e == cudaSuccess ? cudaLaunchKernelEx(&cfg, tree_tc_kernel<D, PAIR, true>, p, groups, items, tmk, tmv) : e;
+  }
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = smem_once(done, tree_tc_kernel<D, PAIR>, smem);
+  cudaError_t e = smem_once(done, tree_tc_kernel<D, PAIR, false>, smem);
   if (e == cudaSuccess)
-    e = launch_k(tree_tc_kernel<D, PAIR>, dim3((unsigned)(items < 148 ? items : 148)), dim3(kTtThreads), smem, st, p,
+    e = launch_k(tree_tc_kernel<D, PAIR, false>, dim3((unsigned)(items < 148 ? items : 148)), dim3(kTtThreads), smem, st, p,
                  groups, items, tmk, tmv);
   if (e == cudaSuccess && p.NS > 1)
     e = launch_k(tree_tc_merge_kernel<D>,

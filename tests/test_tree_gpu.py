@@ -154,6 +154,16 @@ def test_attention(cuda, K, B, N, H, Hkv, D, T, lens, window, chain, ragged, row
     verify_attn(K, c, window)
 
 
+@pytest.mark.parametrize("N,H,D", [(5, 8, 128), (40, 8, 128), (3, 4, 64), (64, 8, 64)])
+@pytest.mark.parametrize("window", [0, 300])
+def test_attention_splits_of_ragged_lengths(cuda, K, N, H, D, window):
+    """Caches cut into up to eight splits (and more where 40 tiles allow), of which
+    a sequence uses none, one, some or all."""
+    lens = [0, 1, 127, 128, 129, 383, 700, 1060]
+    verify_attn(K, attn_case(26, 8, N, H, 2, D, 1124, lens, BF, ragged=True), window)
+    verify_attn(K, attn_case(27, 2, N, H, 2, D, 5100, [5000, 130], BF), window)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_attention_heads_of_256(cuda, K, dtype):
     verify_attn(K, attn_case(5, 2, 6, 8, 2, 256, 300, [280, 31], dtype))
