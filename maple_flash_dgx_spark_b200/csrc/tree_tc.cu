@@ -24,10 +24,10 @@
 //
 // An item is one split of one sequence's keys for one KV head and row tile (or
 // pair).  With JOIN a CTA has one item, and the splits of a row tile form a
-// cluster, which joins their parts through its shared memory.  A tile that some row sees only in part is masked in registers; its
-// V tile is cleared of NaN and infinities in shared memory first (0 x NaN is
-// NaN), and where a visible one was cleared the item's end adds it back to the
-// rows that see it.
+// cluster, which joins their parts through its shared memory.  A tile that some
+// row sees only in part is masked in registers; its V tile is cleared of NaN and
+// infinities in shared memory first (0 x NaN is NaN), and where a visible one was
+// cleared the item's end adds it back to the rows that see it.
 //
 // Up to 128 rows HBM bounds it: 64 sequences x 8150 with eight nodes (32 heads
 // on 4 of 128), 1.08 GB in 164 us = 6.57 TB/s, what a plain copy reaches; held
@@ -793,9 +793,10 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(TreeAttnParams p) {
 // Splits of a sequence's keys: the number with the least expected time.  A key
 // tile takes 0.95 us while few SMs read (1.9 with two row tiles), 1.4 when all
 // share the HBM; an item 4 us to start and end, a launch 3.  Up to 8 splits, as
-// far as such clusters fit the GPU at once, are joined by their cluster in 2.5
-// us; otherwise a second launch takes 4 and 0.19 per split that it walks
-// through, an item's partials 0.02 per 128 rows.
+// far as such clusters fit the GPU at once, are joined by their cluster in 2.3
+// us (4.5 with two row tiles); otherwise a second launch takes 1.5 on the GPU and
+// as much again on the host, 0.25 per split that it walks through and 0.02 per
+// 128 rows of an item's partials.
 // Measured (8 nodes, 8 heads per KV head), us, joined by a second launch:
 //   splits            1     2     3     5     9    18    37
 //   1 x 600        12.3  12.4  11.6  11.2
@@ -804,17 +805,17 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(TreeAttnParams p) {
 //   16 x 8192      70.0  55.0  71.3  73.1  67.9  89.8   135
 //   37 x 4096      55.0  71.7  75.5  81.5   103   157   249
 //   1 x 65440, 64 nodes  941   479   327   204   122  74.8  87.8
-// and as the rule takes them: 1 x 600 in a cluster of 5 10.4, 4 x 1000 11.3 (one
-// split 15.2), 4 x 4000 16.5, 16 x 8192 in clusters of 2 51, 1 x 8192 in one of 8
-// 17.8 (a launch and an allocation fewer on the host: 4 us), 37 x 4096 54.5 in
-// one split, 1 x 65440 75 in 18.
+// and as the rule takes them: 1 x 600 in a cluster of 5 10.8, 4 x 1000 in 5 11.4
+// (one split 15.2), 4 x 4000 in 6 16.5, 16 x 8192 in 2 51, 1 x 8192 in 8 17.9 (a
+// launch and an allocation fewer on the host, 4 us), 37 x 4096 55 in one split,
+// 1 x 65440 73 in 18; 22 x 3800 on 2 KV heads in 3 19.2, in 2 23.5.
 int tree_tc_splits(int64_t ctas, int64_t max_len, bool pair, bool* join) {
   const int64_t tiles = (max_len + kTtKeys - 1) / kTtKeys;
   int64_t best = 1;
   double least = 1e30;
   *join = false;
-  // clusters of 2 to 8 CTAs that 148 SMs hold at once (74, 45, 33, 26, 22, 15, 15), less some
-  constexpr int kFit[kTtCluster + 1] = {0, 0, 70, 42, 31, 24, 20, 14, 14};
+  // clusters of 2 to 8 CTAs that fit a B200 at once (one that fits fewer takes a second turn)
+  constexpr int kFit[kTtCluster + 1] = {0, 0, 74, 45, 33, 26, 22, 15, 15};
   for (int64_t ns = 1; ns <= kTreeMaxSplits && ns <= tiles; ++ns) {
     const int64_t items = ctas * ns, per = (tiles + ns - 1) / ns;
     auto wave = [&](int64_t n) {  // n items side by side
@@ -823,8 +824,8 @@ int tree_tc_splits(int64_t ctas, int64_t max_len, bool pair, bool* join) {
     };
     double t = (double)(items / 148) * wave(148) + wave(items % 148) + 3.0;
     const bool cluster = ns > 1 && ns <= kTtCluster && ctas <= kFit[ns];
-    if (cluster) t += pair ? 4.5 : 2.5;
-    else if (ns > 1) t += 4.0 + 0.19 * (double)ns + (pair ? 0.04 : 0.02) * (double)items;
+    if (cluster) t += pair ? 4.5 : 2.3;
+    else if (ns > 1) t += 1.5 + 0.25 * (double)ns + (pair ? 0.04 : 0.02) * (double)items + 1.5;
     if (t < least) {
       least = t;
       best = ns;
