@@ -84,9 +84,9 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, 
 // not keep NaN out: K and V are cleared of both as they arrive.  A score with a
 // cleared key is computed again from the cache (each such key by its threads);
 // cleared values of V are added at the end for the rows that see them.
-// 16 query heads of 256 on 4 KV heads, 8 nodes, 4 x 4096 bf16: 80 us, 840 GB/s
+// 16 query heads of 256 on 4 KV heads, 8 nodes, 4 x 4096 bf16: 70 us, 960 GB/s
 // of cache (115 with four warps that shared no keys); 32 heads of 128 on 8 with
-// 64 nodes, 8 x 4000 fp32: 975 us, 34 TFLOP/s (1160).  Bound by the latency of
+// 64 nodes, 8 x 4000 fp32: 870 us, 38 TFLOP/s (1160).  Bound by the latency of
 // its instructions: a scheduler issues in two cycles of five at 8 x 4000, eight
 // instructions per product (splits, ldmatrix, V's 4-byte reads), and the
 // registers hold no more than four warps on it.
@@ -139,41 +139,13 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
   const int g = lane >> 2, t = lane & 3;
   const int sp = blockIdx.x, h = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles, b = blockIdx.z;
   const float ninf = __int_as_float(0xff800000);
+  const float scale = p.scale * 1.44269504088896341f;  // scores in powers of 2
   pdl_wait();
   pdl_trigger();
   const int64_t len = p.seqlen[b];
   const int cb = p.row_map != nullptr ? p.row_map[b] : b;
   const int rows = p.N * p.G, r0 = rt * ROWS;
   const uint64_t per_g = (1ull << 32) / (unsigned)p.G + 1;  // row / G by a multiplication, exact while row x G < 2^32
-  // q rows, zero past the last one; a thread's loads in flight together
-  constexpr int QN = ROWS * CH / kMmaThreads, QU = QN < 8 ? QN : 8;
-#pragma unroll 1
-  for (int e0 = 0; e0 < QN; e0 += QU) {
-    uint4 v[QU];
-#pragma unroll
-    for (int e = 0; e < QU; ++e) {
-      const int c = tid + kMmaThreads * (e0 + e), gr = r0 + c / CH;
-      v[e] = make_uint4(0u, 0u, 0u, 0u);
-      if (gr < rows) {
-        const int i = (int)((uint64_t)(unsigned)gr * per_g >> 32), qg = gr - i * p.G;
-        v[e] = ld_u4(static_cast<const char*>(p.q) +
-                     (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + qg) * p.q_sh + c % CH * EPC) * es);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < QU; ++e) {
-      const int c = tid + kMmaThreads * (e0 + e);
-      float f[EPC];
-      widen_u4<XT>(v[e], f);
-      if constexpr (XT == kF32) {
-#pragma unroll
-        for (int u = 0; u < EPC; ++u) f[u] = __uint_as_float(cut_huge(__float_as_uint(f[u])));
-      }
-#pragma unroll
-      for (int u = 0; u < EPC; u += 4)
-        *reinterpret_cast<float4*>(&sq[c / CH * PITCH + c % CH * EPC + u]) = make_float4(f[u], f[u + 1], f[u + 2], f[u + 3]);
-    }
-  }
   if (tid < 32) {
     const unsigned long long keep = p.N < 64 ? (1ull << p.N) - 1 : ~0ull;
     unsigned long long used = 0;
@@ -261,6 +233,36 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
     }
   };
 
+  if (k0 < k1) load(k0, 0);
+  // q rows, zero past the last one; a thread's loads in flight together
+  constexpr int QN = ROWS * CH / kMmaThreads, QU = QN < 8 ? QN : 8;
+#pragma unroll 1
+  for (int e0 = 0; e0 < QN; e0 += QU) {
+    uint4 v[QU];
+#pragma unroll
+    for (int e = 0; e < QU; ++e) {
+      const int c = tid + kMmaThreads * (e0 + e), gr = r0 + c / CH;
+      v[e] = make_uint4(0u, 0u, 0u, 0u);
+      if (gr < rows) {
+        const int i = (int)((uint64_t)(unsigned)gr * per_g >> 32), qg = gr - i * p.G;
+        v[e] = ld_u4(static_cast<const char*>(p.q) +
+                     (b * p.q_sb + i * p.q_sn + (int64_t)(h * p.G + qg) * p.q_sh + c % CH * EPC) * es);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < QU; ++e) {
+      const int c = tid + kMmaThreads * (e0 + e);
+      float f[EPC];
+      widen_u4<XT>(v[e], f);
+      if constexpr (XT == kF32) {
+#pragma unroll
+        for (int u = 0; u < EPC; ++u) f[u] = __uint_as_float(cut_huge(__float_as_uint(f[u])));
+      }
+#pragma unroll
+      for (int u = 0; u < EPC; u += 4)
+        *reinterpret_cast<float4*>(&sq[c / CH * PITCH + c % CH * EPC + u]) = make_float4(f[u], f[u + 1], f[u + 2], f[u + 3]);
+    }
+  }
   // rows g and g + 8 of the warp's 16
   unsigned long long mine[2];
   float m[2] = {ninf, ninf}, l[2] = {0.0f, 0.0f}, acc[D / 8][4];
@@ -285,7 +287,6 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
   };
   const bool idle = r0 + warp * 16 >= rows;  // a warp without rows only loads
   const float* a_at = sq + (warp * 16 + (lane & 7) + (lane >> 3 & 1) * 8) * PITCH + (lane >> 4) * 4;
-  if (k0 < k1) load(k0, 0);
   int stage = 0;
   for (int t0 = k0; t0 < k1; t0 += kMmaKeys, stage ^= 1) {
     if (t0 + kMmaKeys < k1) load(t0 + kMmaKeys, stage ^ 1);
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float& x = s[j][2 * a + c];
-            x = mixed && !sees(a, t0 + 8 * (JW * kw + j) + 2 * t + c) ? ninf : x * p.scale;
+            x = mixed && !sees(a, t0 + 8 * (JW * kw + j) + 2 * t + c) ? ninf : x * scale;
             mt = fmaxf(mt, x);
           }
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
@@ -382,12 +383,12 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float& x = s[j][2 * a + c];
-            x = x == ninf ? 0.0f : mexp(x - base);
+            x = x == ninf ? 0.0f : ex2(x - base);
             sum += x;
           }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        fix[a] = mt == m[a] ? 1.0f : mexp(m[a] - base);
+        fix[a] = mt == m[a] ? 1.0f : ex2(m[a] - base);
         l[a] = fmaf(l[a], fix[a], sum);
         m[a] = mt;
       }
@@ -464,8 +465,8 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
       const float mo = at[(D / 2 + a) * 32], mt = fmaxf(m[a], mo), base = mt == ninf ? 0.0f : mt;
-      w0[a] = mexp(m[a] - base);
-      w1[a] = mexp(mo - base);
+      w0[a] = ex2(m[a] - base);
+      w1[a] = ex2(mo - base);
       l[a] = l[a] * w0[a] + at[(D / 2 + 2 + a) * 32] * w1[a];
       m[a] = mt;
     }
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeAttnParams p, int t
   }
   const float M = warp_max(fmaxf(mj[0], mj[1]));
   const float base = M == ninf ? 0.0f : M;
-  float wj[2] = {mexp(mj[0] - base), mexp(mj[1] - base)};
+  float wj[2] = {ex2(mj[0] - base), ex2(mj[1] - base)};
   float den = 0.0f, num[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) num[u] = 0.0f;
@@ -720,7 +721,7 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
                                    const int32_t* row_map, float scale, int64_t window, void* out, void* workspace,
                                    int64_t workspace_bytes, int* err, void* stream) {
   if (batch < 0 || nodes <= 0 || nodes > kTreeMaxNodes || num_heads <= 0 || num_kv_heads <= 0 || max_len <= 0 ||
-      cache_batch < 0 || window < 0 || !(scale - scale == 0.0f))
+      cache_batch < 0 || window < 0 || !(scale * 2.0f - scale * 2.0f == 0.0f))  // also as powers of 2
     return kErrShape;
   if (batch == 0) return kOk;
   if (x_dtype != kF32 && x_dtype != kBF16) return kErrDtype;

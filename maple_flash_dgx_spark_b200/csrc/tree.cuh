@@ -36,6 +36,11 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
 constexpr int kTreeMaxNodes = 64;
 constexpr int kTreeMaxSplits = 64;
 constexpr int kTreeMaxGroup = 4096;  // query heads per KV head: (row of 64 nodes) x group stays below 2^32

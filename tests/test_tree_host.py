@@ -38,7 +38,7 @@ def test_tree_attention_refuses_before_any_launch(L):
     assert _attn(L, B=0) == 0                        # nothing to do
     for bad in (dict(B=-1), dict(N=0), dict(N=65), dict(H=0), dict(Hkv=0), dict(H=30), dict(D=96), dict(T=0),
                 dict(window=-1), dict(B=1 << 17), dict(Bc=0), dict(T=1 << 31), dict(scale=float("nan")),
-                dict(scale=float("inf")), dict(H=8192, Hkv=1)):
+                dict(scale=float("inf")), dict(scale=-3e38), dict(H=8192, Hkv=1)):
         assert _attn(L, **bad) == 1, bad
     for null in ("q", "k", "out", "err"):
         assert _attn(L, **{null: None}) == 1, null
