@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
   __shared__ unsigned long long s_mask[kTreeMaxNodes];
   __shared__ unsigned s_used[2];
   __shared__ int s_dmax, s_fix;
-  __shared__ unsigned s_odd[2];                           // per stage: keys that were cleared
+  __shared__ unsigned s_odd[4];                           // keys that were cleared, four tiles in turn
   const int tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) % RW, kw = (tid >> 5) / RW;
   const int g = lane >> 2, t = lane & 3;
   const int sp = blockIdx.x, h = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles, b = blockIdx.z;
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
       s_used[1] = hi;
       s_dmax = dm;
       s_fix = 0;
-      s_odd[0] = s_odd[1] = 0;
+      s_odd[0] = s_odd[1] = s_odd[2] = s_odd[3] = 0;
     }
   }
   __syncthreads();
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
   // clears this thread's chunks of NaN and infinities
-  auto clear = [&](int stage) {
+  auto clear = [&](int stage, int turn) {
     float* st = ring + stage * STAGE;
     uint32_t any = 0;
 #pragma unroll
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
         }
         *x = 0u;
         if (e & 1) s_fix = 1;
-        else atomicOr(&s_odd[stage], 1u << r);
+        else atomicOr(&s_odd[turn & 3], 1u << r);
       }
     }
   };
@@ -288,12 +288,12 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
   const bool idle = r0 + warp * 16 >= rows;  // a warp without rows only loads
   const float* a_at = sq + (warp * 16 + (lane & 7) + (lane >> 3 & 1) * 8) * PITCH + (lane >> 4) * 4;
   int stage = 0;
-  for (int t0 = k0; t0 < k1; t0 += kMmaKeys, stage ^= 1) {
+  for (int t0 = k0, turn = 0; t0 < k1; t0 += kMmaKeys, stage ^= 1, ++turn) {
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    clear(stage, turn);
+    __syncthreads();  // the tile is there, and everyone is done with the one before
+    if (tid == 0) s_odd[(turn + 2) & 3] = 0;  // read two tiles ago, written in two
     if (t0 + kMmaKeys < k1) load(t0 + kMmaKeys, stage ^ 1);
-    else asm volatile("cp.async.commit_group;\n" ::: "memory");
-    asm volatile("cp.async.wait_group 1;\n" ::: "memory");
-    clear(stage);
-    __syncthreads();
     const float* sk = ring + stage * STAGE;
     const float* sv = sk + kMmaKeys * PITCH;
     if (!idle) {
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
             for (int c = 0; c < 4; ++c) s[j][c] += fresh[j][c];
         }
       }
-      if (const unsigned odd = s_odd[stage]; odd) {  // rare: keys with a NaN or an infinity, from the cache
+      if (const unsigned odd = s_odd[turn & 3]; odd) {  // rare: keys with a NaN or an infinity, from the cache
 #pragma unroll
         for (int j = 0; j < JW; ++j)
 #pragma unroll
@@ -439,9 +439,8 @@ __global__ void __launch_bounds__(kMmaThreads, D == 256 ? 1 : 2)
           for (int c = 0; c < 4; ++c) acc[j0 + j][c] = XT == kBF16 ? part[j][c] : acc[j0 + j][c] + part[j][c];
       }
     }
-    __syncthreads();  // the stage may be written again
-    if (tid == 0) s_odd[stage] = 0;
   }
+  __syncthreads();  // the tiles' place may be written again
   // the groups' parts of each row, in their order
   float* join = ring;  // [KW - 1][RW][D / 2 + 4][32]
   if (kw > 0 && !idle) {
