@@ -72,21 +72,22 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, 
 // lo hi + hi lo + hi hi leaves out 2^-23 of a product.  The pipe cuts its sums
 // instead of rounding them, so an fp32 sum takes at most four steps on it
 // before it is added to the rest with fp32's own rounding: 7e-7 of error at
-// 4 x 1500, where straight sums had 2.6e-6 (and 8 % less time).  bf16 values are their own hi, which saves two of the
-// three products for the scores and one for the output; their results' rounding
-// to 2^-8 hides the cut sums, which stay straight.  Tiles of 32 keys stand in
-// shared memory as fp32 in two stages (cp.async under the tile before); a pitch
-// of D + 4 floats keeps ldmatrix (K, Q) and the V reads free of bank conflicts.
-// The weights stay in registers: key 2t of a block of eight takes the place of
-// the product's index t and key 2t + 1 that of t + 4, which is how the scores'
-// accumulators lie, and V's rows are read in that order.
+// 4 x 1500, where straight sums had 2.6e-6 (and 8 % less time).  bf16 values are
+// their own hi, which saves two of the three products for the scores and one for
+// the output; their results' rounding to 2^-8 hides the cut sums, which stay
+// straight.  Tiles of 32 keys stand in shared memory as fp32 in two stages
+// (cp.async under the tile before); a pitch of D + 4 floats keeps ldmatrix (K, Q)
+// and the V reads free of bank conflicts.  The weights stay in registers: key 2t
+// of a block of eight takes the place of the product's index t and key 2t + 1
+// that of t + 4, which is how the scores' accumulators lie, and V's rows are read
+// in that order.
 // Infinities do not survive the split (0 x inf), and a masked weight of 0 does
 // not keep NaN out: K and V are cleared of both as they arrive.  A score with a
 // cleared key is computed again from the cache (each such key by its threads);
 // cleared values of V are added at the end for the rows that see them.
-// 16 query heads of 256 on 4 KV heads, 8 nodes, 4 x 4096 bf16: 70 us, 960 GB/s
+// 16 query heads of 256 on 4 KV heads, 8 nodes, 4 x 4096 bf16: 69 us, 980 GB/s
 // of cache (115 with four warps that shared no keys); 32 heads of 128 on 8 with
-// 64 nodes, 8 x 4000 fp32: 870 us, 38 TFLOP/s (1160).  Bound by the latency of
+// 64 nodes, 8 x 4000 fp32: 859 us, 39 TFLOP/s (1160).  Bound by the latency of
 // its instructions: a scheduler issues in two cycles of five at 8 x 4000, eight
 // instructions per product (splits, ldmatrix, V's 4-byte reads), and the
 // registers hold no more than four warps on it.
