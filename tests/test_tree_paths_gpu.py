@@ -82,3 +82,130 @@ def test_attention_single_token_is_decode_bf16(cuda, K, D, T):
     inner = mass * (2.0 ** -8 + 2 * (D * 2.0 ** -24 * reach + 2.0 ** -20) + 2 * T * 2.0 ** -24)
     tol = 2 * (inner + 2.0 ** -8 * (exact.abs() + inner))
     assert ((got.double() - want.transpose(1, 2).double()).abs() <= tol + 1e-30).all()
+
+
+# ------------------------------------------------------------ in the model --
+def test_captured_tree_steps(cuda, K):
+    """forward_tree, verify_tree and the commit in one graph, replayed as the
+    sequences grow, against the same steps called."""
+    torch.set_grad_enabled(False)
+    try:
+        model = tiny(cuda, BF)
+        r = random.Random(8)
+        B, N = 2, 6
+        cache = model.make_cache(max_len=64, batch=B)
+        cache.remap = True
+        prefill(model, cache, [[r.randrange(512) for _ in range(n)] for n in (11, 4)])
+        par = torch.tensor([[-1, 0, 0, 1, 1, 2], [-1, 0, 1, 2, -2, -2]], dtype=torch.int32, device=cuda)
+        inputs = [(torch.randint(0, 512, (B, N), device=cuda), torch.rand(B, N, device=cuda)) for _ in range(3)]
+        tok, u = torch.zeros_like(inputs[0][0]), torch.zeros_like(inputs[0][1])
+        start = cache.snapshot()
+
+        def step(kept=None):
+            logits = model.forward_tree(tok, par, cache)
+            out = K.verify_tree(logits, tok, par, u, temperature=1.0, top_p=0.95, top_k=20)
+            cache.commit_tree(*out[:2], kept=kept)
+            return (logits, *out)
+
+        want = []
+        for t, x in inputs:
+            tok.copy_(t)
+            u.copy_(x)
+            want.append([y.clone() for y in step()] + [cache.seqlen.clone(), list(cache.seen)])
+        rows = [t.clone() for t in cache.k + cache.v]
+        cache.restore(start)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            model.forward_tree(tok, par, cache)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                out = step(kept=[0] * B)  # the host's counts follow each replay
+        torch.cuda.current_stream().wait_stream(side)
+        cache.restore(start)
+        for (t, x), w in zip(inputs, want):
+            tok.copy_(t)
+            u.copy_(x)
+            graph.replay()
+            cache.seen = [a + b for a, b in zip(cache.seen, out[2].tolist())]
+            for got, y in zip((*out, cache.seqlen), w):
+                assert torch.equal(got, y)
+            assert cache.seen == w[-1]
+        for got, y in zip(cache.k + cache.v, rows):
+            for b in range(B):
+                assert torch.equal(got[b, :, :cache.seen[b]], y[b, :, :cache.seen[b]])
+    finally:
+        torch.set_grad_enabled(True)
+
+
+def test_tree_steps_are_steps_of_one_node(cuda, K):
+    """fp32: every node's logits and cache rows against its path taken one node
+    at a time by trees of one, committed one by one, from the same cache.  All but
+    the attention's order of sums is the same arithmetic.  fp32 sums of 64
+    products with sum |q k| scale <= 8 are off by 64 half steps of it at worst
+    (3e-5) and by sqrt(64) of them (4e-6) as they fall, for two routes, two
+    layers and a gain of up to six through the norms and the experts: 1e-4 of the
+    largest logit, where a wrong position or slot changes its second digit.  The
+    first layer's K and V have no attention before them: the same bits, as plain
+    decoding of the accepted tokens has."""
+    torch.set_grad_enabled(False)
+    try:
+        model = tiny(cuda, F32)
+        r = random.Random(9)
+        texts = [[r.randrange(512) for _ in range(n)] for n in (25, 2, 14)]
+        par = [[-1, 0, 0, 1, 1, 2, 5, 3], [-1, 0, 1, 2, 3, 4, 5, 6], [-1, 0, 0, 0, 2, -2, -2, -2]]
+        B, N = 3, 8
+        cache = model.make_cache(max_len=64, batch=B)
+        cache.remap = True
+        prefill(model, cache, texts)
+        cache.swap_slots(0, 1)
+        texts[0], texts[1] = texts[1], texts[0]
+        lens = list(cache.seen)
+        tok = [[r.randrange(512) for _ in range(N)] for _ in range(B)]
+        pt = torch.tensor(par, dtype=torch.int32, device=cuda)
+        start = cache.snapshot()
+        logits = model.forward_tree(torch.tensor(tok, device=cuda), pt, cache)
+        tree = [t.clone() for t in cache.k + cache.v]
+        top = float(logits.abs().max())
+        one, root = torch.ones(1, dtype=torch.int32, device=cuda), torch.full((1, 1), -1, dtype=torch.int32, device=cuda)
+        paths = []
+        for b in range(B):
+            longest = []
+            for i in range(N):
+                if par[b][i] < -1:
+                    continue
+                line, j = [], i
+                while j >= 0:
+                    line.append(j)
+                    j = par[b][j]
+                line = line[::-1]
+                longest = max(longest, line, key=len)
+                cache.restore(start)
+                with cache.prefill_slot(b):
+                    for d, j in enumerate(line):
+                        got = model.forward_tree(torch.tensor([[tok[b][j]]], device=cuda), root, cache)
+                        cache.commit_tree(torch.zeros_like(root), one)
+                assert cache.seen[b] == int(cache.seqlen[b]) == lens[b] + len(line)
+                err = float((got[0, 0] - logits[b, i]).abs().max())
+                assert err <= 1e-4 * top, (b, i, err, top)
+                row, at = cache.row_of[b], lens[b]
+                for li, (x, y) in enumerate(zip(cache.k + cache.v, tree)):
+                    x, y = x[row, :, at + len(line) - 1], y[row, :, at + i]
+                    if li % len(cache.k) == 0:
+                        assert torch.equal(x, y), (b, i)
+                    else:
+                        assert float((x - y).abs().max()) <= 1e-4 * float(y.abs().max()), (b, i, li)
+            paths.append(longest)
+        # the longest paths accepted, against plain decoding
+        cache.restore(start)
+        model.forward_tree(torch.tensor(tok, device=cuda), pt, cache)
+        cache.commit_tree(torch.tensor([p + [-1] * (N - len(p)) for p in paths], device=cuda),
+                          torch.tensor([len(p) for p in paths], dtype=torch.int32, device=cuda))
+        for b, p in enumerate(paths):
+            plain = model.make_cache(max_len=64)
+            model.forward(torch.tensor(texts[b] + [tok[b][j] for j in p], device=cuda).reshape(1, -1), cache=plain)
+            assert cache.seen[b] == plain.seen[0]
+            for got, want in ((cache.k[0], plain.k[0]), (cache.v[0], plain.v[0])):
+                assert torch.equal(got[cache.row_of[b], :, :cache.seen[b]], want[0, :, :cache.seen[b]])
+    finally:
+        torch.set_grad_enabled(True)
