@@ -533,6 +533,15 @@ int maple_commit_tree(void* const* k_caches, void* const* v_caches, int64_t laye
                       int64_t max_len, int64_t head_dim, const int64_t* seqlen, const int32_t* path,
                       const int32_t* n_path, const int32_t* row_map, int* err, void* stream);
 
+/* The same, and kept[b] (unless NULL) = the rows kept of sequence b, by which
+ * its length grows: n_path[b], or 0 where nothing moved because the path was
+ * refused (or n_path[b] <= 0).  With layers = 0 nothing is written. */
+int maple_commit_tree_kept(void* const* k_caches, void* const* v_caches, int64_t layers, int x_dtype, int64_t batch,
+                           int64_t nodes, int64_t cache_batch, int64_t num_kv_heads, int64_t cache_sb,
+                           int64_t cache_sh, int64_t max_len, int64_t head_dim, const int64_t* seqlen,
+                           const int32_t* path, const int32_t* n_path, const int32_t* row_map, int32_t* kept, int* err,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -121,6 +121,8 @@ _SIGS: dict[str, tuple] = {
     "maple_verify_tree": (i32, [vp, i32, i64, i64, i64, i64, i64, vp, vp, vp, vp, i32, i64, i64, f32, f32,
                                 i64, i32, vp, vp, vp, vp, i64, vp, vp]),
     "maple_commit_tree": (i32, [vp, vp, i64, i32, i64, i64, i64, i64, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp]),
+    "maple_commit_tree_kept": (i32, [vp, vp, i64, i32, i64, i64, i64, i64, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp,
+                                     vp]),
     "maple_synth_ternary": (i32, [ctypes.c_uint64, ctypes.c_uint64, i64, vp, vp]),
     "maple_synth_normal": (i32, [ctypes.c_uint64, ctypes.c_uint64, i64, ctypes.c_double, f32, i32, i32, vp, vp]),
     "maple_synth_rtn4_sym": (i32, [ctypes.c_uint64, ctypes.c_uint64, i64, i64, i64, ctypes.c_double, vp, vp, vp]),

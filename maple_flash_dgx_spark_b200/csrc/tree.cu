@@ -606,6 +606,7 @@ struct CommitParams {
   const int32_t* path;
   const int32_t* n_path;
   const int32_t* row_map;
+  int32_t* kept;  // [B] rows kept of each sequence, or null
   int* err;
   int64_t sb, sh, sbh;  // cache strides in 16-byte units (batch, KV head); sbh: units per row
   int B, N, Hkv, Bc, T, nptr;
@@ -620,9 +621,13 @@ __global__ void __launch_bounds__(256) commit_kernel(const __grid_constant__ Com
   const int n = p.n_path[b];
   const int64_t s = p.seqlen[b];
   const int cb = p.row_map != nullptr ? p.row_map[b] : b;
+  const bool tells = p.kept != nullptr && blockIdx.x == 0 && tid == 0;
   if (tid == 0) s_bad = 0;
   __syncthreads();
-  if (n <= 0) return;
+  if (n <= 0) {
+    if (tells) p.kept[b] = 0;
+    return;
+  }
   const bool ok = n <= p.N && s >= 0 && s <= p.T && cb >= 0 && cb < p.Bc;
   if (ok && tid < n) {
     const int d = tid, x = p.path[(int64_t)b * p.N + d];
@@ -631,7 +636,9 @@ __global__ void __launch_bounds__(256) commit_kernel(const __grid_constant__ Com
     s_path[d] = x;
   }
   __syncthreads();
-  if (!ok || s_bad) {  // a path that does not rise or leaves the cache: nothing moves
+  const bool bad = !ok || s_bad;  // a path that does not rise or leaves the cache: nothing moves
+  if (tells) p.kept[b] = bad ? 0 : n;
+  if (bad) {
     if (tid == 0) atomicOr(p.err, kErrFlagBounds);
     return;
   }
@@ -785,11 +792,11 @@ extern "C" int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, in
   return e == cudaSuccess ? kOk : kErrCuda;
 }
 
-extern "C" int maple_commit_tree(void* const* k_caches, void* const* v_caches, int64_t layers, int x_dtype,
-                                 int64_t batch, int64_t nodes, int64_t cache_batch, int64_t num_kv_heads,
-                                 int64_t cache_sb, int64_t cache_sh, int64_t max_len, int64_t head_dim,
-                                 const int64_t* seqlen, const int32_t* path, const int32_t* n_path,
-                                 const int32_t* row_map, int* err, void* stream) {
+extern "C" int maple_commit_tree_kept(void* const* k_caches, void* const* v_caches, int64_t layers, int x_dtype,
+                                      int64_t batch, int64_t nodes, int64_t cache_batch, int64_t num_kv_heads,
+                                      int64_t cache_sb, int64_t cache_sh, int64_t max_len, int64_t head_dim,
+                                      const int64_t* seqlen, const int32_t* path, const int32_t* n_path,
+                                      const int32_t* row_map, int32_t* kept, int* err, void* stream) {
   if (layers < 0 || batch < 0 || nodes <= 0 || nodes > kTreeMaxNodes || num_kv_heads <= 0 || max_len <= 0 ||
       head_dim <= 0 || batch > 65535 || cache_batch < 0 || cache_batch > (1LL << 30) || max_len > (1LL << 30))
     return kErrShape;
@@ -811,6 +818,7 @@ extern "C" int maple_commit_tree(void* const* k_caches, void* const* v_caches, i
       p.ptr[2 * i + 1] = v_caches[l0 + i];
     }
     p.seqlen = seqlen; p.path = path; p.n_path = n_path; p.row_map = row_map; p.err = err;
+    p.kept = l0 == 0 ? kept : nullptr;  // the same for all layers
     p.sb = cache_sb / epu; p.sh = cache_sh / epu; p.sbh = head_dim / epu;
     p.B = (int)batch; p.N = (int)nodes; p.Hkv = (int)num_kv_heads; p.Bc = (int)cache_batch; p.T = (int)max_len;
     p.nptr = (int)(2 * nl);
@@ -820,4 +828,13 @@ extern "C" int maple_commit_tree(void* const* k_caches, void* const* v_caches, i
     if (e != cudaSuccess) return kErrCuda;
   }
   return kOk;
+}
+
+extern "C" int maple_commit_tree(void* const* k_caches, void* const* v_caches, int64_t layers, int x_dtype,
+                                 int64_t batch, int64_t nodes, int64_t cache_batch, int64_t num_kv_heads,
+                                 int64_t cache_sb, int64_t cache_sh, int64_t max_len, int64_t head_dim,
+                                 const int64_t* seqlen, const int32_t* path, const int32_t* n_path,
+                                 const int32_t* row_map, int* err, void* stream) {
+  return maple_commit_tree_kept(k_caches, v_caches, layers, x_dtype, batch, nodes, cache_batch, num_kv_heads, cache_sb,
+                                cache_sh, max_len, head_dim, seqlen, path, n_path, row_map, nullptr, err, stream);
 }

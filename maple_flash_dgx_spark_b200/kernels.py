@@ -1175,11 +1175,14 @@ class CacheRows:
         self.k_ptrs, self.v_ptrs = table(*[t.data_ptr() for t in k]), table(*[t.data_ptr() for t in v])
 
 
-def commit_tree(rows: CacheRows, seqlen, path, n_path, *, row_map=None) -> None:
+def commit_tree(rows: CacheRows, seqlen, path, n_path, *, row_map=None, kept=None) -> None:
     """Keep the accepted nodes' K/V rows, in every layer and in place: slot
     ``seqlen[b] + d`` takes slot ``seqlen[b] + path[b, d]`` for ``d <
     n_path[b]`` (``path`` / ``n_path`` as :func:`verify_tree` returns them).
-    ``seqlen`` is not advanced.  The sequences' cache rows differ."""
+    ``seqlen`` is not advanced.  The sequences' cache rows differ.  A path that
+    does not rise or leaves the cache sets the device error word and moves
+    nothing of its sequence.  ``kept`` (int32 ``[B]``) receives the rows kept
+    of each sequence: ``n_path``, 0 where it was refused."""
     op = "commit_tree"
     d = rows.index
     if path.ndim != 2:
@@ -1198,10 +1201,15 @@ def commit_tree(rows: CacheRows, seqlen, path, n_path, *, row_map=None) -> None:
             raise ValueError(f"{op}: {B} sequences in a cache of {Bc} rows.")
     elif row_map.numel() != B:
         raise ValueError(f"{op}: row_map needs {B} entries.")
+    if kept is not None:
+        if kept.get_device() != d:
+            _device_error(op, kept, rows.k[0])
+        if kept.dtype != torch.int32 or kept.shape != (B,) or not kept.is_contiguous():
+            raise ValueError(f"{op}: kept must be contiguous int32 {(B,)}, got {kept.dtype} {tuple(kept.shape)}.")
     if B == 0:
         return
     sl, pa, n = _as(seqlen, torch.int64), _as(path, torch.int32), _as(n_path, torch.int32)
     rm = _as(row_map, torch.int32) if row_map is not None else None
-    _launch(lib().maple_commit_tree, op, d, rows.k_ptrs, rows.v_ptrs, len(rows.k), rows.code, B, N, Bc, n_kv,
-            rows.strides[0], rows.strides[1], T, D, sl.data_ptr(), pa.data_ptr(), n.data_ptr(), ptr(rm),
+    _launch(lib().maple_commit_tree_kept, op, d, rows.k_ptrs, rows.v_ptrs, len(rows.k), rows.code, B, N, Bc, n_kv,
+            rows.strides[0], rows.strides[1], T, D, sl.data_ptr(), pa.data_ptr(), n.data_ptr(), ptr(rm), ptr(kept),
             _err(rows.device).data_ptr())

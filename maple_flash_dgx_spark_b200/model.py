@@ -215,15 +215,17 @@ class KVCache:
         """Keep the accepted nodes of the last :meth:`MapleForCausalLM.forward_tree`
         (``path`` / ``n_path`` as ``verify_tree`` returns them): their K/V rows
         close up behind the sequences' positions and the lengths grow by
-        ``n_path``.  ``kept`` are the counts on the host, read (synchronising)
-        where the caller has not got them."""
+        ``n_path``, or not at all where the path was refused (the device error
+        word is set then).  ``kept`` are the counts on the host, read
+        (synchronising) where the caller has not got them."""
         first = 0 if self.slot is None else self.slot
         slots = slice(first, first + path.shape[0])
         if self._rows is None:
             self._rows = CacheRows(self.k, self.v)
-        commit_tree(self._rows, self.seqlen[slots], path, n_path, row_map=self.row_map[slots])
-        self.seqlen[slots].add_(n_path)
-        for i, n in enumerate(n_path.tolist() if kept is None else kept):
+        moved = torch.empty(path.shape[0], dtype=torch.int32, device=self.seqlen.device)
+        commit_tree(self._rows, self.seqlen[slots], path, n_path, row_map=self.row_map[slots], kept=moved)
+        self.seqlen[slots].add_(moved)
+        for i, n in enumerate(moved.tolist() if kept is None else kept):
             self.seen[first + i] += int(n)
 
     def snapshot(self) -> dict:

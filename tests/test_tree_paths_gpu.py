@@ -84,6 +84,44 @@ def test_attention_single_token_is_decode_bf16(cuda, K, D, T):
     assert ((got.double() - want.transpose(1, 2).double()).abs() <= tol + 1e-30).all()
 
 
+# ------------------------------------------------------------- the caches --
+def small_cache(cuda, batch=3, max_len=32, layers=2):
+    from maple_flash_dgx_spark_b200.model import KVCache
+
+    cache = KVCache(["full_attention"] * layers, None, n_kv=2, head_dim=64, max_len=max_len, batch=batch, dtype=BF, device=cuda)
+    for t in cache.k + cache.v:
+        t.normal_()
+    return cache
+
+
+@pytest.mark.parametrize("told", [False, True])
+def test_refused_paths_leave_the_lengths(cuda, K, told):
+    """A path that does not rise, or leaves the cache, moves nothing, so its
+    sequence gets no longer either."""
+    cache = small_cache(cuda, batch=5)
+    lens = [3, 28, 5, 6, 7]
+    cache.seqlen.copy_(torch.tensor(lens))
+    cache.seen = list(lens)
+    path = torch.tensor([[0, 2, 3, -1, -1], [0, 2, 4, -1, -1], [0, 3, 1, -1, -1], [-1] * 5, [0, 1, 2, 3, 4]],
+                        dtype=torch.int32, device=cuda)
+    n = torch.tensor([3, 3, 3, 0, 6], dtype=torch.int32, device=cuda)
+    before = [t.clone() for t in cache.k + cache.v]
+    cache.commit_tree(path, n, kept=[3, 0, 0, 0, 0] if told else None)
+    assert flags(cuda) == 2
+    assert cache.seqlen.tolist() == cache.seen == [6, 28, 5, 6, 7]
+    for t, old in zip(cache.k + cache.v, before):
+        assert torch.equal(t[1:], old[1:])
+        assert torch.equal(t[0, :, [4, 5]], old[0, :, [5, 6]])
+
+
+def test_commit_many_layers_reports_once(cuda, K):
+    cache = small_cache(cuda, batch=2, layers=131)
+    path, n = torch.tensor([[0, 2], [0, 1]], device=cuda), torch.tensor([2, 1], device=cuda)
+    path[0, 1] = 1
+    cache.commit_tree(path, n)
+    assert cache.seqlen.tolist() == cache.seen == [2, 1]
+
+
 # ------------------------------------------------------------ in the model --
 def test_captured_tree_steps(cuda, K):
     """forward_tree, verify_tree and the commit in one graph, replayed as the
