@@ -134,6 +134,10 @@ class KVCache:
         self.row_map = torch.arange(batch, dtype=torch.int32, device=device)
         self.remap = False
         self._rows: CacheRows | None = None
+        # Slots with nodes of a forward_tree that are not committed yet (None: none that is known of), and the
+        # slots of captured ones, whose replays the host does not see
+        self.tree_slots: set[int] | None = None
+        self.captured_slots: set[int] = set()
         self.split_len = attn_split_len(max_len, batch, n_kv)
         # Decode attention on the tensor pipe (the reference's bf16 dots) where
         # the canonical CUDA-core kernel is instruction-bound: caches with more
@@ -170,6 +174,8 @@ class KVCache:
         if not self.remap:
             raise RuntimeError("swap_slots needs cache.remap: without the map the kernels read cache row == slot, "
                                "and a swap would silently read the wrong sequence's K/V.")
+        if self.tree_slots is not None:
+            self.tree_slots = {j if s == i else i if s == j else s for s in self.tree_slots}
         self.row_of[i], self.row_of[j] = self.row_of[j], self.row_of[i]
         self.row_map[i], self.row_map[j] = self.row_map[j].clone(), self.row_map[i].clone()
         self.seen[i], self.seen[j] = self.seen[j], self.seen[i]
@@ -184,6 +190,7 @@ class KVCache:
     def reset_identity(self) -> None:
         self.remap = False
         self.slot = None
+        self.tree_slots = None
         self.row_of = list(range(self.batch))
         self.row_map.copy_(torch.arange(self.batch, device=self.row_map.device, dtype=self.row_map.dtype))
         for b in range(self.batch):
@@ -217,16 +224,32 @@ class KVCache:
         close up behind the sequences' positions and the lengths grow by
         ``n_path``, or not at all where the path was refused (the device error
         word is set then).  ``kept`` are the counts on the host, read
-        (synchronising) where the caller has not got them."""
+        (synchronising) where the caller has not got them.  The slots are those
+        current now (the first ones, or the prefill slot), and need to have had
+        a tree in that step."""
+        if path.dim() != 2 or n_path.numel() != path.shape[0]:
+            raise ValueError(f"commit_tree: path must be [B, N] with B counts, got {tuple(path.shape)} and "
+                             f"{tuple(n_path.shape)}.")
+        bsz, nodes = path.shape
         first = 0 if self.slot is None else self.slot
-        slots = slice(first, first + path.shape[0])
+        if bsz > (self.batch if self.slot is None else 1):
+            raise ValueError(f"commit_tree: {bsz} paths for {self.batch if self.slot is None else 1} cache slots.")
+        if kept is not None and (len(kept) != bsz or not all(0 <= int(n) <= nodes for n in kept)):
+            raise ValueError(f"commit_tree: kept must be {bsz} counts of at most {nodes}, got {list(kept)}.")
+        if self.tree_slots is not None and not (self.tree_slots | self.captured_slots).issuperset(
+                range(first, first + bsz)):
+            raise ValueError(f"commit_tree: slots {first} to {first + bsz - 1}, but the step's nodes to commit are in "
+                             f"slots {sorted(self.tree_slots)}.")
+        slots = slice(first, first + bsz)
         if self._rows is None:
             self._rows = CacheRows(self.k, self.v)
-        moved = torch.empty(path.shape[0], dtype=torch.int32, device=self.seqlen.device)
+        moved = torch.empty(bsz, dtype=torch.int32, device=self.seqlen.device)
         commit_tree(self._rows, self.seqlen[slots], path, n_path, row_map=self.row_map[slots], kept=moved)
         self.seqlen[slots].add_(moved)
         for i, n in enumerate(moved.tolist() if kept is None else kept):
             self.seen[first + i] += int(n)
+        if self.tree_slots is not None:
+            self.tree_slots = self.tree_slots.difference(range(first, first + bsz)) or None
 
     def snapshot(self) -> dict:
         return {"seqlen": self.seqlen.clone(), "seen": list(self.seen), "k": [t.clone() for t in self.k],
@@ -235,6 +258,7 @@ class KVCache:
     def restore(self, snap: dict) -> None:
         self.seqlen.copy_(snap["seqlen"])
         self.seen = list(snap["seen"])
+        self.tree_slots = None
         for dst, src in zip(self.k, snap["k"], strict=True):
             dst.copy_(src)
         for dst, src in zip(self.v, snap["v"], strict=True):
@@ -628,6 +652,10 @@ class MapleForCausalLM:
         hidden = self.embed(tokens.reshape(-1))
         for layer in self.layers:
             hidden = layer(hidden, step.slots, step.slot_rows, self.rotary, cache, tree=step)
+        if torch.cuda.is_current_stream_capturing():
+            cache.captured_slots.update(range(first, first + bsz))
+        else:
+            cache.tree_slots = (cache.tree_slots or set()).union(range(first, first + bsz))
         return self.lm_head(self.norm(hidden)).reshape(bsz, n, self.vocab_size)
 
     @torch.inference_mode()

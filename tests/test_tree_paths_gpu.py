@@ -122,6 +122,61 @@ def test_commit_many_layers_reports_once(cuda, K):
     assert cache.seqlen.tolist() == cache.seen == [2, 1]
 
 
+def one_tree(cuda, model, cache, batch, seed=5):
+    g = torch.Generator().manual_seed(seed)
+    tok = torch.randint(0, 512, (batch, 3), generator=g).to(cuda)
+    par = torch.tensor([[-1, 0, 1]] * batch, dtype=torch.int32, device=cuda)
+    model.forward_tree(tok, par, cache)
+    n = torch.full((batch,), 2, dtype=torch.int32, device=cuda)
+    return torch.tensor([[0, 1, -1]] * batch, dtype=torch.int32, device=cuda), n
+
+
+def test_commit_goes_to_the_slots_of_the_step(cuda, K):
+    """The commit of a tree step is refused for slots that had none in it, and
+    changes nothing then."""
+    model = tiny(cuda, BF)
+    cache = model.make_cache(max_len=32, batch=3)
+    cache.remap = True
+    with cache.prefill_slot(1):
+        path, n = one_tree(cuda, model, cache, 1)
+    with pytest.raises(ValueError, match="slot"):
+        cache.commit_tree(path, n)
+    with cache.prefill_slot(2), pytest.raises(ValueError, match="slot"):
+        cache.commit_tree(path, n)
+    assert cache.seen == cache.seqlen.tolist() == [0, 0, 0]
+    cache.swap_slots(1, 2)  # the sequence is in slot 2 now, with its length and its rows
+    with cache.prefill_slot(1), pytest.raises(ValueError, match="slot"):
+        cache.commit_tree(path, n)
+    with cache.prefill_slot(2):
+        cache.commit_tree(path, n)
+        assert cache.seen == cache.seqlen.tolist() == [0, 0, 2]
+    # a whole batch, committed slot by slot
+    path, n = one_tree(cuda, model, cache, 2)
+    with cache.prefill_slot(1):
+        cache.commit_tree(path[1:], n[1:])
+        with pytest.raises(ValueError, match="slot"):
+            cache.commit_tree(path[1:], n[1:])  # a second time
+    with cache.prefill_slot(0):
+        cache.commit_tree(path[:1], n[:1])
+    assert cache.seen == cache.seqlen.tolist() == [2, 2, 2]
+    # two steps, each in a slot of its own, before their commits
+    for slot in (0, 2):
+        with cache.prefill_slot(slot):
+            path, n = one_tree(cuda, model, cache, 1)
+    with cache.prefill_slot(1), pytest.raises(ValueError, match="slot"):
+        cache.commit_tree(path, n)
+    for slot in (0, 2):
+        with cache.prefill_slot(slot):
+            cache.commit_tree(path, n)
+    assert cache.seen == cache.seqlen.tolist() == [4, 2, 4]
+    # one that was given up
+    one_tree(cuda, model, cache, 2)
+    cache.reset_identity()
+    path, n = one_tree(cuda, model, cache, 3)
+    cache.commit_tree(path, n, kept=[2, 2, 2])
+    assert cache.seen == cache.seqlen.tolist() == [2, 2, 2]
+
+
 # ------------------------------------------------------------ in the model --
 def test_captured_tree_steps(cuda, K):
     """forward_tree, verify_tree and the commit in one graph, replayed as the
