@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 
+import numpy as np
 import torch
 
 from maple_flash_dgx_spark_b200 import _lib
@@ -1140,6 +1141,17 @@ def verify_tree(logits, tokens, parents, uniform, *, temperature: float, top_p: 
     return path, n_path, ids
 
 
+def _rows_overlap(pointers, shape, strides, itemsize: int) -> bool:
+    """Whether two rows ``[T, D]`` of caches ``[Bc, n_kv, T, D]`` at ``pointers``
+    (one shape and stride) share bytes: each row starts behind the one before it
+    in memory."""
+    Bc, n_kv, T, D = shape
+    at = np.asarray(pointers, np.int64)[:, None, None] + itemsize * (
+        np.arange(Bc, dtype=np.int64)[:, None] * strides[0] + np.arange(n_kv, dtype=np.int64) * strides[1])
+    at = np.sort(at, axis=None)
+    return bool((np.diff(at) < T * D * itemsize).any())
+
+
 class CacheRows:
     """The K and V caches of all layers for :func:`commit_tree`: looked over
     once and held as a table of device pointers (the caches stay where they
@@ -1164,9 +1176,8 @@ class CacheRows:
                                  f"{tuple(first.shape)}.")
             if t.dtype != first.dtype:
                 raise TypeError(f"{op}: caches of {first.dtype} and {t.dtype}.")
-        # rows are moved in place, so none may be another's: nor one tensor's twice (expanded), nor two tensors'
-        if any(n > 1 and s < first.shape[2] * first.shape[3] for n, s in zip(first.shape[:2], first.stride()[:2])) or \
-                len({t.data_ptr() for t in k + v}) < len(k + v):
+        # rows are moved in place, so none may share memory with another: nor in one tensor (expanded), nor in two
+        if _rows_overlap([t.data_ptr() for t in k + v], first.shape, first.stride(), first.element_size()):
             raise ValueError(f"{op}: the caches' rows overlap.")
         self.k, self.v = k, v
         self.shape = tuple(int(x) for x in first.shape)

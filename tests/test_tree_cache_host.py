@@ -1,6 +1,10 @@
-"""Speculative decoding, host side (no GPU): the cache's checks before a commit."""
+"""Speculative decoding, host side (no GPU): the cache's checks before a commit, and
+which caches' rows share memory."""
 
 from __future__ import annotations
+
+import itertools
+import random
 
 import pytest
 
@@ -33,3 +37,25 @@ def test_commit_tree_checks_slots_and_counts():
     refused(path[:1], n[:1])
     with cache.prefill_slot(2):
         refused(path[:1], n[:1])
+
+
+def test_rows_that_share_memory():
+    """Against every pair of rows compared, over strides in any order, gaps,
+    overlaps by one position and caches in one another's gaps."""
+    from maple_flash_dgx_spark_b200.kernels import _rows_overlap
+
+    r, seen = random.Random(3), set()
+    for _ in range(4000):
+        Bc, n_kv, T, D, es = r.randint(1, 3), r.randint(1, 3), r.randint(1, 3), 8, r.choice([2, 4])
+        R = T * D
+        strides = [r.choice([0, R - D, R, 2 * R - D, 2 * R, 2 * R + D, 3 * R, 4 * R, 6 * R]) for _ in range(2)]
+        ptrs = [4096 + es * r.choice([0, D, R, 2 * R, 3 * R, 6 * R, 9 * R, 40 * R]) for _ in range(r.randint(1, 3))]
+        starts = [(p + es * (b * strides[0] + h * strides[1])) for p in ptrs for b in range(Bc) for h in range(n_kv)]
+        want = any(abs(x - y) < R * es for x, y in itertools.combinations(starts, 2))
+        assert _rows_overlap(ptrs, (Bc, n_kv, T, D), (*strides, D, 1), es) == want
+        seen.add((want, len(ptrs) > 1, Bc * n_kv > 1))
+    assert len(seen) == 7  # one row of one cache has nothing to overlap with
+    assert not _rows_overlap([0], (0, 2, 4, 8), (64, 32, 8, 1), 2)
+    # offsets past 32 bits
+    assert not _rows_overlap([0, 1 << 40], (64, 8, 1 << 20, 128), (1 << 30, 1 << 27, 128, 1), 2)
+    assert _rows_overlap([0, 1 << 33], (64, 8, 1 << 20, 128), (1 << 30, 1 << 27, 128, 1), 2)

@@ -122,6 +122,30 @@ def test_commit_many_layers_reports_once(cuda, K):
     assert cache.seqlen.tolist() == cache.seen == [2, 1]
 
 
+def test_overlapping_caches_are_refused(cuda, K):
+    """Rows move in place: no strides or views that let two of them share elements."""
+    R = 30 * 64
+
+    def view(strides, shift=0, base=torch.zeros(1 << 15, dtype=BF, device=cuda)):
+        return base.as_strided((2, 2, 30, 64), (*strides, 64, 1), shift)
+
+    def apart(strides):
+        return view(strides, base=torch.zeros(1 << 15, dtype=BF, device=cuda))
+
+    for k, v in ((view((R, R)), apart((R, R))),                             # head 1 of one is head 0 of the next
+                 (view((R, 2 * R - 64)), apart((R, 2 * R - 64))),           # by a position
+                 (view((2 * R, R)), view((2 * R, R), 64)),                  # two caches, a position apart
+                 (view((2 * R, R)), view((2 * R, R), 2 * R))):              # one's second sequence, the other's first
+        with pytest.raises(ValueError, match="overlap"):
+            K.CacheRows([k], [v])
+    K.CacheRows([view((3 * R, 2 * R))], [apart((3 * R, 2 * R))])            # rows 0, 2, 3 and 5
+    K.CacheRows([view((4 * R, R))], [view((4 * R, R), 2 * R)])              # each in the other's gaps
+    for perm in ((0, 1, 2), (1, 0, 2), (2, 0, 1), (1, 2, 0)):               # of (K or V, sequence, head)
+        size = [(2, 3, 4)[p] for p in perm]
+        both = torch.zeros(*size, 30, 64, dtype=BF, device=cuda).permute(*[perm.index(i) for i in range(3)], 3, 4)
+        K.CacheRows([both[0]], [both[1]])
+
+
 def one_tree(cuda, model, cache, batch, seed=5):
     g = torch.Generator().manual_seed(seed)
     tok = torch.randint(0, 512, (batch, 3), generator=g).to(cuda)
