@@ -407,8 +407,9 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     const unsigned lanes = (unsigned)(warp & 3) << 21;  // TMEM lane base of this warp, in bits 31:16
     const unsigned t_s = tmem + lanes + w * kTtKeys, t_o = tmem + lanes + 2 * kTtKeys;
     const float ninf = __int_as_float(0xff800000);
-    // above 0, so that a masked score of -inf stays one under scale 0
-    const float c = fmaxf(fabsf(p.scale) * 1.44269504088896341f, 1e-30f);
+    // above 0, so that a masked score of -inf stays one under scale 0: by the least fp32, 2^-149, which makes
+    // no more than 2^-21 of any score
+    const float c = fmaxf(fabsf(p.scale) * 1.44269504088896341f, __int_as_float(1));
     const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;  // the queries carry the scale's sign
     const int rows = p.N * p.G;
     // row / G by a multiplication: exact while row x G < 2^32

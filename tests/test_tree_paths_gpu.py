@@ -84,6 +84,19 @@ def test_attention_single_token_is_decode_bf16(cuda, K, D, T):
     assert ((got.double() - want.transpose(1, 2).double()).abs() <= tol + 1e-30).all()
 
 
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (BF, 256), (F32, 128)])
+@pytest.mark.parametrize("scale", [2.0 ** -116, -(2.0 ** -110), 1e-33, 0.0])
+def test_attention_tiny_scales(cuda, K, dtype, D, scale):
+    """Scales far below 1 with keys as far above it (both types reach 2^127):
+    scores near 1; and a scale of 0, whose weights are all the same."""
+    c = attn_case(46, 2, 6, 8, 2, D, 300, [250, 17], dtype)
+    c["scale"] = scale
+    c["k"] = c["k"] * (2.0 ** 113 if scale == 0 else 0.25 / abs(scale))
+    got = run_attn(K, c)
+    want, mass, reach = ref.attention(c["q"], c["k"], c["v"], c["lens"], c["mask"], None, scale, 0)
+    check_attention(got, want, mass, reach.abs(), dtype, 256)
+
+
 # ------------------------------------------------------------- the caches --
 def small_cache(cuda, batch=3, max_len=32, layers=2):
     from maple_flash_dgx_spark_b200.model import KVCache
