@@ -11,7 +11,6 @@ from __future__ import annotations
 import ctypes
 import functools
 
-import numpy as np
 import torch
 
 from maple_flash_dgx_spark_b200 import _lib
@@ -1146,10 +1145,9 @@ def _rows_overlap(pointers, shape, strides, itemsize: int) -> bool:
     (one shape and stride) share bytes: each row starts behind the one before it
     in memory."""
     Bc, n_kv, T, D = shape
-    at = np.asarray(pointers, np.int64)[:, None, None] + itemsize * (
-        np.arange(Bc, dtype=np.int64)[:, None] * strides[0] + np.arange(n_kv, dtype=np.int64) * strides[1])
-    at = np.sort(at, axis=None)
-    return bool((np.diff(at) < T * D * itemsize).any())
+    at = torch.tensor(pointers, dtype=torch.int64)[:, None, None] + itemsize * (
+        torch.arange(Bc)[:, None] * strides[0] + torch.arange(n_kv) * strides[1])
+    return bool((at.reshape(-1).sort().values.diff() < T * D * itemsize).any())
 
 
 class CacheRows:
