@@ -1145,8 +1145,8 @@ def _rows_overlap(pointers, shape, strides, itemsize: int) -> bool:
     (one shape and stride) share bytes: each row starts behind the one before it
     in memory."""
     Bc, n_kv, T, D = shape
-    at = torch.tensor(pointers, dtype=torch.int64)[:, None, None] + itemsize * (
-        torch.arange(Bc)[:, None] * strides[0] + torch.arange(n_kv) * strides[1])
+    at = torch.tensor(pointers, dtype=torch.int64, device="cpu")[:, None, None] + itemsize * (
+        torch.arange(Bc, device="cpu")[:, None] * strides[0] + torch.arange(n_kv, device="cpu") * strides[1])
     return bool((at.reshape(-1).sort().values.diff() < T * D * itemsize).any())
 
 
