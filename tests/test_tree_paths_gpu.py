@@ -97,6 +97,33 @@ def test_attention_tiny_scales(cuda, K, dtype, D, scale):
     check_attention(got, want, mass, reach.abs(), dtype, 256)
 
 
+# ------------------------------------------- arguments at their types' ends --
+def test_whole_numbers_past_32_bits(cuda, K):
+    """int64 parents, paths, counts and cache rows that int32 does not hold are
+    out of range, not their low words."""
+    big = 1 << 32
+    plan = K.tree_plan(torch.tensor([[-1, 0, big, 1, -big - 1]], device=cuda))
+    assert flags(cuda) == 2 and plan.mask.tolist() == [[1, 3, 0, 11, 0]]
+    logits, tok, par, u, _ = verify_inputs(51, 1, 4, 50, chain=True)
+    kw = dict(temperature=1.0, top_p=1.0, top_k=20)
+    args = (logits, torch.from_numpy(tok).to(cuda))
+    path, n, ids = K.verify_tree(*args, torch.tensor([[-1, big, big, big]], device=cuda), torch.zeros(1, 4, device=cuda), **kw)
+    assert flags(cuda) == 2 and n.tolist() == [1] and path.tolist() == [[0, -1, -1, -1]]
+    k, v = (torch.randn(2, 2, 20, 64, device=cuda).to(BF) for _ in range(2))
+    keep = k.clone(), v.clone()
+    rows, s = K.CacheRows([k], [v]), torch.tensor([4, 5], device=cuda)
+    good, cnt = torch.tensor([[0, 2, -1], [0, 2, -1]], device=cuda), torch.tensor([2, 2], device=cuda)
+    for path, n, row_map in ((good + torch.tensor([0, big, 0], device=cuda), cnt, None), (good, cnt + big, None),
+                             (good, cnt, torch.tensor([big, big + 1], device=cuda))):
+        K.commit_tree(rows, s, path, n, row_map=row_map)
+        assert flags(cuda) == 2
+        assert torch.equal(k, keep[0]) and torch.equal(v, keep[1])
+    c = attn_case(52, 2, 3, 4, 2, 64, 40, [3, 4], BF, rows=[0, 1])
+    got = K.tree_gqa_attn(c["q"], c["k"], c["v"], torch.tensor([3, 4], device=cuda), torch.from_numpy(c["mask"]).to(cuda),
+                          row_map=torch.tensor([0, big + 1], device=cuda), scale=1.0)
+    assert flags(cuda) == 2 and (got[1] == 0).all() and (got[0] != 0).any()
+
+
 # ------------------------------------------------------------- the caches --
 def small_cache(cuda, batch=3, max_len=32, layers=2):
     from maple_flash_dgx_spark_b200.model import KVCache
