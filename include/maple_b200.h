@@ -509,7 +509,7 @@ int maple_tree_gqa_attn(const void* q, int x_dtype, int64_t batch, int64_t nodes
  * logits [batch, nodes, vocab] (f32 or bf16, element strides l_sb, l_sn),
  * draft_probs likewise; tokens, parents, uniform [batch, nodes] contiguous.
  * path [batch, nodes]: the accepted nodes, node 0 first, then -1; n_path: their
- * number (0 where node 0 is padding); out [batch, nodes]: the n_path tokens
+ * number (0 where node 0 is padding, or has a parent); out [batch, nodes]: the n_path tokens
  * drawn, the last one from the target itself, then -1.  A drafted token outside
  * the vocabulary is refused and sets bit 2 of *err, as a parent >= its node
  * does.  NaN logits rank lowest.  Workspace as above, 16-byte aligned. */

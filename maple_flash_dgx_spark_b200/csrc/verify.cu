@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kVerWalkThreads) verify_walk_kernel(VerifyPara
   if (wrong) atomicOr(p.err, kErrFlagBounds);
   __syncwarp();
   int kept = 0;
-  if (__shfl_sync(0xffffffffu, par[0], 0) >= -1) {
+  if (__shfl_sync(0xffffffffu, par[0], 0) == -1) {  // below it padding, above it not before its node: padding too
     const float u0 = __shfl_sync(0xffffffffu, un[0], 0);
     int cur = 0, done = 0;  // children up to `done` have been tried
     double pr[2], q[2], left = 1.0;

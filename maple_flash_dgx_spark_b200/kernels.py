@@ -1100,7 +1100,8 @@ def verify_tree(logits, tokens, parents, uniform, *, temperature: float, top_p: 
     Returns ``(path, n_path, ids)``: ``path`` int32 ``[B, N]`` the accepted
     nodes from node 0 on, then -1; ``n_path`` int32 ``[B]``; ``ids`` int64
     ``[B, N]`` the ``n_path`` tokens drawn, then -1.  A sequence whose node 0 is
-    padding has ``n_path`` 0."""
+    padding (or has a parent, which :func:`tree_plan` makes padding) has
+    ``n_path`` 0."""
     op = "verify_tree"
     if logits.ndim != 3:
         raise ValueError(f"{op} expects logits [B, N, V], got {tuple(logits.shape)}.")

@@ -124,6 +124,20 @@ def test_whole_numbers_past_32_bits(cuda, K):
     assert flags(cuda) == 2 and (got[1] == 0).all() and (got[0] != 0).any()
 
 
+def test_verify_node_0_with_a_parent_is_padding(cuda, K):
+    """As in the plan: a parent that is not before its node makes it padding, and
+    a sequence whose node 0 is padding draws nothing."""
+    logits, tok, _, u, q = verify_inputs(53, 4, 5, 60, draft=F32)
+    par = torch.tensor([[0, 0, 1, 0, 0], [3, 0, 0, 0, 0], [-1, 0, 1, 1, 2], [-2, 0, 1, 1, 2]], dtype=torch.int32, device=cuda)
+    assert (K.tree_plan(par).mask[[0, 1, 3]] == 0).all() and flags(cuda) == 2
+    for draft in (None, q):
+        path, n, ids = K.verify_tree(logits, torch.from_numpy(tok).to(cuda), par, torch.zeros_like(torch.from_numpy(u)).to(cuda),
+                                     temperature=1.0, top_p=1.0, top_k=20, draft_probs=draft)
+        assert flags(cuda) == 2
+        assert n[[0, 1, 3]].tolist() == [0, 0, 0] and int(n[2]) >= 1
+        assert (path[[0, 1, 3]] == -1).all() and (ids[[0, 1, 3]] == -1).all()
+
+
 # ------------------------------------------------------------- the caches --
 def small_cache(cuda, batch=3, max_len=32, layers=2):
     from maple_flash_dgx_spark_b200.model import KVCache
