@@ -632,7 +632,7 @@ class MapleForCausalLM:
     def forward_tree(self, tokens: torch.Tensor, parents: torch.Tensor | TreePlan, cache: KVCache) -> torch.Tensor:
         """Logits ``[B, N, V]`` of every node of ``B`` trees of drafted tokens
         (``tokens`` and ``parents`` ``[B, N]``, node 0 the last drawn token; see
-        :func:`kernels.tree_plan`) over the first ``B`` slots of ``cache``, or
+        :func:`kernels.tree_plan`; the tokens of padding are not looked at) over the first ``B`` slots of ``cache``, or
         its prefill slot.  The nodes' K/V rows go to the slots behind each
         sequence's positions; :meth:`KVCache.commit_tree` keeps those that
         ``verify_tree`` accepts.  The lengths stay as they are."""
@@ -649,7 +649,7 @@ class MapleForCausalLM:
         self.rotary.ensure_length(cache.max_len)
         slots = slice(first, first + bsz)
         step = TreeStep(plan, cache.seqlen[slots], cache.row_map[slots], self.rotary)
-        hidden = self.embed(tokens.reshape(-1))
+        hidden = self.embed(tokens.masked_fill(plan.mask == 0, 0).reshape(-1))  # whatever stands at padding
         for layer in self.layers:
             hidden = layer(hidden, step.slots, step.slot_rows, self.rotary, cache, tree=step)
         if torch.cuda.is_current_stream_capturing():

@@ -256,6 +256,21 @@ def test_commit_goes_to_the_slots_of_the_step(cuda, K):
 
 
 # ------------------------------------------------------------ in the model --
+def test_tokens_of_padding_are_not_looked_at(cuda, K):
+    """Padding is the parents' alone: -1, as verify_tree fills its ids with, may
+    stand there."""
+    model = tiny(cuda, BF)
+    cache = model.make_cache(max_len=32, batch=2)
+    par = torch.tensor([[-1, 0, 0, 1], [-1, 0, -2, -2]], dtype=torch.int32, device=cuda)
+    tok = torch.tensor([[3, 4, 5, 6], [7, 8, 0, 0]], device=cuda)
+    want = model.forward_tree(tok, par, cache)
+    odd = tok.clone()
+    odd[1, 2:] = torch.tensor([-1, 1 << 40])
+    got = model.forward_tree(odd, par, cache)
+    assert flags(cuda) == 0
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1, :2], want[1, :2])
+
+
 def test_captured_tree_steps(cuda, K):
     """forward_tree, verify_tree and the commit in one graph, replayed as the
     sequences grow, against the same steps called."""
