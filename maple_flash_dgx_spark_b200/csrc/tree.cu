@@ -677,7 +677,7 @@ inline bool tree_use_tc(int x_dtype, int64_t head_dim) {
 inline int tree_splits(int64_t batch, int64_t nodes, int64_t num_heads, int64_t num_kv_heads, int64_t max_len,
                        int x_dtype, int64_t head_dim, int64_t window, bool* join) {
   *join = false;
-  if (window > 0 && window + nodes < max_len) max_len = window + nodes;  // no row's keys span more
+  if (window > 0 && window < max_len - nodes) max_len = window + nodes;  // no row's keys span more
   const int64_t rows = nodes * (num_heads / num_kv_heads);
   if (tree_use_tc(x_dtype, head_dim))
     return tree_tc_splits(batch * num_kv_heads * tree_tc_groups(rows), max_len, rows > tree_tc_partial_rows(1), join);

@@ -1,5 +1,5 @@
-"""Speculative decoding, host side (no GPU): the cache's checks before a commit, and
-which caches' rows share memory."""
+"""Speculative decoding, host side (no GPU): the cache's checks before a commit,
+which caches' rows share memory, and the split rule at its arguments' ends."""
 
 from __future__ import annotations
 
@@ -9,6 +9,15 @@ import random
 import pytest
 
 torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def L():
+    from maple_flash_dgx_spark_b200 import _lib
+    from maple_flash_dgx_spark_b200.build import build
+
+    build()
+    return _lib.lib()
 
 
 def test_commit_tree_checks_slots_and_counts():
@@ -59,3 +68,15 @@ def test_rows_that_share_memory():
     # offsets past 32 bits
     assert not _rows_overlap([0, 1 << 40], (64, 8, 1 << 20, 128), (1 << 30, 1 << 27, 128, 1), 2)
     assert _rows_overlap([0, 1 << 33], (64, 8, 1 << 20, 128), (1 << 30, 1 << 27, 128, 1), 2)
+
+
+@pytest.mark.parametrize("dtype,D", [(1, 64), (1, 128), (1, 256), (0, 128)])
+def test_windows_past_every_cache_split_as_none(L, dtype, D):
+    """A window no position is outside of leaves the splits as they are, the
+    largest number as well."""
+    def size(window):
+        return L.maple_tree_gqa_workspace_bytes(1, 64, 32, 4, D, 65536, window, dtype)
+
+    assert size(0) > 0
+    for window in (65536, 1 << 31, 1 << 62, (1 << 63) - 60, (1 << 63) - 1):
+        assert size(window) == size(0), window
