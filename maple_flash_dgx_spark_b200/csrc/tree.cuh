@@ -1,5 +1,5 @@
-// Attention over a KV cache for trees of drafted tokens: what the CUDA-core
-// and the tcgen05 kernels share (arguments, visibility, the split of a row's
+// Attention over a KV cache for trees of drafted tokens: what the mma.sync and
+// the tcgen05 kernels share (arguments, visibility, the split of a row's
 // keys and the layout of the partial results).
 //
 // A sequence has s = seqlen[b] cached positions and N <= 64 drafted nodes

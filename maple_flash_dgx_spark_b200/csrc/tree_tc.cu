@@ -62,7 +62,7 @@ constexpr float kTtGrow = 8.0f;  // log2 growth of a row's maximum that rescales
 
 struct TtItem {
   int b, h, rt, sp;     // sequence, KV head, row tile (pair), split
-  int s, lo, k0, k1;    // cached positions, the row's first key, this split's keys
+  int s, k0, k1;        // cached positions, this split's keys
   int item, tiles, used, fix, dmax;  // key tiles; splits that hold keys; V was cleared; largest depth
   unsigned long long mask[kTreeMaxNodes];
 };
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       it.mask[lane + 32] = m[1];
       if (lane == 0) {
         it.item = item; it.b = b; it.h = h; it.rt = rt; it.sp = sp;
-        it.s = rg.s; it.lo = rg.lo; it.k0 = k0; it.k1 = k1; it.tiles = tiles; it.fix = 0; it.dmax = dm;
+        it.s = rg.s; it.k0 = k0; it.k1 = k1; it.tiles = tiles; it.fix = 0; it.dmax = dm;
         it.used = tree_splits_used(rg.lo, rg.hi, kTtKeys, p.NS);
       }
       __syncwarp();
