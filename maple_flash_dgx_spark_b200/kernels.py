@@ -1151,9 +1151,17 @@ def verify_tree(logits, tokens, parents, uniform, *, temperature: float, top_p: 
 
 def _rows_overlap(pointers, shape, strides, itemsize: int) -> bool:
     """Whether two rows ``[T, D]`` of caches ``[Bc, n_kv, T, D]`` at ``pointers``
-    (one shape and stride) share bytes: each row starts behind the one before it
-    in memory."""
+    (one shape and stride) share bytes."""
     Bc, n_kv, T, D = shape
+    # plain layouts in a few comparisons: the dimensions nest, and each cache ends before the next begins
+    end, nested = T * D, True
+    for s, n in sorted((s, n) for s, n in zip(strides, (Bc, n_kv)) if n > 1):
+        nested = nested and s >= end
+        end += s * (n - 1)
+    order = sorted(pointers)
+    if nested and all(y - x >= end * itemsize for x, y in zip(order, order[1:])):
+        return False
+    # any others: every row starts behind the end of the one before it
     at = torch.tensor(pointers, dtype=torch.int64, device="cpu")[:, None, None] + itemsize * (
         torch.arange(Bc, device="cpu")[:, None] * strides[0] + torch.arange(n_kv, device="cpu") * strides[1])
     return bool((at.reshape(-1).sort().values.diff() < T * D * itemsize).any())
