@@ -240,12 +240,14 @@ class KVCache:
                 range(first, first + bsz)):
             raise ValueError(f"commit_tree: slots {first} to {first + bsz - 1}, but the step's nodes to commit are in "
                              f"slots {sorted(self.tree_slots)}.")
-        slots = slice(first, first + bsz)
+        seqlen, row_map = self.seqlen, self.row_map
+        if bsz != self.batch:
+            seqlen, row_map = seqlen[first:first + bsz], row_map[first:first + bsz]
         if self._rows is None:
             self._rows = CacheRows(self.k, self.v)
-        moved = torch.empty(bsz, dtype=torch.int32, device=self.seqlen.device)
-        commit_tree(self._rows, self.seqlen[slots], path, n_path, row_map=self.row_map[slots], kept=moved)
-        self.seqlen[slots].add_(moved)
+        moved = torch.empty(bsz, dtype=torch.int32, device=seqlen.device)
+        commit_tree(self._rows, seqlen, path, n_path, row_map=row_map, kept=moved)
+        seqlen.add_(moved)
         for i, n in enumerate(moved.tolist() if kept is None else kept):
             self.seen[first + i] += int(n)
         if self.tree_slots is not None:
