@@ -464,10 +464,14 @@ int maple_dequantize_rtn(const uint32_t* packed, const float* scales, const floa
  * that was drawn, not yet in the cache.  The nodes' K/V rows stand in the cache
  * behind the sequence's seqlen positions, node j at slot seqlen + j.
  *
+ * maple_narrow_int64: out[i] = x[i] as int32, numbers past it as its ends (for
+ * parents, paths, counts and cache rows in 64 bits: the ends are none of any).
+ *
  * maple_tree_plan: mask[i] = bit i and the bits of node i's ancestors, depth[i]
  * = their number (both [batch, nodes], contiguous; 0 for padding).  parents:
  * element strides p_sb, p_sn.  A parent >= i sets bit 2 of *err; the node and
  * what hangs on it become padding. */
+int maple_narrow_int64(const int64_t* x, int64_t n, int32_t* out, void* stream);
 int maple_tree_plan(const int32_t* parents, int64_t batch, int64_t nodes, int64_t p_sb, int64_t p_sn, int64_t* mask,
                     int32_t* depth, int* err, void* stream);
 

@@ -113,6 +113,7 @@ _SIGS: dict[str, tuple] = {
     "maple_fused_sample": (i32, [vp, i32, i64, i64, i64, vp, f32, f32, i64, vp, vp, i64, vp]),
     "maple_embedding": (i32, [vp, i64, vp, i32, i64, i64, vp, i32, i64, vp, vp]),
     "maple_rtn4_embedding": (i32, [vp, i64, vp, vp, vp, i32, i64, i64, i64, vp, i32, i64, vp, vp]),
+    "maple_narrow_int64": (i32, [vp, i64, vp, vp]),
     "maple_tree_plan": (i32, [vp, i64, i64, i64, i64, vp, vp, vp, vp]),
     "maple_tree_gqa_workspace_bytes": (i64, [i64, i64, i64, i64, i64, i64, i64, i32]),
     "maple_tree_gqa_attn": (i32, [vp, i32, i64, i64, i64, i64, i64, i64, vp, vp, i64, i64, i64, i64, i64, i64, vp, vp,

@@ -63,6 +63,18 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(const int32_t* parents, 
   if (wrong) atomicOr(err, kErrFlagBounds);
 }
 
+// ----------------------------------------------------------------- narrow --
+// Saturating, so that no number past int32 turns into a node or a cache row.
+// A few hundred numbers: the launch is the bound.
+__global__ void __launch_bounds__(256) narrow_kernel(const int64_t* x, int64_t n, int32_t* out) {
+  pdl_wait();
+  pdl_trigger();
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t v = x[i];
+    out[i] = v > INT32_MAX ? INT32_MAX : v < INT32_MIN ? INT32_MIN : (int32_t)v;
+  }
+}
+
 // ------------------------------------- attention, fp32 and heads of 256 --
 // One CTA per (split of the keys, KV head and tile of query rows, sequence).
 // Row r of a KV head is node r / G, query head h G + r % G; a warp has 16 rows
@@ -697,6 +709,16 @@ inline int64_t tree_partial_bytes(int64_t batch, int64_t num_kv_heads, int64_t r
 }  // namespace mb
 
 using namespace mb;
+
+extern "C" int maple_narrow_int64(const int64_t* x, int64_t n, int32_t* out, void* stream) {
+  if (n < 0) return kErrShape;
+  if (n == 0) return kOk;
+  if (!x || !out) return kErrShape;
+  const int64_t blocks = (n + 255) / 256;
+  const cudaError_t e = launch_k(narrow_kernel, dim3((unsigned)(blocks < 592 ? blocks : 592)), dim3(256), 0,
+                                 static_cast<cudaStream_t>(stream), x, n, out);
+  return e == cudaSuccess ? kOk : kErrCuda;
+}
 
 extern "C" int maple_tree_plan(const int32_t* parents, int64_t batch, int64_t nodes, int64_t p_sb, int64_t p_sn,
                                int64_t* mask, int32_t* depth, int* err, void* stream) {

@@ -955,12 +955,15 @@ def _as(t, dtype):
     return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
-def _as_int32(t):
-    """Contiguous int32; numbers that it does not hold become its ends, which no
-    operator takes for a node, a count or a cache row."""
-    if t.dtype == torch.int64:
-        t = t.clamp(-(1 << 31), (1 << 31) - 1)
-    return _as(t, torch.int32)
+def _as_int32(t, op, d):
+    """Contiguous int32 of a tensor on GPU ``d``; numbers that it does not hold
+    become its ends, which no operator takes for a node, a count or a cache row."""
+    if t.dtype != torch.int64:
+        return _as(t, torch.int32)
+    t = t.contiguous()
+    out = torch.empty(t.shape, dtype=torch.int32, device=t.device)
+    _launch(lib().maple_narrow_int64, op, d, t.data_ptr(), t.numel(), out.data_ptr())
+    return out
 
 
 def _bad_nodes(op, n):
@@ -997,7 +1000,7 @@ def tree_plan(parents: torch.Tensor) -> TreePlan:
         _device_error(op, parents)
     if parents.dtype != torch.int32 and (parents.is_floating_point() or parents.dtype == torch.bool):
         raise TypeError(f"{op}: parents must be whole numbers, got {parents.dtype}.")
-    par = _as_int32(parents)
+    par = _as_int32(parents, op, d)
     dev = par.device
     mask, depth = torch.empty_like(par, dtype=torch.int64), torch.empty_like(par)
     _launch(lib().maple_tree_plan, op, d, par.data_ptr(), B, N, N, 1, mask.data_ptr(), depth.data_ptr(),
@@ -1065,7 +1068,7 @@ def tree_gqa_attn(q, k_cache, v_cache, seqlen, tree_mask, *, row_map=None, scale
             q = q.clone()
         qb, qn, qh, qd = q.stride()
     sl, tm = _as(seqlen, torch.int64), _as(tree_mask, torch.int64)
-    rm = _as_int32(row_map) if row_map is not None else None
+    rm = _as_int32(row_map, op, d) if row_map is not None else None
     dev = q.device
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0:
@@ -1134,7 +1137,7 @@ def verify_tree(logits, tokens, parents, uniform, *, temperature: float, top_p: 
         dcode = dtype_code(draft_probs, op)
         dp = draft_probs if draft_probs.stride(2) == 1 else draft_probs.contiguous()
         db, dn, _ = dp.stride()
-    tok, par, u = _as(tokens, torch.int64), _as_int32(parents), _as(uniform, torch.float32)
+    tok, par, u = _as(tokens, torch.int64), _as_int32(parents, op, d), _as(uniform, torch.float32)
     dev = lg.device
     path, ids = torch.empty_like(par), torch.empty_like(tok)
     n_path = torch.empty(B, dtype=torch.int32, device=dev)
@@ -1234,8 +1237,8 @@ def commit_tree(rows: CacheRows, seqlen, path, n_path, *, row_map=None, kept=Non
             raise ValueError(f"{op}: kept must be contiguous int32 {(B,)}, got {kept.dtype} {tuple(kept.shape)}.")
     if B == 0:
         return
-    sl, pa, n = _as(seqlen, torch.int64), _as_int32(path), _as_int32(n_path)
-    rm = _as_int32(row_map) if row_map is not None else None
+    sl, pa, n = _as(seqlen, torch.int64), _as_int32(path, op, d), _as_int32(n_path, op, d)
+    rm = _as_int32(row_map, op, d) if row_map is not None else None
     _launch(lib().maple_commit_tree_kept, op, d, rows.k_ptrs, rows.v_ptrs, len(rows.k), rows.code, B, N, Bc, n_kv,
             rows.strides[0], rows.strides[1], T, D, sl.data_ptr(), pa.data_ptr(), n.data_ptr(), ptr(rm), ptr(kept),
             _err(rows.device).data_ptr())

@@ -80,3 +80,10 @@ def test_windows_past_every_cache_split_as_none(L, dtype, D):
     assert size(0) > 0
     for window in (65536, 1 << 31, 1 << 62, (1 << 63) - 60, (1 << 63) - 1):
         assert size(window) == size(0), window
+
+
+def test_narrowing_refuses_before_any_launch(L):
+    assert L.maple_narrow_int64(256, 0, 256, None) == 0
+    assert L.maple_narrow_int64(256, -1, 256, None) == 1
+    assert L.maple_narrow_int64(None, 4, 256, None) == 1
+    assert L.maple_narrow_int64(256, 4, None, None) == 1

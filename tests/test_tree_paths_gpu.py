@@ -124,6 +124,21 @@ def test_whole_numbers_past_32_bits(cuda, K):
     assert flags(cuda) == 2 and (got[1] == 0).all() and (got[0] != 0).any()
 
 
+@pytest.mark.parametrize("n", [0, 1, 255, 256, 257, 300000])
+def test_narrowing_saturates(cuda, K, n):
+    g = torch.Generator().manual_seed(n)
+    x = torch.randint(-(1 << 33), 1 << 33, (n, 2), generator=g)
+    x[: n // 3] >>= 12
+    ends = [v for e in (1 << 31, 1 << 32, 1 << 63) for v in (e - 2, e - 1, e, e + 1, -e - 1, -e, -e + 1)]
+    ends = torch.tensor([v for v in ends if -(1 << 63) <= v < 1 << 63])
+    x[: ends.numel(), 0] = ends[:n]
+    want = x.clamp(-(1 << 31), (1 << 31) - 1).int()
+    x = x.to(cuda)
+    for got, w in ((K._as_int32(x, "narrow", 0), want), (K._as_int32(x[:, 0], "narrow", 0), want[:, 0]),
+                   (K._as_int32(x[:, 1].int(), "narrow", 0), x[:, 1].int().cpu())):
+        assert got.dtype == torch.int32 and got.is_contiguous() and torch.equal(got.cpu(), w)
+
+
 def test_verify_node_0_with_a_parent_is_padding(cuda, K):
     """As in the plan: a parent that is not before its node makes it padding, and
     a sequence whose node 0 is padding draws nothing."""
