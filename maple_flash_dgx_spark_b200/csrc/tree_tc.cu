@@ -19,8 +19,9 @@
 // a unit's scores overwrite its predecessor's weights right behind the product
 // that read them.  Because scores are committed behind that product, a
 // warpgroup that sees them knows its output is at rest, and may rescale it;
-// it does so only when a row's maximum has grown by more than 2^8 (the weights
-// then still fit fp32 and bf16 many times over).
+// it does so only when a row's maximum has grown by more than 2^8.  The weights
+// are relative to 2^8 times the maximum of the last time, so that they are at
+// most 1, as are their products with V at most V: fp32 holds these for any V.
 //
 // An item is one split of one sequence's keys for one KV head and row tile (or
 // pair).  With JOIN a CTA has one item, and the splits of a row tile form a
@@ -58,7 +59,7 @@ constexpr int kTtRows = 128;   // rows per tile: MMA M
 constexpr int kTtThreads = 384;
 constexpr int kTtInfo = 2;     // items known ahead
 constexpr int kTtCluster = 8;  // splits that a cluster joins (the portable size)
-constexpr float kTtGrow = 8.0f;  // log2 growth of a row's maximum that rescales
+constexpr float kTtGrow = 8.0f;  // log2 growth of a row's maximum that rescales, and what weights leave for it
 
 struct TtItem {
   int b, h, rt, sp;     // sequence, KV head, row tile (pair), split
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         }
       }
       const int64_t out = (((int64_t)b * p.N + node) * p.H + head) * D;
-      float mc = ninf, l = 0.0f;  // maximum times c, sum of weights
+      float mc = ninf, l = 0.0f;  // what weights are relative to (a maximum times c, and kTtGrow), their sum
       int mine_units = 0;
       if (tiles > 0) {
         // Q, 128-byte swizzled: the warpgroup's own tile, or half of the shared one each
@@ -528,10 +529,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             // a row's new maximum, and its output and sum brought to it where it has grown enough
             auto settle = [&](float top) {
               const float tc = top * c;
-              const bool grow = tc > mc + kTtGrow || (mc == ninf && tc > ninf);
+              const bool grow = tc > mc;
               if (!__any_sync(0xffffffffu, grow)) return;
-              const float f = grow ? (mc == ninf ? 0.0f : ex2(mc - tc)) : 1.0f;
-              if (grow) mc = tc;
+              const float f = grow ? (mc == ninf ? 0.0f : ex2(mc - (tc + kTtGrow))) : 1.0f;
+              if (grow) mc = tc + kTtGrow;
               l *= f;
               if (mine_units == 0) return;
 #pragma unroll 1

@@ -97,6 +97,24 @@ def test_attention_tiny_scales(cuda, K, dtype, D, scale):
     check_attention(got, want, mass, reach.abs(), dtype, 256)
 
 
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (BF, 256), (F32, 128)])
+@pytest.mark.parametrize("N", [1, 40])
+@pytest.mark.parametrize("up", [3.0, 7.0, 7.9])
+def test_attention_largest_value_behind_a_rising_maximum(cuda, K, dtype, D, N, up):
+    """A key whose weight is 2^up times all that came before it, and with it the
+    type's largest value: no partial product leaves fp32."""
+    c = attn_case(47, 1, N, 4, 1, D, 5000, [4900], dtype)
+    c["scale"] = 1.0
+    c["q"] = torch.zeros_like(c["q"])
+    c["q"][..., 0] = 1.0
+    c["k"][..., 0] = 0.0
+    for t in (300, 1700, 4800):
+        c["k"][:, :, t, 0] = up * 0.6931
+    c["v"][0, 0, 300, 1] = torch.finfo(dtype).max
+    c["v"][0, 0, 300, 2] = -torch.finfo(dtype).max
+    verify_attn(K, c)
+
+
 # ------------------------------------------- arguments at their types' ends --
 def test_whole_numbers_past_32_bits(cuda, K):
     """int64 parents, paths, counts and cache rows that int32 does not hold are
