@@ -487,8 +487,11 @@ int maple_tree_plan(const int32_t* parents, int64_t batch, int64_t nodes, int64_
  * out [batch, nodes, H, D] contiguous; caches [cache_batch, Hkv, max_len, D],
  * (max_len, D) contiguous, cache row row_map[b] (b when NULL).  f32 or bf16,
  * D in {64, 128, 256}, H / Hkv at most 4096; pointers and strides multiples of
- * 16 bytes.  With nodes
- * = 1 and mask 1 this is maple_decode_gqa_attn.  A length or cache row outside
+ * 16 bytes.  Scores, softmax statistics and output sums are f32; bf16 heads of 64
+ * and 128 round the weights to bf16 before the product with V (half a step,
+ * 2^-8, of each), as maple_decode_gqa_attn does, the others do not.  With nodes
+ * = 1 and mask 1 this is maple_decode_gqa_attn to those roundings and the order
+ * of its sums.  A length or cache row outside
  * the cache sets bit 2 of *err (that sequence gets zeros); a bounded wait that
  * gives up sets bit 1.  A row's result depends on no other sequence's length
  * or contents.  The workspace needs no initial value and is free again when

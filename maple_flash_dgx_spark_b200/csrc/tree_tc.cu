@@ -32,11 +32,11 @@
 //
 // Up to 128 rows HBM bounds it: 64 sequences x 8150 with eight nodes (32 heads
 // on 4 of 128), 1.08 GB in 164 us = 6.57 TB/s, what a plain copy reaches; held
-// for seconds the power limit makes it 181.  With more rows the softmax does:
-// 64 nodes x 65440, 68.7 GFLOP in 72 us = 950 TFLOP/s; a warpgroup's loads from
-// tensor memory, exponentials (a thread's 128 per unit at 16 per cycle and SM
-// for four warps) and stores take longer than its two MMAs.  Exponentials by a
-// polynomial on the FMA pipes gave 280 to 316 us for 273 (37 x 8192, 64 nodes),
+// for seconds the power limit makes it 181.  With more rows the chain of a unit
+// does (scores, loads from tensor memory, exponentials, stores, product), of
+// which two run in turn: 64 nodes x 65440, 68.7 GFLOP in 72 us = 950 TFLOP/s; at
+// 1 x 32768 the exponential unit is busy 45 % of the time, the tensor pipe 44 %,
+// the issue slots 32 %, so that no unit is full.  Exponentials by a polynomial on the FMA pipes gave 280 to 316 us for 273 (37 x 8192, 64 nodes),
 // units of 64 keys with their scores a unit ahead 320.
 //
 // Waits are bounded: one that gives up sets the error word; every role then

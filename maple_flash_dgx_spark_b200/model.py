@@ -637,7 +637,10 @@ class MapleForCausalLM:
         :func:`kernels.tree_plan`; the tokens of padding are not looked at) over the first ``B`` slots of ``cache``, or
         its prefill slot.  The nodes' K/V rows go to the slots behind each
         sequence's positions; :meth:`KVCache.commit_tree` keeps those that
-        ``verify_tree`` accepts.  The lengths stay as they are."""
+        ``verify_tree`` accepts.  The lengths stay as they are.  The logits are
+        those of :meth:`forward` over a node's path but for the attention's
+        roundings and order of sums, and always the whole head's (not
+        ``lm_head_flash``'s)."""
         plan = parents if isinstance(parents, TreePlan) else tree_plan(parents)
         bsz, n = plan.mask.shape
         if bsz < 1 or tuple(tokens.shape) != (bsz, n):
