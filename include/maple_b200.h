@@ -464,8 +464,8 @@ int maple_dequantize_rtn(const uint32_t* packed, const float* scales, const floa
  * that was drawn, not yet in the cache.  The nodes' K/V rows stand in the cache
  * behind the sequence's seqlen positions, node j at slot seqlen + j.
  *
- * maple_narrow_int64: out[i] = x[i] as int32, numbers past it as its ends (for
- * parents, paths, counts and cache rows in 64 bits: the ends are none of any).
+ * maple_narrow_int64: out[i] = x[i] as int32, numbers past it as its ends: for
+ * parents, paths, counts and cache rows in 64 bits, none of which is an end.
  *
  * maple_tree_plan: mask[i] = bit i and the bits of node i's ancestors, depth[i]
  * = their number (both [batch, nodes], contiguous; 0 for padding).  parents:

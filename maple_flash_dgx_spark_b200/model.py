@@ -634,13 +634,13 @@ class MapleForCausalLM:
     def forward_tree(self, tokens: torch.Tensor, parents: torch.Tensor | TreePlan, cache: KVCache) -> torch.Tensor:
         """Logits ``[B, N, V]`` of every node of ``B`` trees of drafted tokens
         (``tokens`` and ``parents`` ``[B, N]``, node 0 the last drawn token; see
-        :func:`kernels.tree_plan`; the tokens of padding are not looked at) over the first ``B`` slots of ``cache``, or
-        its prefill slot.  The nodes' K/V rows go to the slots behind each
-        sequence's positions; :meth:`KVCache.commit_tree` keeps those that
-        ``verify_tree`` accepts.  The lengths stay as they are.  The logits are
-        those of :meth:`forward` over a node's path but for the attention's
-        roundings and order of sums, and always the whole head's (not
-        ``lm_head_flash``'s)."""
+        :func:`kernels.tree_plan`; the tokens of padding are not looked at) over
+        the first ``B`` slots of ``cache``, or its prefill slot.  The nodes' K/V
+        rows go to the slots behind each sequence's positions;
+        :meth:`KVCache.commit_tree` keeps those that ``verify_tree`` accepts.  The
+        lengths stay as they are.  The logits are those of :meth:`forward` over a
+        node's path but for the attention's roundings and order of sums, and always
+        the whole head's (not ``lm_head_flash``'s)."""
         plan = parents if isinstance(parents, TreePlan) else tree_plan(parents)
         bsz, n = plan.mask.shape
         if bsz < 1 or tuple(tokens.shape) != (bsz, n):
